@@ -130,6 +130,14 @@ _SIGNATURES = {
     "crane_b200_decode_path": (C.c_int, [C.c_void_p]),
     "crane_b200_prof_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "crane_b200_prof_report": (C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t, C.POINTER(C.c_size_t)]),
+    "crane_b200_fp8_last_error": (C.c_char_p, []),
+    "crane_b200_fp8_quantize": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "crane_b200_fp8_silu_mul": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "crane_b200_fp8_rms_norm": (C.c_int, [C.c_int, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p, C.c_int, C.c_float, C.c_size_t,
+                                          C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "crane_b200_fp8_linear": (C.c_int, [C.c_int, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_size_t, C.c_size_t, C.c_size_t,
+                                        C.c_void_p, C.c_size_t, C.c_void_p, C.c_int, C.c_size_t, C.c_void_p]),
+    "crane_b200_fp8_status": (C.c_int, [C.c_int, C.c_void_p]),
     "crane_b200_op_gemm_epi": (C.c_int, [C.c_int] + [C.c_void_p] * 3 + [C.c_int] * 4 + [C.c_void_p] * 4 + [C.c_float] + [C.c_void_p] * 2),
     "crane_b200_op_gemm": (C.c_int, [C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p,
                                      C.c_void_p, C.c_int]),

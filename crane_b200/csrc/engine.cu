@@ -20,6 +20,7 @@
 
 #include "decode.cuh"
 #include "decode_ll.cuh"
+#include "fp8.cuh"
 #include "host_pool.h"
 #include "gdn.cuh"
 #include "gemm.cuh"
@@ -3080,5 +3081,6 @@ int crane_b200_op_gemm(int device, const uint16_t* a, const uint16_t* a_lo, cons
 }  // extern "C"
 
 #include "engine_tts.inc"
+#include "engine_fp8.inc"
 #include "engine_comm.inc"
 #include "engine_loaders.inc"

@@ -36,6 +36,17 @@ struct TmapKeyHash {
         return h;
     }
 };
+bool tc_tmap_encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols,
+                    CUtensorMapSwizzle swizzle) {
+    PFN_encodeTiled enc = get_encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld * (type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : type == CU_TENSOR_MAP_DATA_TYPE_UINT8 ? 1 : 2)};
+    cuuint32_t box[2] = {box_cols, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 bool tc_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols,
              CUtensorMapSwizzle swizzle) {
     static std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> cache;
@@ -46,16 +57,7 @@ bool tc_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint6
         auto it = cache.find(key);
         if (it != cache.end()) { *map = it->second; return true; }
     }
-    PFN_encodeTiled enc = get_encode_fn();
-    if (!enc) return false;
-    cuuint64_t dims[2] = {cols, rows};
-    cuuint64_t strides[1] = {ld * (type == CU_TENSOR_MAP_DATA_TYPE_FLOAT32 ? 4 : 2)};
-    cuuint32_t box[2] = {box_cols, box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return false;
+    if (!tc_tmap_encode(map, base, type, rows, cols, ld, box_rows, box_cols, swizzle)) return false;
     std::lock_guard<std::mutex> g(mu);
     if (cache.size() > 8192) cache.clear();
     cache.emplace(key, *map);

@@ -108,6 +108,13 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
         ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
 }
+__device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {      // 32 codes of K
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate) : "memory");
+}
 // Arrives on `bar` when every tcgen05.mma issued so far by this thread has completed.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -222,6 +229,8 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw32(uint32_t smem_addr) {
 }
 // A, B = f16 instead of bf16
 __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+// A, B = e4m3 (kind::f8f6f4)
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
 // 128-byte rows: byte offset of the 16-byte piece c of row r
 __device__ __forceinline__ uint32_t sw128_off(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 // 64- and 32-byte rows
@@ -229,8 +238,10 @@ __device__ __forceinline__ uint32_t sw32_off(int r, int c) { return (uint32_t)(r
 __device__ __forceinline__ uint32_t sw64_off(int r, int c) { return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4)); }
 
 // ---- host side (tc.cu) ---------------------------------------------------------------------
-// 2-D row-major [rows, cols] of 16- or 32-bit elements with `ld` elements between rows; box = [box_rows, box_cols].  Encoded maps are cached by
+// 2-D row-major [rows, cols] of 8- (UINT8), 16- or 32-bit elements with `ld` elements between rows; box = [box_rows, box_cols].  tc_tmap caches encoded maps by
 // their defining tuple: encoding costs a few microseconds of host time, as much as a small kernel runs.
+bool tc_tmap_encode(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols,
+                    CUtensorMapSwizzle swizzle);
 bool tc_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols,
              CUtensorMapSwizzle swizzle);
 inline bool tc_tmap_16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_rows, uint32_t box_cols, CUtensorMapSwizzle swizzle) {

@@ -318,6 +318,36 @@ CRANE_B200_API int crane_b200_prof_report(const crane_b200_model* m, char* buf, 
  * 0 = the kernel chain (one graph replay per step: hybrid / quantised / TTS models, batched sequences, borrowed streams). */
 CRANE_B200_API int crane_b200_decode_path(const crane_b200_model* m);
 
+/* ---- linears in 8-bit floating point, on device memory ---------------------------------------------------------- */
+/* What a checkpoint with `quantization_config` {"quant_method": "fp8", "weight_block_size": [128, 128]} runs its projections with, for programs that keep
+ * their tensors on the device themselves: activation rows become e4m3 codes with an f32 scale for every 128 columns, weights are codes with a scale for every 128 x 128.
+ *   block of a row:  a = max(max |y|, 2^-100), scale = a / 448, code = e4m3(y * (448 / a)), to nearest even (a NaN's code is NaN; an infinity makes its block NaN in use)
+ * Every pointer is memory of `device`, `stream` a cudaStream_t of that device (NULL: its default stream); a call enqueues its work there, with no wait and no
+ * copy to the host, and may be captured into a graph.  Inputs and results have to stay while that work runs.  Nothing is kept between calls: several threads may make them at once.
+ * dtype: crane_b200_dtype; a row distance (ld..) counts elements.  Codes: rows start on 16-byte boundaries (base and ld multiples of 16, ld >= columns), any number of
+ * columns.  Scales of rows: block by block, that of row i and block b at scales[b * lds + i], lds >= rows.  m = 0 (or n = 0) does nothing.
+ * Bytes behind a row's last column and rows behind the last are left as they are.
+ * On an error the message is crane_b200_fp8_last_error()'s, the calling thread's own. */
+CRANE_B200_API const char* crane_b200_fp8_last_error(void);
+/* Rows x [m, k] -> codes [m, k] and scales. */
+CRANE_B200_API int crane_b200_fp8_quantize(int device, const void* x, int dtype, size_t ldx, size_t m, size_t k, uint8_t* codes, size_t ld, float* scales, size_t lds,
+                                           void* stream);
+/* Rows gate_up [m, 2 k], gates in the first k columns -> codes and scales of SiLU(gate) * up, computed in f32. */
+CRANE_B200_API int crane_b200_fp8_silu_mul(int device, const void* gate_up, int dtype, size_t ldx, size_t m, size_t k, uint8_t* codes, size_t ld, float* scales, size_t lds,
+                                           void* stream);
+/* h = x + residual, rounded to the residual's type and stored to residual_out (which may be `residual`; both NULL: h = x); codes and scales of
+ * h * rsqrt(mean(h^2) + eps) * weight, computed in f32. */
+CRANE_B200_API int crane_b200_fp8_rms_norm(int device, const void* x, int dtype, size_t ldx, const void* residual, void* residual_out, int res_dtype, size_t ldr,
+                                           const void* weight, int w_dtype, float eps, size_t m, size_t k, uint8_t* codes, size_t ld, float* scales, size_t lds,
+                                           void* stream);
+/* out[i, j] = add[i, j] + sum over blocks b of x_scales[b * lds + i] * w_scales[(j / 128) * ldws + b] * sum over the block's columns of x[i, :] w[j, :].
+ * w [n, k] codes, w_scales [ceil(n / 128), ceil(k / 128)].  Sums in f32, rounded once to out's type; `add` (NULL: nothing) has that type and may be `out`. */
+CRANE_B200_API int crane_b200_fp8_linear(int device, const uint8_t* x, size_t ldx, const float* x_scales, size_t lds, const uint8_t* w, size_t ldw, const float* w_scales,
+                                         size_t ldws, size_t m, size_t n, size_t k, const void* add, size_t ldadd, void* out, int dtype, size_t ldo, void* stream);
+/* Waits for `stream`; CRANE_B200_CUDA_ERROR when its work failed, or when a linear's bounded wait ran out on the GPU since the last such call (its results are
+ * worth nothing then). */
+CRANE_B200_API int crane_b200_fp8_status(int device, void* stream);
+
 /* ---- kernel-level test hooks (used by tests/ only; host buffers in, host buffers out) ------------ */
 /* C[M,N] = epilogue((A + A_lo)[M,K] bf16 x W[N,K]^T bf16); a_lo = optional low-order plane of a split-precision A
  * (NULL: plain bf16); mode = cb::GemmEpiMode; out dtype follows the mode. */

@@ -114,6 +114,12 @@ extern "C" {
     pub fn crane_b200_prof_enable(m: *mut crane_b200_model, on: c_int) -> c_int;
     pub fn crane_b200_prof_report(m: *const crane_b200_model, buf: *mut c_char, cap: usize, needed: *mut usize) -> c_int;
     pub fn crane_b200_decode_path(m: *const crane_b200_model) -> c_int;
+    pub fn crane_b200_fp8_last_error() -> *const c_char;
+    pub fn crane_b200_fp8_quantize(device: c_int, x: *const c_void, dtype: c_int, ldx: usize, m: usize, k: usize, codes: *mut u8, ld: usize, scales: *mut f32, lds: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_fp8_silu_mul(device: c_int, gate_up: *const c_void, dtype: c_int, ldx: usize, m: usize, k: usize, codes: *mut u8, ld: usize, scales: *mut f32, lds: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_fp8_rms_norm(device: c_int, x: *const c_void, dtype: c_int, ldx: usize, residual: *const c_void, residual_out: *mut c_void, res_dtype: c_int, ldr: usize, weight: *const c_void, w_dtype: c_int, eps: f32, m: usize, k: usize, codes: *mut u8, ld: usize, scales: *mut f32, lds: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_fp8_linear(device: c_int, x: *const u8, ldx: usize, x_scales: *const f32, lds: usize, w: *const u8, ldw: usize, w_scales: *const f32, ldws: usize, m: usize, n: usize, k: usize, add: *const c_void, ldadd: usize, out: *mut c_void, dtype: c_int, ldo: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_fp8_status(device: c_int, stream: *mut c_void) -> c_int;
     pub fn crane_b200_op_gemm(device: c_int, a: *const u16, a_lo: *const u16, w: *const u16, M: c_int, N: c_int, K: c_int, mode: c_int, bias: *const f32, out_inout: *mut c_void, use_simt: c_int) -> c_int;
     pub fn crane_b200_op_gemm_epi(device: c_int, a: *const u16, a_lo: *const u16, w: *const u16, M: c_int, N: c_int, K: c_int, mode: c_int, bias: *const f32, col_scale: *const f32, gate: *const f32, gate_bias: *const f32, glu_limit: f32, out_inout: *mut c_void, out_lo: *mut u16) -> c_int;
     pub fn crane_b200_op_qlinear(device: c_int, x: *const f32, m: usize, k: usize, raw: *const c_void, raw_bytes: usize, ggml_type: c_int, n: usize, norm_w: *const f32, eps: f32, y: *mut f32) -> c_int;
