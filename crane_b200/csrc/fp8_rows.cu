@@ -6,11 +6,15 @@
 // finite (an empty block: codes 0).  The two divisions are f32, rounded to nearest; the code is the one rounding to 8 bits, to nearest even.  A NaN's code is NaN; an
 // infinite magnitude makes its block's scale infinite and the block NaN wherever it is used.
 //
-// These kernels are bound by the bytes of the rows: one pass, a thread has 8 neighbouring columns (16 or 32 bytes in, 8 out) and 16 threads a block of 128, whose
-// maximum takes four shuffles.
+// These kernels are bound by the bytes of the rows, and next to them by instructions: one pass, a thread has 16 columns, 8 threads a block of 128, whose maximum takes three
+// shuffles and whose two divisions are made eight times, not sixteen; as many blocks as the chip runs at once take rows in turn, with the next ones' loads on their way.
 #include "fp8.cuh"
 
 #include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 namespace cb {
 
@@ -55,172 +59,314 @@ __device__ __forceinline__ void f8_load8(const void* base, int type, long long a
     else if (type == F8_BF16) f8_load8(static_cast<const bf16*>(base) + at, c, K, vec, v);
     else f8_load8(static_cast<const __half*>(base) + at, c, K, vec, v);
 }
+// What a chunk brings, as it is loaded: to be asked for well ahead of its use, it must not be unpacked where it is loaded.  VEC: every chunk is whole and on its boundary.
+template <typename T, bool VEC> struct F8Chunk {
+    uint4 q[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* row, int c, int, bool in) {
+        q[0] = in ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
+        if constexpr (sizeof(T) == 4) q[1] = in ? *reinterpret_cast<const uint4*>(row + c + 4) : make_uint4(0, 0, 0, 0);
+        else static_assert(sizeof(q) == 16, "one piece");
+    }
+    __device__ __forceinline__ void get(float* v) const {
+        if constexpr (sizeof(T) == 4) {
+            v[0] = __uint_as_float(q[0].x); v[1] = __uint_as_float(q[0].y); v[2] = __uint_as_float(q[0].z); v[3] = __uint_as_float(q[0].w);
+            v[4] = __uint_as_float(q[1].x); v[5] = __uint_as_float(q[1].y); v[6] = __uint_as_float(q[1].z); v[7] = __uint_as_float(q[1].w);
+        } else f8_unpack(q[0], T(), v);
+    }
+};
+template <typename T> struct F8Chunk<T, false> {
+    T q[8];
+    __device__ __forceinline__ void load(const T* row, int c, int K, bool) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = c + i < K ? row[c + i] : T(0.f);
+    }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = f8_float(q[i]);
+    }
+};
 // h = v rounded to the type, stored and given back in f32
-template <typename T>
-__device__ __forceinline__ void f8_store8(T* row, int c, int K, bool vec, float* v) {
-    if constexpr (sizeof(T) == 4) {
-        if (vec && c + 8 <= K) {
-            *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
+template <typename T, bool VEC>
+__device__ __forceinline__ void f8_store8(T* row, int c, int K, float* v) {
+    alignas(16) T h[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) if (c + i < K) row[c + i] = v[i];
-        }
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (std::is_same<T, float>::value) h[i] = v[i];
+        else if constexpr (std::is_same<T, bf16>::value) h[i] = __float2bfloat16_rn(v[i]);
+        else h[i] = __float2half_rn(v[i]);
+        v[i] = f8_float(h[i]);
+    }
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(h)[i];
     } else {
-        T h[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if constexpr (std::is_same<T, bf16>::value) h[i] = __float2bfloat16_rn(v[i]); else h[i] = __float2half_rn(v[i]);
-            v[i] = f8_float(h[i]);
-        }
-        if (vec && c + 8 <= K) *reinterpret_cast<uint4*>(row + c) = *reinterpret_cast<const uint4*>(h);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) if (c + i < K) row[c + i] = h[i];
-        }
+        for (int i = 0; i < 8; ++i) if (c + i < K) row[c + i] = h[i];
     }
 }
-__device__ __forceinline__ void f8_store8(void* base, int type, long long at, int c, int K, bool vec, float* v) {
-    if (type == F8_F32) f8_store8(static_cast<float*>(base) + at, c, K, vec, v);
-    else if (type == F8_BF16) f8_store8(static_cast<bf16*>(base) + at, c, K, vec, v);
-    else f8_store8(static_cast<__half*>(base) + at, c, K, vec, v);
-}
 
-__device__ __forceinline__ uint32_t f8_pair(float a, float b) {      // a in the low byte
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
+__device__ __forceinline__ uint32_t f8_quad(float a, float b, float c, float d) {      // a in the low byte
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
-// The block of 16 neighbouring threads (a half warp): scale and codes.  Every lane of the warp calls; `in`: this thread's columns c .. exist
-__device__ __forceinline__ void f8_emit(const float* v, long long m, int c, int K, bool in, const F8Out& o) {
+// A thread has 16 columns of a block of 128, 8 from 8 (lane % 8) on and 8 from 64 behind those, 8 neighbouring threads the block.
+__device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
+// Scale and codes of it.  Every lane of the warp calls
+template <bool VEC>
+__device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c, int K, bool row_in, const F8Out& o) {
     float a = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[i]));
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int s = 8; s > 0; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
+        for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[h][i]));
+#pragma unroll
+    for (int s = 4; s > 0; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
     a = fmaxf(a, F8_TINY);
     const float inv = __fdiv_rn(F8_TOP, a);
-    if (!in) return;
+    if (!row_in || c >= K) return;
     if ((c & (F8_BLOCK - 1)) == 0) o.scales[(c / F8_BLOCK) * o.lds + m] = __fdiv_rn(a, F8_TOP);
-    const uint32_t lo = f8_pair(v[0] * inv, v[1] * inv) | f8_pair(v[2] * inv, v[3] * inv) << 16, hi = f8_pair(v[4] * inv, v[5] * inv) | f8_pair(v[6] * inv, v[7] * inv) << 16;
     unsigned char* p = o.codes + m * o.ld + c;
-    if (c + 8 <= K) *reinterpret_cast<uint2*>(p) = make_uint2(lo, hi);
-    else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (c + i < K) p[i] = (unsigned char)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t lo = f8_quad(v[h][0] * inv, v[h][1] * inv, v[h][2] * inv, v[h][3] * inv), hi = f8_quad(v[h][4] * inv, v[h][5] * inv, v[h][6] * inv, v[h][7] * inv);
+        const int at = c + 64 * h;
+        if (VEC ? at < K : at + 8 <= K) *reinterpret_cast<uint2*>(p + 64 * h) = make_uint2(lo, hi);
+        else if (!VEC) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (at + i < K) p[64 * h + i] = (unsigned char)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+        }
     }
 }
 
-template <typename T, bool GATED>
+// SiLU(g) u: with z = exp(-|g|), which neither overflows nor cancels, (g or g z) / (1 + z) u.  The quotient by rcp.approx (1 + z lies in [1, 2]) and one step of Newton's: half of
+// the instructions of a division, whose form took 166 us where the bytes (8192 x 2 x 12288 bf16) take 78.
+__device__ __forceinline__ float f8_silu_mul(float g, float u) {
+    const float z = expf(-fabsf(g)), d = 1.f + z, n = g < 0.f ? g * z : g;
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    const float q = n * r;
+    return fmaf(fmaf(-q, d, n), r, q) * u;
+}
+
+// A warp takes 512 columns of a row (four blocks) at a time and asks for U such pieces before it works on the first.
+template <typename T, bool GATED, bool VEC, int U>
 __global__ void __launch_bounds__(256)
-f8_rows_kernel(const T* __restrict__ x, long long ldx, long long M, int K, int KB, bool vec, F8Out o) {
+f8_rows_kernel(const T* __restrict__ x, long long ldx, long long M, int K, F8Out o) {
+    const int c0 = f8_col(threadIdx.x & 31), per = (K + 511) / 512;
+    const unsigned warps = gridDim.x * 8, w = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int dm = (int)(warps / per), dc = (int)(warps % per);             // a step of all warps: rows and pieces
+    long long m = w / per;
+    int piece = (int)(w % per);
     pdl_wait();
     pdl_launch_dependents();
-    const long long g = (long long)blockIdx.x * 16 + (threadIdx.x >> 4), m = g / KB;
-    const int c = (int)(g - m * KB) * F8_BLOCK + (threadIdx.x & 15) * 8;
-    const bool in = m < M && c < K;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (in) {
-        const T* row = x + m * ldx;
-        f8_load8(row, c, K, vec, v);
-        if constexpr (GATED) {
-            float u[8];
-            f8_load8(row + K, c, K, vec, u);
+    while (m < M) {
+        F8Chunk<T, VEC> v[U][2], g[GATED ? U : 1][2];
+        long long row[U];
+        int col[U];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = silu_f(v[i]) * u[i];
+        for (int u = 0; u < U; ++u) {
+            row[u] = m; col[u] = piece * 512 + c0;
+            const T* at = x + (m < M ? m : 0) * ldx;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = col[u] + 64 * h;
+                const bool in = m < M && c < K;
+                if constexpr (GATED) g[u][h].load(at, in ? c : 0, K, in);
+                v[u][h].load(at + (GATED ? K : 0), in ? c : 0, K, in);
+            }
+            m += dm; piece += dc;
+            if (piece >= per) { piece -= per; ++m; }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (row[u] >= M) break;                                          // (the warp as one)
+            float y[2][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                v[u][h].get(y[h]);
+                if constexpr (GATED) {
+                    float gate[8];
+                    g[u][h].get(gate);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[h][i] = f8_silu_mul(gate[i], y[h][i]);
+                }
+                if (!VEC && col[u] + 64 * h >= K) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[h][i] = 0.f;
+                }
+            }
+            f8_emit<VEC>(y, row[u], col[u], K, true, o);
         }
     }
-    f8_emit(v, m, c, K, in, o);
 }
 
-struct F8NormArgs { F8Norm n; long long M; int K, tpr; bool vec_x, vec_r, vec_w; F8Out o; };
-// `tpr` threads have a row (a block several, where it has fewer columns than 8 x 256), J chunks of 8 columns each, in registers between the sum and the codes; J = 0: any
-// number, read again for the codes (what the thread itself stored, where there is a residual).
-template <typename T, int J>
-__global__ void __launch_bounds__(1024)
+struct F8NormArgs { F8Norm n; long long M; int K, tpr; bool vec_w; F8Out o; };
+// `tpr` threads have a row (a block several, where it has fewer columns than 16 x 256), PER times 16 columns each, in registers between the sum and the codes; PER = 0: wider rows,
+// read again for the codes (what the thread itself stored, where there is a residual).  A block keeps its weights in registers over the rows it takes in turn, and asks for the
+// next row before it finishes one.
+template <typename T, typename R, bool VEC, int PER>
+__global__ void __launch_bounds__(512)
 f8_norm_kernel(const F8NormArgs a) {
-    __shared__ float red[32];
-    const int t = threadIdx.x & (a.tpr - 1), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K;
-    const long long m = (long long)blockIdx.x * (blockDim.x / a.tpr) + threadIdx.x / a.tpr;
-    const bool row_in = m < a.M;
-    const T* xr = static_cast<const T*>(a.n.x) + m * a.n.ldx;
-    auto first = [&](int c, float* v) {                 // h of a chunk, stored where there is a residual
-        if (!(row_in && c < K)) {
+    constexpr bool RES = !std::is_same<R, void>::value;
+    using RT = typename std::conditional<RES, R, T>::type;
+    __shared__ float red[2][16];
+    const int t = threadIdx.x & (a.tpr - 1), sub = threadIdx.x / a.tpr, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K, rpb = blockDim.x / a.tpr;
+    const T* x = static_cast<const T*>(a.n.x);
+    const RT* res = static_cast<const RT*>(a.n.residual);
+    RT* res_out = static_cast<RT*>(a.n.residual_out);
+    struct Piece { F8Chunk<T, VEC> x[2]; F8Chunk<RT, VEC> r[2]; };
+    auto load = [&](long long m, int c0, Piece& p) {
+        const long long at = m < a.M ? m : 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-            return;
-        }
-        f8_load8(xr, c, K, a.vec_x, v);
-        if (a.n.residual) {
-            float r[8];
-            f8_load8(a.n.residual, a.n.res_type, m * a.n.ldr, c, K, a.vec_r, r);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] += r[i];
-            f8_store8(a.n.residual_out, a.n.res_type, m * a.n.ldr, c, K, a.vec_r, v);
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + 64 * h;
+            const bool in = m < a.M && c < K;
+            p.x[h].load(x + at * a.n.ldx, in ? c : 0, K, in);
+            if constexpr (RES) p.r[h].load(res + at * a.n.ldr, in ? c : 0, K, in);
         }
     };
-    auto finish = [&](int c, float* v, float rstd) {
-        const bool in = row_in && c < K;
-        if (in) {
-            float w[8];
-            f8_load8(a.n.w, a.n.w_type, 0, c, K, a.vec_w, w);
+    auto sum = [&](long long m, int c0, const Piece& p, float (*v)[8]) {       // h of 16 columns, stored where there is a residual -> their squares
+        float s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * rstd * w[i];
+        for (int h = 0; h < 2; ++h) {
+            const int c = c0 + 64 * h;
+            const bool in = m < a.M && c < K;
+            p.x[h].get(v[h]);
+            if constexpr (RES) {
+                float r[8];
+                p.r[h].get(r);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[h][i] += r[i];
+                if (in) f8_store8<RT, VEC>(res_out + m * a.n.ldr, c, K, v[h]);
+            }
+            if (!VEC && !in) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[h][i] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[h][i] * v[h][i];
         }
-        f8_emit(v, m, c, K, in, a.o);
+        return s;
     };
-    auto row_rstd = [&](float s) {
+    auto row_rstd = [&](float s, int turn) {
         s = warp_sum(s);
         if (a.tpr > 32) {
             const int nw = a.tpr >> 5, w0 = warp & ~(nw - 1);
-            if (lane == 0) red[warp] = s;
-            __syncthreads();
-            s = warp_sum(lane < nw ? red[w0 + lane] : 0.f);
+            if (lane == 0) red[turn & 1][warp] = s;
+            __syncthreads();                        // (the other half of `red` is the next row's: nobody is still reading it)
+            s = warp_sum(lane < nw ? red[turn & 1][w0 + lane] : 0.f);
         }
         return rsqrtf(s / (float)K + a.n.eps);
     };
+    auto weights = [&](int c0, float (*w)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (c0 + 64 * h < K) f8_load8(a.n.w, a.n.w_type, 0, c0 + 64 * h, K, a.vec_w, w[h]);
+            else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[h][i] = 0.f;
+            }
+        }
+    };
+    const long long step = (long long)gridDim.x * rpb;
+    long long base = (long long)blockIdx.x * rpb;
+    const int c0 = f8_col(t);
+    int turn = 0;
     pdl_wait();
     pdl_launch_dependents();
-    float s = 0.f;
-    if constexpr (J > 0) {
-        float v[J][8];
+    if constexpr (PER > 0) {
+        float w[PER][2][8];
+        Piece p[PER];
 #pragma unroll
-        for (int j = 0; j < J; ++j) first((t + j * a.tpr) * 8, v[j]);
+        for (int j = 0; j < PER; ++j) load(base + sub, c0 + j * a.tpr * 16, p[j]);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < PER; ++j) weights(c0 + j * a.tpr * 16, w[j]);
+        for (; base < a.M; base += step, ++turn) {
+            const long long m = base + sub;
+            float v[PER][2][8], s = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[j][i] * v[j][i];
-        const float rstd = row_rstd(s);
+            for (int j = 0; j < PER; ++j) s += sum(m, c0 + j * a.tpr * 16, p[j], v[j]);
+            if (base + step < a.M) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) finish((t + j * a.tpr) * 8, v[j], rstd);
-    } else {
-        for (int c = t * 8; c < K; c += a.tpr * 8) {
-            float v[8];
-            first(c, v);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i] * v[i];
-        }
-        const float rstd = row_rstd(s);
-        for (int c = t * 8; c < (K + 255) / 256 * 256; c += a.tpr * 8) {        // (a warp's threads leave the loop together)
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (row_in && c < K) {
-                if (a.n.residual) f8_load8(a.n.residual_out, a.n.res_type, m * a.n.ldr, c, K, a.vec_r, v);
-                else f8_load8(xr, c, K, a.vec_x, v);
+                for (int j = 0; j < PER; ++j) load(m + step, c0 + j * a.tpr * 16, p[j]);
             }
-            finish(c, v, rstd);
+            const float rstd = row_rstd(s, turn);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[j][h][i] = v[j][h][i] * rstd * w[j][h][i];
+                f8_emit<VEC>(v[j], m, c0 + j * a.tpr * 16, K, m < a.M, a.o);
+            }
+        }
+    } else {
+        for (; base < a.M; base += step, ++turn) {
+            const long long m = base + sub;
+            float s = 0.f;
+            for (int c = c0; c < K; c += a.tpr * 16) {
+                Piece p;
+                float v[2][8];
+                load(m, c, p);
+                s += sum(m, c, p, v);
+            }
+            const float rstd = row_rstd(s, turn);
+            for (int i0 = 0; i0 < K; i0 += a.tpr * 16) {        // (all threads alike: shuffles)
+                const int c = i0 + c0;
+                float v[2][8], w[2][8];
+                weights(c, w);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const bool in = m < a.M && c + 64 * h < K;
+                    if constexpr (RES) {
+                        F8Chunk<RT, VEC> q;
+                        q.load(static_cast<const RT*>(res_out) + (in ? m : 0) * a.n.ldr, in ? c + 64 * h : 0, K, in);
+                        q.get(v[h]);
+                    } else {
+                        F8Chunk<T, VEC> q;
+                        q.load(x + (in ? m : 0) * a.n.ldx, in ? c + 64 * h : 0, K, in);
+                        q.get(v[h]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * rstd * w[h][i] : 0.f;
+                }
+                f8_emit<VEC>(v, m, c, K, m < a.M, a.o);
+            }
         }
     }
 }
 
 static bool f8_aligned(const void* p, long long ld, int type) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * f8_bytes(type)) % 16 == 0; }
+// blocks of a kernel that the current device runs at once
+template <typename F>
+static int f8_resident(F kernel, int threads, std::atomic<int>* known) {
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= CB_MAX_DEV) return 148;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        int sms = 0;
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+            cudaGetLastError();
+            return 148;
+        }
+        n = n > 0 ? n * sms : sms;
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 
+template <typename T, bool GATED, bool VEC>
+static int f8_rows_v(cudaStream_t st, const void* x, long long ldx, long long M, int K, const F8Out& out, bool pdl) {
+    constexpr int U = VEC && !GATED ? 2 : 1;
+    static std::atomic<int> known[CB_MAX_DEV];
+    const long long pieces = M * ((K + 511) / 512);
+    const long long blocks = std::min<long long>((pieces + 7) / 8, f8_resident(f8_rows_kernel<T, GATED, VEC, U>, 256, known));
+    return launch_k(f8_rows_kernel<T, GATED, VEC, U>, dim3((unsigned)blocks), dim3(256), 0, st, pdl, static_cast<const T*>(x), ldx, M, K, out);
+}
 template <typename T, bool GATED>
 static int f8_rows_t(cudaStream_t st, const void* x, int type, long long ldx, long long M, int K, const F8Out& out, bool pdl) {
-    const int KB = f8_blocks(K);
-    const long long blocks = (M * KB + 15) / 16;
-    if (blocks > 0x7fffffffLL) return -1000;
-    const bool vec = f8_aligned(x, ldx, type) && (!GATED || (long long)K * f8_bytes(type) % 16 == 0);
-    return launch_k(f8_rows_kernel<T, GATED>, dim3((unsigned)blocks), dim3(256), 0, st, pdl, static_cast<const T*>(x), ldx, M, K, KB, vec, out);
+    return f8_aligned(x, ldx, type) && K % 8 == 0 ? f8_rows_v<T, GATED, true>(st, x, ldx, M, K, out, pdl) : f8_rows_v<T, GATED, false>(st, x, ldx, M, K, out, pdl);
 }
 template <bool GATED>
 static int f8_rows_launch(cudaStream_t st, const void* x, int type, long long ldx, long long M, int K, const F8Out& out, bool pdl) {
@@ -239,22 +385,41 @@ int f8_silu_mul_launch(cudaStream_t st, const void* x, int type, long long ldx, 
     return f8_rows_launch<true>(st, x, type, ldx, M, K, out, pdl);
 }
 
+template <typename T, typename R, bool VEC, int PER>
+static int f8_norm_p(cudaStream_t st, const F8NormArgs& a, int block, bool pdl) {
+    static std::atomic<int> known[2][CB_MAX_DEV];               // by the block's size
+    const int rows = block / a.tpr;
+    const long long blocks = std::min<long long>((a.M + rows - 1) / rows, f8_resident(f8_norm_kernel<T, R, VEC, PER>, block, known[block > 256]));
+    return launch_k(f8_norm_kernel<T, R, VEC, PER>, dim3((unsigned)blocks), dim3(block), 0, st, pdl, a);
+}
+template <typename T, typename R, bool VEC>
+static int f8_norm_v(cudaStream_t st, F8NormArgs& a, bool pdl) {
+    a.tpr = 32;
+    while (a.tpr < 512 && a.tpr * 16 < (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK) a.tpr *= 2;
+    const int block = a.tpr < 256 ? 256 : a.tpr;
+    if (a.K <= a.tpr * 16) return f8_norm_p<T, R, VEC, 1>(st, a, block, pdl);
+    if (VEC && a.K <= a.tpr * 32) return f8_norm_p<T, R, VEC, VEC ? 2 : 0>(st, a, block, pdl);
+    return f8_norm_p<T, R, VEC, 0>(st, a, block, pdl);
+}
+template <typename T, typename R>
+static int f8_norm_r(cudaStream_t st, F8NormArgs& a, bool pdl) {
+    const F8Norm& n = a.n;
+    const bool vec = a.K % 8 == 0 && f8_aligned(n.x, n.ldx, n.type) && (!n.residual || (f8_aligned(n.residual, n.ldr, n.res_type) && f8_aligned(n.residual_out, n.ldr, n.res_type)));
+    return vec ? f8_norm_v<T, R, true>(st, a, pdl) : f8_norm_v<T, R, false>(st, a, pdl);
+}
 template <typename T>
 static int f8_norm_t(cudaStream_t st, F8NormArgs& a, bool pdl) {
-    const int chunks = (a.K + 7) / 8;
-    a.tpr = 32;
-    while (a.tpr < 1024 && a.tpr < chunks) a.tpr *= 2;
-    const int block = a.tpr < 256 ? 256 : a.tpr, rows = block / a.tpr;
-    const long long blocks = (a.M + rows - 1) / rows;
-    if (blocks > 0x7fffffffLL) return -1000;
-    if (chunks <= a.tpr) return launch_k(f8_norm_kernel<T, 1>, dim3((unsigned)blocks), dim3(block), 0, st, pdl, a);
-    if (chunks <= 2 * a.tpr) return launch_k(f8_norm_kernel<T, 2>, dim3((unsigned)blocks), dim3(block), 0, st, pdl, a);
-    return launch_k(f8_norm_kernel<T, 0>, dim3((unsigned)blocks), dim3(block), 0, st, pdl, a);
+    if (!a.n.residual) return f8_norm_r<T, void>(st, a, pdl);
+    switch (a.n.res_type) {
+        case F8_F32:  return f8_norm_r<T, float>(st, a, pdl);
+        case F8_BF16: return f8_norm_r<T, bf16>(st, a, pdl);
+        case F8_F16:  return f8_norm_r<T, __half>(st, a, pdl);
+        default: return -1000;
+    }
 }
 int f8_rms_norm_launch(cudaStream_t st, const F8Norm& n, long long M, int K, const F8Out& out, bool pdl) {
     if (M == 0) return 0;
-    F8NormArgs a = {n, M, K, 0, f8_aligned(n.x, n.ldx, n.type), n.residual && f8_aligned(n.residual, n.ldr, n.res_type) && f8_aligned(n.residual_out, n.ldr, n.res_type),
-                    f8_aligned(n.w, 0, n.w_type), out};
+    F8NormArgs a = {n, M, K, 0, f8_aligned(n.w, 0, n.w_type), out};
     switch (n.type) {
         case F8_F32:  return f8_norm_t<float>(st, a, pdl);
         case F8_BF16: return f8_norm_t<bf16>(st, a, pdl);
