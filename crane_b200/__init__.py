@@ -22,7 +22,7 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libcrane_b200.so")
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, F8_E4M3 = 0, 1, 2, 3
 OK, INVALID_ARG, OOM, CUDA_ERROR, UNSUPPORTED, NOT_LOADED = 0, -1, -2, -3, -4, -5
 
 # cb::GemmEpiMode (crane_b200/csrc/gemm.cuh)
@@ -245,7 +245,7 @@ class Engine:
 
     # ---- weights ----
     def load_tensor(self, name: str, arr: np.ndarray):
-        """f32 arrays are rounded to bf16 for the matrices; uint16 arrays are taken as bf16 bit patterns."""
+        """f32 arrays are rounded to bf16 for the matrices; uint16 arrays are taken as bf16 bit patterns, uint8 arrays as the e4m3 codes of an fp8 checkpoint."""
         a = np.ascontiguousarray(arr)
         if a.dtype == np.float32:
             dt = F32
@@ -253,6 +253,8 @@ class Engine:
             dt = BF16
         elif a.dtype == np.float16:
             dt = F16
+        elif a.dtype == np.uint8:
+            dt = F8_E4M3
         else:
             raise TypeError(f"{name}: unsupported dtype {a.dtype}")
         shape = (C.c_int64 * a.ndim)(*a.shape)

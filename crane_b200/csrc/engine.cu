@@ -173,6 +173,10 @@ struct LayerW {
     // GGUF-quantised linears (ggml bytes repacked by q_repack_rows): qt_* == 0 means the bf16 buffer above is used
     unsigned char *q_wq = nullptr, *q_wk = nullptr, *q_wv = nullptr, *q_wo = nullptr, *q_wgu = nullptr, *q_wdown = nullptr;
     int qt_q = 0, qt_k = 0, qt_v = 0, qt_o = 0, qt_gu = 0, qt_down = 0, qt_gate_seen = 0, qt_up_seen = 0;
+    // e4m3 linears of an fp8 checkpoint (fp8.cuh): codes, and a scale for each 128 x 128.  f8: a bit for each projection's codes, the bits of `loaded`, and one 7 further up for its scales
+    unsigned char *f8_qkv = nullptr, *f8_o = nullptr, *f8_gu = nullptr, *f8_down = nullptr;       // q|k|v rows, and gate rows ahead of up rows (not interleaved: a scale is 128 rows')
+    float *f8s_qkv = nullptr, *f8s_o = nullptr, *f8s_gu = nullptr, *f8s_down = nullptr;
+    int f8 = 0;
     // Gated-Delta-Net layers (Qwen3.5 `linear_attn.*`)
     bool full = true;                       // softmax-attention layer (else GDN)
     bf16 *w_in = nullptr, *w_out = nullptr; // [in_pad, H] rows = q|k|v|z|b|a ; [H, value_dim]
@@ -263,6 +267,16 @@ struct crane_b200_model {
     int qt_lm = 0;
     unsigned char* q_embed = nullptr;     // quantised embedding table: rows are dequantised as they are gathered (modules/embedding.rs:31-105)
     int qt_embed = 0;
+    // fp8 checkpoints (config.json quantization_config fp8, blocks of 128 x 128): rows as codes, their scales, and the gate / up rows ahead of the gated unit
+    struct F8Rooms { unsigned char* codes = nullptr; float *scales = nullptr, *gu = nullptr; int rows = 0; };
+    bool fp8 = false, any_f8 = false;
+    F8Rooms f8_dec, f8_pre;
+    bool load_f8(LayerW& l, const std::string& n, const std::string& t, int dt, const int64_t* shape, int ndim, const void* data);
+    F8Rooms f8_rooms(int rows);
+    void f8_linear(const F8Rooms& r, const unsigned char* w, const float* ws, int N, int K, const float* add, float* y, int rows);
+    void f8_qkv(const LayerW& l, const F8Rooms& r, const float* xin, float* y, int rows);            // y = W_qkv norm(x)
+    void f8_o(const LayerW& l, const F8Rooms& r, const float* a, float* xio, int rows);              // x += W_o a
+    void f8_mlp(const LayerW& l, const F8Rooms& r, float* xio, int rows);                            // x += W_down(SiLU(W_gate norm(x)) * W_up norm(x))
     void embed_step_input(int B);         // x_dec <- embedding rows of state[b].token
     bool any_quant = false;
     float* final_norm = nullptr;
@@ -560,6 +574,14 @@ void crane_b200_model::parse_config(const char* json) {
             fail(CRANE_B200_UNSUPPORTED, "Gated-Delta-Net geometry key_head_dim=%d (64, 128 or 256) value_head_dim=%d (multiple of 32) key_heads=%d value_heads=%d (multiple of key_heads, <= 256) conv_kernel=%d (1..8)", dk, dv, nk, nv, ck);
         if (rot_half < 32 || rot_half % 32) fail(CRANE_B200_UNSUPPORTED, "rotary width %d", 2 * rot_half);
     }
+    const cbjson::Value* qc = root.has("quantization_config") ? &root.at("quantization_config") : tc.has("quantization_config") ? &tc.at("quantization_config") : nullptr;
+    if (qc && qc->type == cbjson::Value::OBJ && qc->string("quant_method", "") == "fp8" && !hybrid && !is_tts) {
+        bool blocks = qc->has("weight_block_size") && qc->at("weight_block_size").arr.size() == 2;
+        if (blocks) for (const auto& v : qc->at("weight_block_size").arr) blocks = blocks && v.num == 128;
+        if (!blocks || qc->string("fmt", "e4m3") != "e4m3" || qc->string("activation_scheme", "dynamic") != "dynamic")
+            fail(CRANE_B200_UNSUPPORTED, "quantization_config: fp8 is e4m3 with weight_block_size [128, 128] and activation_scheme \"dynamic\" here");
+        fp8 = true;
+    }
     layer_is_full.assign(L, 1);
     if (hybrid) {
         for (int i = 0; i < L; ++i) layer_is_full[i] = ((i + 1) % full_interval == 0) ? 1 : 0;
@@ -739,6 +761,7 @@ bool crane_b200_model::load_text_tensor(const std::string& n, int dt, const int6
     const std::string t = n.substr(dot + 1);
     LayerW& l = layers[li];
     const int qd = q_dim(), kvd = nkv * D, qs = nh * q_stride();
+    if (dt == CRANE_B200_F8_E4M3 || (fp8 && t.size() > 17 && t.compare(t.size() - 17, 17, ".weight_scale_inv") == 0)) return load_f8(l, n, t, dt, shape, ndim, data);
     auto rows_bf16 = [&](bf16* dst, int rows, int cols) { up_bf16(dst, data, dt, (size_t)rows * cols); };
     if (l.full && !l.wqkv && (t == "self_attn.q_proj.weight" || t == "self_attn.k_proj.weight" || t == "self_attn.v_proj.weight"))
         l.wqkv = dalloc<bf16>((size_t)qkv_dim() * H);
@@ -890,7 +913,11 @@ void crane_b200_model::load_tensor(const std::string& name_in, int dt, const int
     struct Flag { bool& f; ~Flag() { f = false; } } flag_reset{tensor_gguf_named};
     tensor_gguf_named = name != name_in;
     if (finalized) fail(CRANE_B200_INVALID_ARG, "load_tensor after finalize");
-    if (dt < 0 || dt > 2) fail(CRANE_B200_INVALID_ARG, "tensor %s: unknown dtype %d", name.c_str(), dt);
+    if (dt == CRANE_B200_F8_E4M3) {          // (load_f8 takes the projections of the text layers alone)
+        if (!fp8) fail(CRANE_B200_UNSUPPORTED, "tensor %s: e4m3 codes, but config.json has no quantization_config of quant_method fp8 that this model can use", name.c_str());
+        const size_t at = name.find("layers.");
+        if (at == std::string::npos || name.find("visual.") != std::string::npos) fail(CRANE_B200_UNSUPPORTED, "tensor %s: e4m3 codes are the text layers' projections only", name.c_str());
+    } else if (dt < 0 || dt > 2) fail(CRANE_B200_INVALID_ARG, "tensor %s: unknown dtype %d", name.c_str(), dt);
     CUDA_OK(cudaSetDevice(device));
     static const char* vis_prefix[] = {"model.visual.", "visual."};
     for (const char* p : vis_prefix)
@@ -1105,6 +1132,71 @@ void crane_b200_model::qkv_rows(const LayerW& l, unsigned char* buf, int cap, co
 }
 
 // =================================================================================================
+// fp8 checkpoints: e4m3 projections with a scale for each 128 x 128 (`*.weight`, `*.weight_scale_inv`), activation rows as codes with a scale for each 128 columns (fp8.cuh)
+// =================================================================================================
+bool crane_b200_model::load_f8(LayerW& l, const std::string& n, const std::string& t, int dt, const int64_t* shape, int ndim, const void* data) {
+    const int qd = q_dim(), kvd = nkv * D, qkvd = qd + 2 * kvd;
+    const struct { const char* name; int bit; unsigned char*& w; float*& s; int rows, all, at, cols; } p[] = {
+        {"self_attn.q_proj", 1, l.f8_qkv, l.f8s_qkv, qd, qkvd, 0, H}, {"self_attn.k_proj", 2, l.f8_qkv, l.f8s_qkv, kvd, qkvd, qd, H},
+        {"self_attn.v_proj", 4, l.f8_qkv, l.f8s_qkv, kvd, qkvd, qd + kvd, H}, {"self_attn.o_proj", 8, l.f8_o, l.f8s_o, H, H, 0, qd},
+        {"mlp.gate_proj", 16, l.f8_gu, l.f8s_gu, I, 2 * I, 0, H}, {"mlp.up_proj", 32, l.f8_gu, l.f8s_gu, I, 2 * I, I, H}, {"mlp.down_proj", 64, l.f8_down, l.f8s_down, H, H, 0, I}};
+    const std::string base = t.substr(0, t.find(".weight"));
+    for (const auto& e : p) {
+        if (base != e.name) continue;
+        if (dt == CRANE_B200_F8_E4M3) {
+            if (t != base + ".weight") break;
+            want_shape(n, shape, ndim, {e.rows, e.cols});
+            if (!e.w) e.w = dalloc<unsigned char>((size_t)e.all * e.cols);
+            CUDA_OK(cudaMemcpy(e.w + (size_t)e.at * e.cols, data, (size_t)e.rows * e.cols, cudaMemcpyHostToDevice));
+            l.f8 |= e.bit; l.loaded |= e.bit;
+            any_f8 = true;
+        } else {                                                   // (heads are 128 or 256 wide, H and I multiples of 256: every matrix is whole blocks)
+            want_shape(n, shape, ndim, {e.rows / F8_BLOCK, e.cols / F8_BLOCK});
+            if (!e.s) e.s = dalloc<float>((size_t)(e.all / F8_BLOCK) * (e.cols / F8_BLOCK));
+            up_f32(e.s + (size_t)(e.at / F8_BLOCK) * (e.cols / F8_BLOCK), data, dt, (size_t)(e.rows / F8_BLOCK) * (e.cols / F8_BLOCK));
+            l.f8 |= e.bit << 7;
+        }
+        return true;
+    }
+    fail(CRANE_B200_UNSUPPORTED, "tensor %s: e4m3 codes and their scales are the seven projections' of a layer", n.c_str());
+}
+
+crane_b200_model::F8Rooms crane_b200_model::f8_rooms(int rows) {
+    const int kmax = std::max(std::max(H, I), q_dim());
+    F8Rooms r;
+    r.codes = dalloc<unsigned char>((size_t)rows * kmax);
+    r.scales = dalloc<float>((size_t)(kmax / F8_BLOCK) * rows);
+    r.gu = dalloc<float>((size_t)rows * 2 * I);
+    r.rows = rows;
+    return r;
+}
+
+void crane_b200_model::f8_linear(const F8Rooms& r, const unsigned char* w, const float* ws, int N, int K, const float* add, float* y, int rows) {
+    const F8Linear a = {F8Rows{r.codes, K, r.scales, r.rows}, w, K, ws, K / F8_BLOCK, y, F8_F32, N, add, N, true};
+    LAUNCH_OK(f8_linear_launch(stream, a, rows, N, K, use_pdl));
+    ++launches;
+}
+void crane_b200_model::f8_qkv(const LayerW& l, const F8Rooms& r, const float* xin, float* y, int rows) {
+    const F8Norm n = {xin, F8_F32, H, nullptr, nullptr, F8_F32, 0, l.ln1, F8_F32, eps};
+    LAUNCH_OK(f8_rms_norm_launch(stream, n, rows, H, F8Out{r.codes, H, r.scales, r.rows}, use_pdl));
+    ++launches;
+    f8_linear(r, l.f8_qkv, l.f8s_qkv, qkv_dim(), H, nullptr, y, rows);
+}
+void crane_b200_model::f8_o(const LayerW& l, const F8Rooms& r, const float* a, float* xio, int rows) {
+    LAUNCH_OK(f8_quantize_launch(stream, a, F8_F32, q_dim(), rows, q_dim(), F8Out{r.codes, q_dim(), r.scales, r.rows}, use_pdl));
+    ++launches;
+    f8_linear(r, l.f8_o, l.f8s_o, H, q_dim(), xio, xio, rows);
+}
+void crane_b200_model::f8_mlp(const LayerW& l, const F8Rooms& r, float* xio, int rows) {
+    const F8Norm n = {xio, F8_F32, H, nullptr, nullptr, F8_F32, 0, l.ln2, F8_F32, eps};
+    LAUNCH_OK(f8_rms_norm_launch(stream, n, rows, H, F8Out{r.codes, H, r.scales, r.rows}, use_pdl));
+    f8_linear(r, l.f8_gu, l.f8s_gu, 2 * I, H, nullptr, r.gu, rows);
+    LAUNCH_OK(f8_silu_mul_launch(stream, r.gu, F8_F32, 2 * I, rows, I, F8Out{r.codes, I, r.scales, r.rows}, use_pdl));
+    launches += 2;
+    f8_linear(r, l.f8_down, l.f8s_down, H, I, xio, xio, rows);
+}
+
+// =================================================================================================
 // finalize: tables, KV pages, decode buffers
 // =================================================================================================
 void crane_b200_model::finalize() {
@@ -1129,6 +1221,12 @@ void crane_b200_model::finalize() {
         }
         (void)mx;
         xq_buf = dalloc<unsigned char>(xquant_bytes(4, std::max(std::max(H, I), q_dim())));      // calls of up to four rows / sequences
+    }
+    for (int i = 0; i < L; ++i) {
+        const int codes = layers[i].f8 & 127, scales = layers[i].f8 >> 7;
+        if (codes != scales) fail(CRANE_B200_NOT_LOADED, "layer %d: e4m3 projections and scales do not match (masks 0x%x, 0x%x)", i, codes, scales);
+        if (codes && (codes != 127 || layers[i].wqkv || layers[i].wo || layers[i].wgu || layers[i].wdown || layers[i].qt_q || layers[i].qt_o || layers[i].qt_gu || layers[i].qt_down))
+            fail(CRANE_B200_UNSUPPORTED, "layer %d: all seven projections are e4m3, or none", i);
     }
     for (int i = 0; i < L; ++i) {
         // full: q,k,v,o (1|2|4|8) gate,up,down (16|32|64) ln1,ln2 (128|256) q_norm,k_norm (512|1024)
@@ -1228,6 +1326,7 @@ void crane_b200_model::finalize() {
         TcScratch sc;                               // (taken here, not by the first decode step)
         LAUNCH_OK(tc_scratch_get(stream, (std::max(std::max(V, 2 * I), qkv_dim()) + 127) / 128, &sc));
     }
+    if (any_f8) f8_dec = f8_rooms(B);
     x_dec = dalloc<float>((size_t)B * H);
     qkv_dec = dalloc<float>((size_t)B * qkv_dim());
     attn_dec = dalloc<float>((size_t)B * q_dim());
@@ -1246,7 +1345,7 @@ void crane_b200_model::finalize() {
     CUDA_OK(cudaMemset(ticket, 0, sizeof(unsigned int)));
     CUDA_OK(cudaMemset(state, 0, B * sizeof(SeqState)));
     // single-sequence bf16 decode runs as ONE persistent launch per call (decode_ll.cu) when the geometry allows it
-    use_persistent = use_persistent && !hybrid && !any_quant && !is_tts && !kv_bits && owns_stream && L <= LL_MAX_LAYERS &&
+    use_persistent = use_persistent && !hybrid && !any_quant && !any_f8 && !is_tts && !kv_bits && owns_stream && L <= LL_MAX_LAYERS &&
                      decode_ll_supported(D, rot_half, nh, nkv, H, I, q_dim(), qkv_dim(), V, num_sms);
     if (use_persistent) {
         int coop = 0;
@@ -1279,7 +1378,8 @@ void crane_b200_model::ensure_prefill_ws(int S) {
     if (S <= ws_S) return;
     CUDA_OK(cudaStreamSynchronize(stream));
     for (void* p : {(void*)x, (void*)qkv, (void*)xn, (void*)q_bf, (void*)attn_bf, (void*)act_bf, (void*)ids_dev, (void*)pos3_dev,
-                    (void*)rows_dev, (void*)embeds_in, (void*)rows_f32, (void*)xqr_buf, (void*)g_proj, (void*)g_conv, (void*)g_qn, (void*)g_kn, (void*)g_gb, (void*)g_y, (void*)g_gl, (void*)g_chunk})
+                    (void*)rows_dev, (void*)embeds_in, (void*)rows_f32, (void*)xqr_buf, (void*)g_proj, (void*)g_conv, (void*)g_qn, (void*)g_kn, (void*)g_gb, (void*)g_y, (void*)g_gl, (void*)g_chunk,
+                    (void*)f8_pre.codes, (void*)f8_pre.scales, (void*)f8_pre.gu})
         dfree(p);
     const int cap = (S + 127) / 128 * 128;
     x = dalloc<float>((size_t)cap * H);
@@ -1306,7 +1406,8 @@ void crane_b200_model::ensure_prefill_ws(int S) {
     pos3_dev = dalloc<int>((size_t)3 * cap);
     rows_dev = dalloc<int>(cap);
     embeds_in = dalloc<float>((size_t)cap * H);
-    rows_f32 = any_quant ? dalloc<float>((size_t)cap * std::max(I, q_dim())) : nullptr;
+    if (any_f8) f8_pre = f8_rooms(cap);
+    rows_f32 = any_quant || any_f8 ? dalloc<float>((size_t)cap * std::max(I, q_dim())) : nullptr;
     xqr_buf = any_quant ? dalloc<unsigned char>(qrows_bytes(cap, std::max(std::max(H, I), q_dim()))) : nullptr;
     xqr_rows = cap;
     ws_S = cap;
@@ -1354,6 +1455,13 @@ void crane_b200_model::enqueue_decode_step(int advance, bool with_embed, int B) 
     for (int li = 0; li < L; ++li) {
         LayerW& l = layers[li];
         if (l.full) {
+            if (l.f8) {
+                f8_qkv(l, f8_dec, x_dec, qkv_dec, B);
+                attn_decode(l, B);
+                f8_o(l, f8_dec, attn_dec, x_dec, B);
+                f8_mlp(l, f8_dec, x_dec, B);
+                continue;
+            }
             if (l.qt_q) {   // GGUF keeps q/k/v as separate quantised matrices (qwen3/modeling.rs:252-255): GEMVs into one qkv row
                 qkv_linears(l, [&](const unsigned char* w, int t, int n, int col, const QMore& more, bool again) {
                     linear_decode(GEMV_STORE, true, nullptr, w, t, n, H, x_dec, H, l.ln1, qkv_dec + col, qkv_dim(), nullptr, B, again, more);
@@ -1486,6 +1594,13 @@ void crane_b200_model::linear_wide(int epi, const bf16* w, const unsigned char* 
 void crane_b200_model::enqueue_wide_step(int advance, int B) {
     for (int li = 0; li < L; ++li) {
         LayerW& l = layers[li];
+        if (l.f8) {
+            f8_qkv(l, f8_dec, x_dec, qkv_dec, B);
+            attn_decode(l, B);
+            f8_o(l, f8_dec, attn_dec, x_dec, B);
+            f8_mlp(l, f8_dec, x_dec, B);
+            continue;
+        }
         if (l.qt_q) {
             qkv_rows(l, xqd_buf, wide_rows, x_dec, qkv_dec, B);
         } else {
@@ -1678,10 +1793,12 @@ void crane_b200_model::prefill(const uint32_t* ids, const float* embeds, size_t 
         LayerW& l = layers[li];
         const bool q_qkv = l.full && l.qt_q != 0;
         spans.mark(SP_NORM);
-        if (!q_qkv) LAUNCH_OK(rmsnorm_rows_launch(stream, x, S, H, l.ln1, eps, xn, lo_xn));
+        if (!q_qkv && !l.f8) LAUNCH_OK(rmsnorm_rows_launch(stream, x, S, H, l.ln1, eps, xn, lo_xn));
         if (l.full) {
             spans.mark(SP_ATTN_QKV);
-            if (q_qkv) {   // GGUF keeps q / k / v separate and quantised (qwen3/modeling.rs:252-255): integer dots
+            if (l.f8) {
+                f8_qkv(l, f8_pre, x, qkv, S);
+            } else if (q_qkv) {   // GGUF keeps q / k / v separate and quantised (qwen3/modeling.rs:252-255): integer dots
                 const bool all = S >= std::max(qrows_min(l.qt_q), std::max(qrows_min(l.qt_k), qrows_min(l.qt_v)));
                 if (all) qkv_rows(l, xqr_buf, xqr_rows, x, qkv, S);
                 for (int s0 = 0; s0 < S && !all;) {       // (a few rows: groups of up to four)
@@ -1716,7 +1833,11 @@ void crane_b200_model::prefill(const uint32_t* ids, const float* embeds, size_t 
             LAUNCH_OK(flash_prefill_launch(stream, D, true, true, fa));
             if (hybrid) { LAUNCH_OK(gate_mul_launch(stream, attn_bf, qkv, S, nh, D, q_stride(), qkv_dim(), lo_attn)); ++launches; }
             spans.mark(SP_ATTN_O);
-            if (l.qt_o) {
+            if (l.f8) {
+                LAUNCH_OK(planes_to_f32_launch(stream, attn_bf, lo_attn, (size_t)S * qd, rows_f32));
+                ++launches;
+                f8_o(l, f8_pre, rows_f32, x, S);
+            } else if (l.qt_o) {
                 LAUNCH_OK(planes_to_f32_launch(stream, attn_bf, lo_attn, (size_t)S * qd, rows_f32));
                 ++launches;
                 qlinear_rows(GEMV_RESID, l.q_wo, l.qt_o, H, qd, rows_f32, qd, nullptr, x, H, S);
@@ -1736,8 +1857,10 @@ void crane_b200_model::prefill(const uint32_t* ids, const float* embeds, size_t 
             launches += gdn_forward_launch_count(ga);     // conv (+ norms + gates), conv state, recurrence (1 kernel, or 3 chunkwise), gated norm
         }
         // MLP: either linear may be quantised on its own (Q4_K_M keeps ffn_down in Q6_K, the others in Q4_K)
-        spans.mark(l.qt_gu ? SP_MLP_GATE_UP : SP_NORM);
-        if (l.qt_gu) {
+        spans.mark(l.qt_gu || l.f8 ? SP_MLP_GATE_UP : SP_NORM);
+        if (l.f8) {
+            f8_mlp(l, f8_pre, x, S);
+        } else if (l.qt_gu) {
             qlinear_rows(GEMV_SILU_MUL, l.q_wgu, l.qt_gu, 2 * I, H, x, H, l.ln2, rows_f32, I, S);
             if (!l.qt_down) { LAUNCH_OK(cast_f32_bf16_launch(stream, rows_f32, act_bf, (size_t)S * I, lo_act)); ++launches; }
         } else {
@@ -1747,7 +1870,8 @@ void crane_b200_model::prefill(const uint32_t* ids, const float* embeds, size_t 
             if (l.qt_down) { LAUNCH_OK(planes_to_f32_launch(stream, act_bf, lo_act, (size_t)S * I, rows_f32)); ++launches; }
         }
         spans.mark(SP_MLP_DOWN);
-        if (l.qt_down) qlinear_rows(GEMV_RESID, l.q_wdown, l.qt_down, H, I, rows_f32, I, nullptr, x, H, S);
+        if (l.f8) {}
+        else if (l.qt_down) qlinear_rows(GEMV_RESID, l.q_wdown, l.qt_down, H, I, rows_f32, I, nullptr, x, H, S);
         else gemm(act_bf, lo_act, I, l.wdown, S, H, I, EPI_RESID_F32, x, H, nullptr);
         launches += 4;
         if (n_vis > 0 && li < (int)v_deepstack.size()) {   // DeepStack (qwen3_vl/text.rs:262-268)

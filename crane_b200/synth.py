@@ -801,6 +801,50 @@ def synth_checkpoint(cfg: dict):
         yield name, make_tensor(name, shape, kind)
 
 
+# the projections of a layer that an fp8 checkpoint holds as e4m3 codes
+FP8_PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+
+def e4m3_values() -> np.ndarray:
+    """The 127 values of the codes 0 .. 126 (sign bit off, ascending; 127 is NaN): e = 0: m 2^-9, else (8 + m) 2^(e - 10)."""
+    c = np.arange(127)
+    e, m = c >> 3, c & 7
+    return np.where(e == 0, m * 2.0 ** -9, (8 + m) * 2.0 ** (e - 10.0)).astype(np.float32)
+
+
+def e4m3_encode(x: np.ndarray) -> np.ndarray:
+    """The codes of x rounded to the nearest e4m3 value, ties to the even code, saturating at 448."""
+    v = e4m3_values().astype(np.float64)
+    a = np.abs(np.asarray(x, np.float64))
+    mid = (v[1:] + v[:-1]) / 2
+    lo, hi = np.searchsorted(mid, a, "left"), np.searchsorted(mid, a, "right")      # they differ on a tie
+    code = np.where(lo == hi, lo, np.where(lo % 2 == 0, lo, hi)).astype(np.uint8)
+    return code | (np.signbit(x).astype(np.uint8) << 7)
+
+
+def e4m3_decode(codes: np.ndarray) -> np.ndarray:
+    v = np.append(e4m3_values(), np.float32(np.nan))
+    return np.where(codes & 128, -v[codes & 127], v[codes & 127])
+
+
+def fp8_config(cfg: dict) -> dict:
+    return dict(cfg, quantization_config={"quant_method": "fp8", "fmt": "e4m3", "activation_scheme": "dynamic", "weight_block_size": [128, 128]})
+
+
+def fp8_checkpoint(cfg: dict):
+    """synth_checkpoint(cfg) with the layers' projections as an fp8 checkpoint has them: uint8 codes, and `weight_scale_inv` for every 128 x 128."""
+    for name, arr in synth_checkpoint(cfg):
+        part = name.split(".")
+        if "layers" not in part or part[-2] not in FP8_PROJECTIONS or "visual" in part:
+            yield name, arr
+            continue
+        n, k = arr.shape
+        b = arr.astype(np.float32).reshape(n // 128, 128, k // 128, 128)
+        scale = (np.abs(b).max((1, 3)) / np.float32(448)).astype(np.float32)
+        yield name, e4m3_encode((b / scale[:, None, :, None]).reshape(n, k))
+        yield name + "_scale_inv", scale
+
+
 def synth_token_ids(n: int, vocab: int, tag: str = "ids", forbid=()) -> np.ndarray:
     ids = _rng(tag).integers(0, vocab, size=n, dtype=np.int64)
     for f in forbid:

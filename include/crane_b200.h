@@ -45,7 +45,8 @@ typedef enum {
 typedef enum {
     CRANE_B200_F32 = 0,
     CRANE_B200_BF16 = 1,
-    CRANE_B200_F16 = 2
+    CRANE_B200_F16 = 2,
+    CRANE_B200_F8_E4M3 = 3 /* crane_b200_load_tensor only: codes of an fp8 checkpoint's projections */
 } crane_b200_dtype;
 
 /* Logits of the LAST position of the most recent forward call (f32, device memory, `stream` ordered).
@@ -86,7 +87,9 @@ CRANE_B200_API const char* crane_b200_last_error(const crane_b200_model* m);
 /* Register one checkpoint tensor by its safetensors name (`model.layers.{i}.self_attn.q_proj.weight`,
  * `model.language_model...`, `model.visual.blocks.{i}.attn.qkv.weight`, `lm_head.weight`, ... exactly
  * the names read at crane-core/src/models/qwen3/modeling.rs:160-282,598-606,771-813 and
- * qwen3_5/vision.rs:23-35,70-71,114-115,245-250,321-339).  `data` is host memory. */
+ * qwen3_5/vision.rs:23-35,70-71,114-115,245-250,321-339).  `data` is host memory.
+ * An fp8 checkpoint (dense and VL text layers; config.json's quantization_config: quant_method "fp8", weight_block_size [128, 128], activation_scheme "dynamic") has the
+ * seven projections of a layer as CRANE_B200_F8_E4M3 codes, each with a scale for every 128 x 128 as `*.weight_scale_inv` [rows / 128, columns / 128] (f32, bf16 or f16). */
 CRANE_B200_API int crane_b200_load_tensor(crane_b200_model* m, const char* name, int dtype, const int64_t* shape, int ndim,
                            const void* data);
 /* Register a GGUF-quantised 2-D tensor as raw ggml blocks (ggml_type: Q8_0 = 8, Q4_K = 12, Q6_K = 14), shape = [rows, cols]
