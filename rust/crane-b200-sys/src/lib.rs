@@ -19,6 +19,7 @@ pub const CRANE_B200_NOT_LOADED: c_int = -5;
 pub const CRANE_B200_F32: c_int = 0;
 pub const CRANE_B200_BF16: c_int = 1;
 pub const CRANE_B200_F16: c_int = 2;
+pub const CRANE_B200_F8_E4M3: c_int = 3;
 
 #[repr(C)]
 #[derive(Clone, Copy)]
