@@ -29,10 +29,10 @@ int f8_err_word(cudaStream_t st, int** out) {
     return r;
 }
 
-// A load that stays where it is written, ahead of waits that it overlaps (the compiler may move __ldg down to its use)
+// A load that stays where it is written, ahead of waits that it overlaps (the compiler may move __ldg down to its use), of what the kernel ahead has written
 __device__ __forceinline__ float f8_fetch(const float* p) {
     float v;
-    asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
     return v;
 }
 
@@ -195,6 +195,10 @@ f8_rows_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             if (++s == STAGES) { s = 0; ph ^= 1; }
             if (++b == BUFS) { b = 0; bph ^= 1; }
         }
+        // TMEM is given back as soon as it has been read: a CTA that waits for its cluster holds none that another cluster's CTA may be waiting for
+        named_bar_sync(2, 32 + 32 * F8_EPI);
+        tc_fence_after();
+        tmem_dealloc(tmem, Cfg::COLS);
     } else {
         pdl_wait();
         float* patch = reinterpret_cast<float*>(sm + Cfg::MAIN + Cfg::ROOM) + (warp - 2) * 2 * F8_CH * CW;
@@ -258,6 +262,8 @@ f8_rows_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             if (lane == 0) f8_arrive(smem_u32(&d_empty[b]));
             if (++b == BUFS) { b = 0; bph ^= 1; }
         }
+        tc_fence_before();
+        asm volatile("bar.arrive 2, %0;" ::"n"(32 + 32 * F8_EPI) : "memory");
         // the sums, a row of 128 a column of the tile: to the CTA that finishes the row, or in place of this CTA's stages (its MMAs are complete, all of them)
         const int row0 = part * CW;
         if (Cfg::PUSH && a.cl > 1) {
@@ -322,9 +328,6 @@ f8_rows_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             cluster_sync_all();                      // nobody leaves while its shared memory is still being read
         }
     }
-    tc_fence_before();
-    __syncthreads();
-    if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem, Cfg::COLS); }
 }
 
 static bool f8_vec_out(const F8Linear& p) {
@@ -408,12 +411,12 @@ struct F8PairArgs {
     long long lds, ldws;
     int M, N, KB, tiles_m, tiles_n, pairs;
     int whole, items, cut;             // tiles 0 .. whole - 1 as they are, then strips of 256 / cut columns: `items` together
-    bool vec, w_static;
+    bool vec, tma, w_static;
     int* err;
 };
 constexpr int F8_BAND = 8;                         // rows of tiles that are walked together: neighbours in time share weights and activations in L2
 struct F8PairCfg {
-    static constexpr int A_BYTES = 128 * 128, STAGE = A_BYTES + 128 * 128, PATCH = F8_EPI * 4096;
+    static constexpr int A_BYTES = 128 * 128, STAGE = A_BYTES + 128 * 128, PATCH = F8_EPI * 8192;
     static constexpr int STAGES = (226 * 1024 - PATCH - 1024) / STAGE;
     static constexpr int SMEM = STAGES * STAGE + PATCH + 1024;
 };
@@ -496,10 +499,34 @@ __device__ __forceinline__ void f8_store_rows(const F8Epi& e, bool vec, int M, i
     }
 }
 
+// The same rows by TMA, two pieces of 128 bytes a row under way: the tiles of all SMs end together, and what they store then (64 KB each) takes the chip longer than the two blocks
+// of K that the MMAs run ahead.
+template <typename T, int C>
+__device__ __forceinline__ void f8_store_tma(const CUtensorMap* map, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
+    constexpr int PER = 16 / (int)sizeof(T), W = 8 * PER;
+#pragma unroll
+    for (int c = 0; c < C; c += W) {
+        if (n0 + c >= N || m0 >= M) break;
+        uint8_t* to = patch + (c / W & 1) * 4096;
+        if (lane == 0) tma_store_wait_read<1>();
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            alignas(16) T h[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) h[i] = f8_round<T>(v[c + p * PER + i]);
+            *reinterpret_cast<uint4*>(to + sw128_off(lane, p)) = *reinterpret_cast<const uint4*>(h);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) { tma_store_2d(map, to, n0 + c, m0); tma_store_commit(); }
+    }
+}
+
 // One tile, or strip, of an epilogue warp: C columns of each lane's row
 struct F8Ring { uint64_t *full, *empty; int b; uint32_t phases; };
 template <int C, typename T>
-__device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const float* xs, const float* ws, uint32_t lanes, F8Ring& ring, const TcWait& wait, int m0, int n0, int N,
+__device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensorMap* tmO, const float* xs, const float* ws, uint32_t lanes, F8Ring& ring, const TcWait& wait, int m0, int n0, int N,
                                              uint8_t* patch, int lane) {
     constexpr int BUFS = 256 / C;
     float v[C];
@@ -509,14 +536,17 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const float* x
     constexpr int AHEAD = C == 128 ? 1 : 2;
     float nx[AHEAD], nw[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) { nx[u] = f8_fetch(xs + min(u, a.KB - 1) * a.lds); nw[u] = f8_fetch(ws + min(u, a.KB - 1)); }
+    for (int u = 0; u < AHEAD; ++u) {
+        nx[u] = f8_fetch(xs); nw[u] = f8_fetch(ws);
+        if (u + 1 < a.KB) { xs += a.lds; ++ws; }
+    }
     for (int k0 = 0; k0 < a.KB; k0 += AHEAD)
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
         const int kb = k0 + u;
         if (kb >= a.KB) break;
         const float sc = nx[u] * nw[u];
-        if (kb + AHEAD < a.KB) { nx[u] = f8_fetch(xs + (kb + AHEAD) * a.lds); nw[u] = f8_fetch(ws + kb + AHEAD); }
+        if (kb + AHEAD < a.KB) { nx[u] = f8_fetch(xs); nw[u] = f8_fetch(ws); xs += a.lds; ++ws; }
         wait(&ring.full[ring.b], (ring.phases >> ring.b) & 1);
         tc_fence_after();
         const uint32_t d = lanes + (uint32_t)(ring.b * 2 * C);
@@ -538,6 +568,11 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const float* x
         ring.phases ^= 1u << ring.b;
         if (++ring.b == BUFS) ring.b = 0;
     }
+    if constexpr (C * sizeof(T) >= 128) {
+        if (a.tma) { f8_store_tma<T, C>(tmO, a.M, N, m0, n0, v, patch, lane); return; }
+    }
+    if (lane == 0) tma_store_wait_read<0>();          // (the whole tiles' stores have left the patch)
+    __syncwarp();
     f8_store_rows<T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
 }
 
@@ -547,7 +582,8 @@ static_assert(128 * F8_REGS_LOW + 32 * F8_EPI * F8_REGS_EPI <= F8_PAIR_THREADS *
 //   warp 0: TMA producer    warp 1: TMEM allocator and (even CTA) MMA issuer    warps 4 - 11: epilogue (32 rows from 32 (warp % 4), half of the columns)
 template <typename T>
 __global__ void __launch_bounds__(F8_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
-f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW32, const F8PairArgs a) {
+f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW32,
+               const __grid_constant__ CUtensorMap tmO, const F8PairArgs a) {
     using Cfg = F8PairCfg;
     constexpr int STAGE = Cfg::STAGE, STAGES = Cfg::STAGES, C = 128;
     extern __shared__ uint8_t smem_raw[];
@@ -641,7 +677,7 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F8_REGS_EPI));
         pdl_wait();
         const int q = warp & 3, part = (warp - 4) >> 2;
-        uint8_t* patch = sm + STAGES * STAGE + (warp - 4) * 4096;
+        uint8_t* patch = sm + STAGES * STAGE + (warp - 4) * 8192;
         int width = 256;
         F8Ring ring = {d_full, d_empty, 0, 0};
         for (int i = pair; i < a.items; i += a.pairs) {
@@ -652,10 +688,11 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             const float* xs = a.xs + min(m0 + lane, a.M - 1);
             const float* ws = a.ws + (long long)min(n0 / 128, (a.N - 1) / 128) * a.ldws;
             const int N = min(a.N, n0 + cw);
-            if (width == 256) f8_pair_tile<128, T>(a, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
-            else if (width == 128) f8_pair_tile<64, T>(a, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
-            else f8_pair_tile<32, T>(a, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            if (width == 256) f8_pair_tile<128, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            else if (width == 128) f8_pair_tile<64, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            else f8_pair_tile<32, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
         }
+        if (lane == 0) tma_store_wait_read<0>();      // (the writes themselves are complete when the grid is)
     }
     tc_fence_before();
     __syncthreads();
@@ -688,13 +725,17 @@ static int f8_pair_t(cudaStream_t st, const F8Linear& p, int M, int N, int K, bo
     a.pairs = std::min(a.items, pairs);
     a.vec = f8_vec_out(p);
     if (const int err = f8_err_word(st, &a.err)) return err;
-    CUtensorMap tmX, tmW, tmW32;
+    CUtensorMap tmX, tmW, tmW32, tmO;
     if (!tc_tmap_encode(&tmX, p.x.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K, (uint64_t)p.x.ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmW, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmW32, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
+    a.tma = a.vec && !p.add && (long long)N * (long long)sizeof(T) % 16 == 0;      // (a row that ends inside 16 bytes would be written to their end)
+    tmO = tmX;
+    if (a.tma && !tc_tmap_encode(&tmO, p.out, std::is_same<T, float>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                                 (uint64_t)M, (uint64_t)N, (uint64_t)p.ldo, 32, 128 / sizeof(T), CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
     static SmemOptIn seen;
     if (const int err = ensure_dyn_smem(f8_pair_kernel<T>, (size_t)Cfg::SMEM, seen)) return err;
-    return launch_k(f8_pair_kernel<T>, dim3(2 * a.pairs), dim3(F8_PAIR_THREADS), Cfg::SMEM, st, pdl, tmX, tmW, tmW32, a);
+    return launch_k(f8_pair_kernel<T>, dim3(2 * a.pairs), dim3(F8_PAIR_THREADS), Cfg::SMEM, st, pdl, tmX, tmW, tmW32, tmO, a);
 }
 static int f8_pair_launch(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
     switch (p.type) {

@@ -152,7 +152,7 @@ __device__ __forceinline__ float f8_silu_mul(float g, float u) {
 // A warp takes 512 columns of a row (four blocks) at a time and asks for U such pieces before it works on the first.
 template <typename T, bool GATED, bool VEC, int U>
 __global__ void __launch_bounds__(256)
-f8_rows_kernel(const T* __restrict__ x, long long ldx, long long M, int K, F8Out o) {
+f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
     const int c0 = f8_col(threadIdx.x & 31), per = (K + 511) / 512;
     const unsigned warps = gridDim.x * 8, w = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int dm = (int)(warps / per), dc = (int)(warps % per);             // a step of all warps: rows and pieces

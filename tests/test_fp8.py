@@ -323,6 +323,21 @@ def test_linear_of_wide_strides_and_codes_of_every_value(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m, n, k", [(1, 100, 256), (60, 1001, 256), (100, 77, 640), (129, 260, 128), (700, 1001, 256), (1300, 2085, 384), (4900, 4200, 128)])
+def test_linear_leaves_what_lies_around_its_rows(m, n, k, dt):
+    """Results in rows on 16-byte boundaries that are wider than the result, on every route: columns behind the last and the rows around stay as they are."""
+    from crane_b200 import fp8
+    gen = gen_of("around", m, n, k, dt)
+    x, xs = fp8.quantize(rows_of(gen, m, k, torch.float32))
+    w, ws = weights(gen, n, k)
+    wide = torch.full((m + 2, (n + 15) // 8 * 8), 99.0, device="cuda", dtype=TYPES[dt])
+    out = fp8.linear(x, xs, w, ws, out=wide[1:m + 1, :n])
+    check_linear(out, linear_ref(x, xs, w, ws))
+    assert (wide[0] == 99).all() and (wide[m + 1] == 99).all() and (wide[:, n:] == 99).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 40, 100, 700])
 def test_linear_keeps_nan_and_infinity_in_their_rows(m):
     from crane_b200 import fp8
