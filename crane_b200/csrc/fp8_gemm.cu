@@ -546,12 +546,12 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensor
         const int kb = k0 + u;
         if (kb >= a.KB) break;
         const float sc = nx[u] * nw[u];
-        if (kb + AHEAD < a.KB) { nx[u] = f8_fetch(xs); nw[u] = f8_fetch(ws); xs += a.lds; ++ws; }
         wait(&ring.full[ring.b], (ring.phases >> ring.b) & 1);
         tc_fence_after();
         const uint32_t d = lanes + (uint32_t)(ring.b * 2 * C);
         uint32_t r[2][16];
         tmem_ld16_async(d, r[0]);
+        if (kb + AHEAD < a.KB) { nx[u] = f8_fetch(xs); nw[u] = f8_fetch(ws); xs += a.lds; ++ws; }
         tmem_ld_wait();
 #pragma unroll
         for (int c = 0; c < C; c += 16) {

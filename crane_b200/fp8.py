@@ -143,22 +143,25 @@ def rms_norm(x, weight, eps: float = 1e-6, *, residual=None, residual_out=None, 
     """(codes, scales) of the RMS norm of h = x, or of h = x + residual, which is stored to `residual_out` (None: in place of `residual`) in the residual's type and
     normalised as stored.  `weight` [k] f32, bf16 or f16."""
     dev, m, k, ldx, dtype = _rows_in("x", x)
-    if not isinstance(weight, torch.Tensor) or weight.dtype not in _DTYPES or weight.shape != (k,) or weight.get_device() != dev or (k > 1 and weight.stride(0) != 1):
+    wtype = _DTYPES.get(weight.dtype) if isinstance(weight, torch.Tensor) else None
+    if wtype is None or weight.shape != (k,) or weight.get_device() != dev or (k > 1 and weight.stride(0) != 1):
         _refuse(f"weight: {k} contiguous f32, bf16 or f16 values on cuda:{dev} are wanted")
     res = res_out = None
     rtype = ldr = 0
     if residual is not None:
-        if residual_out is None:
-            residual_out = residual
-        device = torch.device("cuda", dev)
-        ldr, rtype = _matrix("residual", residual, _DTYPES, device, (m, k)), _DTYPES[residual.dtype]
-        if residual_out is not residual and _matrix("residual_out", residual_out, (residual.dtype,), device, (m, k)) != ldr:
-            _refuse("residual_out: its rows lie as far apart as the residual's")
-        res, res_out = residual.data_ptr(), residual_out.data_ptr()
+        rdev, rm, rk, ldr, rtype = _rows_in("residual", residual)
+        if (rdev, rm, rk) != (dev, m, k):
+            _refuse(f"residual: shape {(rm, rk)} on cuda:{rdev}, expected {(m, k)} on cuda:{dev}")
+        res = res_out = residual.data_ptr()
+        if residual_out is not None and residual_out is not residual:
+            if (not isinstance(residual_out, torch.Tensor) or residual_out.dtype is not residual.dtype or residual_out.get_device() != dev or residual_out.shape != residual.shape
+                    or (m > 1 and residual_out.stride() != residual.stride()) or (k > 1 and residual_out.stride(1) != 1)):
+                _refuse("residual_out: a tensor of the residual's type, device, shape and strides is wanted")
+            res_out = residual_out.data_ptr()
     elif residual_out is not None:
         _refuse("residual_out without a residual")
     codes, scales, ld, lds = _out(out, m, k, dev)
-    rc = _entry("rms_norm")(dev, x.data_ptr(), dtype, ldx, res, res_out, rtype, ldr, weight.data_ptr(), _DTYPES[weight.dtype], eps, m, k, codes.data_ptr(), ld,
+    rc = _entry("rms_norm")(dev, x.data_ptr(), dtype, ldx, res, res_out, rtype, ldr, weight.data_ptr(), wtype, eps, m, k, codes.data_ptr(), ld,
                             scales.data_ptr(), lds, _raw_stream(dev))
     if rc:
         _failed(rc)
