@@ -79,7 +79,7 @@ struct F8RowsArgs {
     F8Epi ep;
     const float *xs, *ws;
     long long lds, ldws;
-    int M, N, KB, cl;
+    int M, N, KB, cl, tiles_n;
     bool vec, w_static;
     int* err;
 };
@@ -131,7 +131,7 @@ f8_rows_gemm_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     __shared__ int gave_up;
     const TcWait wait{&gave_up, a.err};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = blockIdx.x % a.cl, n0 = blockIdx.x / a.cl * 128, m0 = blockIdx.y * NT;
+    const int rank = blockIdx.x % a.cl, tile = blockIdx.x / a.cl, n0 = tile % a.tiles_n * 128, m0 = tile / a.tiles_n * NT;
     const int kb0 = (int)((long long)rank * a.KB / a.cl), kb1 = (int)((long long)(rank + 1) * a.KB / a.cl);
 
     if (threadIdx.x == 0) {
@@ -377,12 +377,13 @@ static int f8_rows_gemm_t(cudaStream_t st, const F8Linear& p, int M, int N, int 
     CUtensorMap tmW, tmX;
     if (!tc_tmap_encode(&tmW, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmX, p.x.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K, (uint64_t)p.x.ld, Cfg::NT, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
-    const int tn = (N + 127) / 128, tm = (M + Cfg::NT - 1) / Cfg::NT;
-    if (tm > 65535) return -1000;
+    const long long tiles = (long long)((N + 127) / 128) * ((M + Cfg::NT - 1) / Cfg::NT);
+    if (tiles > 0x0fffffffLL) return -1000;
+    a.tiles_n = (N + 127) / 128;
     if (const int e = f8_rows_smem<CW, OCC>()) return e;
-    a.cl = f8_rows_cluster<CW, OCC>((long long)tn * tm, a.KB);
+    a.cl = f8_rows_cluster<CW, OCC>(tiles, a.KB);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(tn * a.cl, tm); cfg.blockDim = dim3(64 + 32 * F8_EPI); cfg.dynamicSmemBytes = Cfg::SMEM; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)(tiles * a.cl)); cfg.blockDim = dim3(64 + 32 * F8_EPI); cfg.dynamicSmemBytes = Cfg::SMEM; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int na = 0;
     if (a.cl > 1) {
@@ -404,6 +405,10 @@ static int f8_rows_gemm_t(cudaStream_t st, const F8Linear& p, int M, int N, int 
 // an epilogue thread has one activation row and half of the columns, so that its scale is one product a block of K.
 // A persistent pair an SM pair takes tiles in turn; MMAs run up to two blocks of K ahead of the epilogue, into the next tile too.  Tiles left over for the last turn, or
 // for the only one, are cut into 2 or 4 strips of columns when that many pairs are free.
+// What bounds it (8192 x 24576 x 4096, 2 310 TFLOP/s; the MMAs and stores alone 2 700 at 1.3 GHz under the power limit): the two accumulators.  A block's MMAs take 512 cycles, its
+// epilogue 440 (TMEM reads and 256 FMA issues a scheduler, next to MMAs that read and write the same TMEM), the hand-overs between them (commit, wait, arrival at
+// the even CTA) some 600 more, so that a block passes every 800.  Measured and left: two MMAs of 128 columns, for four accumulators (1 850 TFLOP/s, an MMA takes 125 cycles all the same),
+// sixteen epilogue warps, 32 columns a read, two producers, two issuing warps (no gain).
 // =====================================================================================
 struct F8PairArgs {
     F8Epi ep;
@@ -750,7 +755,8 @@ static int f8_pair_launch(cudaStream_t st, const F8Linear& p, int M, int N, int 
 //   77 x 4096 x 2048 7.1 / 7.8 / 8.3 / 11.5   77 x 12288 x 2048 15.9 / 11.0 / 12.9 / 13.3   128 x 4096 x 12288 18.2 / 22.6 / 19.0 / 48   128 x 24576 x 4096 42 / 48 / 41 / 39
 //   256 x 4096 x 4096 13.0 / 16.3 / 13.8 / 19.1   256 x 12288 x 2048 25.7 / 21.3 / 25.7 / 14.1   512 x 2048 x 6144 17.2 / 21.8 / 17.5 / 26.8   512 x 4096 x 2048 16.9 / 20.3 / 13.3 / 13.0
 //   700 x 2048 x 6144 - / 22.0 / 28.2 / 29.3   1024 x 4096 x 4096 - / - / 40.7 / 22.2
-// A CTA takes c us a block of K (in two turns a tenth, in more a quarter more), a pair 0.45, whatever the width of its strip: the copies' way to shared memory is what both wait for.
+// A CTA takes c us a block of K (in two turns a tenth, in more a quarter more), a pair 0.45, whatever the width of its strip: an MMA of 256 rows takes some 125 cycles with 64 to 256
+// columns, so that strips shorten the last turn by their stores and their scales only (1111 x 4096 x 2048 20.5 / 18.7, 256 x 24576 x 4096 38.4 / 37.1, none 400 x 4096 x 4096 19.7 / 20.4).
 template <int CW>
 static double f8_rows_us(int M, int N, int KB, double t0, double c) {
     const long long tiles = (long long)((N + 127) / 128) * ((M + 2 * CW - 1) / (2 * CW));

@@ -328,7 +328,7 @@ CRANE_B200_API int crane_b200_decode_path(const crane_b200_model* m);
  * Every pointer is memory of `device`, `stream` a cudaStream_t of that device (NULL: its default stream); a call enqueues its work there, with no wait and no
  * copy to the host, and may be captured into a graph.  Inputs and results have to stay while that work runs.  Nothing is kept between calls: several threads may make them at once.
  * dtype: crane_b200_dtype; a row distance (ld..) counts elements.  Codes: rows start on 16-byte boundaries (base and ld multiples of 16, ld >= columns), any number of
- * columns.  Scales of rows: block by block, that of row i and block b at scales[b * lds + i], lds >= rows.  m = 0 (or n = 0) does nothing.
+ * columns.  Scales of rows: block by block, that of row i and block b at scales[b * lds + i], lds >= rows.  m = 0 (or n = 0) does nothing; m, n and k go to 2^30.
  * Bytes behind a row's last column and rows behind the last are left as they are.
  * On an error the message is crane_b200_fp8_last_error()'s, the calling thread's own. */
 CRANE_B200_API const char* crane_b200_fp8_last_error(void);

@@ -447,6 +447,66 @@ def test_streams_threads_and_graphs():
 
 
 @pytest.mark.gpu
+def test_many_rows_of_few_columns():
+    """More tiles of rows than a grid's second dimension has room for, offsets past 2^31, and the largest sizes that are taken."""
+    from crane_b200 import fp8
+    gen = gen_of("many")
+    m, n, k = 4_300_000, 3, 16
+    x, xs = fp8.quantize(rows_of(gen, m, k, torch.bfloat16, loud=False))
+    w, ws = weights(gen, n, k)
+    check_linear(fp8.linear(x, xs, w, ws), linear_ref(x, xs, w, ws))
+    # rows that lie far apart: the last ones' offsets pass 2^31 elements
+    far = torch.zeros(3 * 2 ** 30 + 4096, dtype=torch.bfloat16, device="cuda").as_strided((4, 256), (2 ** 30, 1))
+    far.copy_(rows_of(gen, 4, 256, torch.bfloat16))
+    near = far.clone()
+    for a, b in zip(fp8.quantize(far), fp8.quantize(near)):
+        assert torch.equal(a.view(torch.uint8) if a.dtype == F8 else a, b.view(torch.uint8) if b.dtype == F8 else b)
+    weight = torch.ones(256, device="cuda")
+    for a, b in zip(fp8.rms_norm(near, weight, residual=far, residual_out=far), fp8.rms_norm(near, weight, residual=near.clone())):
+        assert torch.equal(a.view(torch.uint8) if a.dtype == F8 else a, b.view(torch.uint8) if b.dtype == F8 else b)
+    c, s = fp8.quantize(near)
+    w, ws = weights(gen, 130, 256)
+    out = far.as_strided((4, 130), (2 ** 30, 1))
+    fp8.linear(c, s, w, ws, out=out)
+    assert torch.equal(out, fp8.linear(c, s, w, ws))
+    del far, out
+
+
+FIRST_IN_A_CAPTURE = """
+import sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+import test_fp8 as t
+from crane_b200 import fp8
+gen = t.gen_of("first")
+p = t.layer_params(gen, 512, 768)
+rows = {{m: (t.rows_of(gen, m, 512, torch.bfloat16), t.rows_of(gen, m, 512, torch.float32)) for m in (1, 40, 300)}}
+keep = {{m: s.clone() for m, (x, s) in rows.items()}}
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = {{m: t.layer(x, s, p) for m, (x, s) in rows.items()}}
+for m, (x, s) in rows.items():
+    s.copy_(keep[m])
+g.replay()
+torch.cuda.synchronize()
+for m, (x, s) in rows.items():
+    assert torch.equal(out[m], t.layer(x, keep[m].clone(), p)), m
+fp8.status()
+print("fine")
+"""
+
+
+@pytest.mark.gpu
+def test_first_calls_of_a_process_inside_a_capture():
+    """The first use of every kernel, and of the stream, happens while torch captures in its strict mode."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_A_CAPTURE.format(root=os.path.dirname(here), tests=here)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "fine" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 def test_tensors_are_refused():
     from crane_b200 import fp8
     x = torch.zeros((4, 256), device="cuda")
