@@ -89,12 +89,23 @@ template <typename T> struct F8Chunk<T, false> {
 template <typename T, bool VEC>
 __device__ __forceinline__ void f8_store8(T* row, int c, int K, float* v) {
     alignas(16) T h[8];
+    if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (std::is_same<T, float>::value) h[i] = v[i];
-        else if constexpr (std::is_same<T, bf16>::value) h[i] = __float2bfloat16_rn(v[i]);
-        else h[i] = __float2half_rn(v[i]);
-        v[i] = f8_float(h[i]);
+        for (int i = 0; i < 8; ++i) h[i] = v[i];
+    } else {                                    // two at a time, as the instruction has them
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            if constexpr (std::is_same<T, bf16>::value) {
+                const uint32_t u = pack_bf16(v[i], v[i + 1]);
+                *reinterpret_cast<uint32_t*>(h + i) = u;
+                v[i] = bf16lo(u); v[i + 1] = bf16hi(u);
+            } else {
+                const __half2 u = __floats2half2_rn(v[i], v[i + 1]);
+                *reinterpret_cast<__half2*>(h + i) = u;
+                const float2 f = __half22float2(u);
+                v[i] = f.x; v[i + 1] = f.y;
+            }
+        }
     }
     if constexpr (VEC) {
 #pragma unroll
@@ -112,9 +123,9 @@ __device__ __forceinline__ uint32_t f8_quad(float a, float b, float c, float d) 
 }
 // A thread has 16 columns of a block of 128, 8 from 8 (lane % 8) on and 8 from 64 behind those, 8 neighbouring threads the block.
 __device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
-// Scale and codes of it.  Every lane of the warp calls
+// Scale and codes of y = v rs.  Where y's largest magnitude counts, rs takes no part in the codes: v (448 / max |v|).  Every lane of the warp calls
 template <bool VEC>
-__device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c, int K, bool row_in, const F8Out& o) {
+__device__ __forceinline__ void f8_emit(const float (*v)[8], float rs, long long m, int c, int K, bool row_in, const F8Out& o) {
     float a = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -122,10 +133,10 @@ __device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c,
         for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[h][i]));
 #pragma unroll
     for (int s = 4; s > 0; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
-    a = fmaxf(a, F8_TINY);
-    const float inv = __fdiv_rn(F8_TOP, a);
+    const bool large = a * rs >= F8_TINY;         // (false for a row's NaN)
+    const float inv = __fdiv_rn(F8_TOP, large ? a : F8_TINY) * (large ? 1.f : rs);
     if (!row_in || c >= K) return;
-    if ((c & (F8_BLOCK - 1)) == 0) o.scales[(c / F8_BLOCK) * o.lds + m] = __fdiv_rn(a, F8_TOP);
+    if ((c & (F8_BLOCK - 1)) == 0) o.scales[(c / F8_BLOCK) * o.lds + m] = __fdiv_rn(large ? a * rs : F8_TINY, F8_TOP);
     unsigned char* p = o.codes + m * o.ld + c;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -202,7 +213,7 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
                     for (int i = 0; i < 8; ++i) y[h][i] = 0.f;
                 }
             }
-            f8_emit<VEC>(y, row[u], col[u], K, true, o);
+            f8_emit<VEC>(y, 1.f, row[u], col[u], K, true, o);
         }
     }
 }
@@ -297,15 +308,15 @@ f8_norm_kernel(const F8NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) load(m + step, c0 + j * a.tpr * 16, p[j]);
             }
-            const float rstd = row_rstd(s, turn);
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
+            for (int j = 0; j < PER; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[j][h][i] = v[j][h][i] * rstd * w[j][h][i];
-                f8_emit<VEC>(v[j], m, c0 + j * a.tpr * 16, K, m < a.M, a.o);
-            }
+                    for (int i = 0; i < 8; ++i) v[j][h][i] *= w[j][h][i];
+            const float rstd = row_rstd(s, turn);
+#pragma unroll
+            for (int j = 0; j < PER; ++j) f8_emit<VEC>(v[j], rstd, m, c0 + j * a.tpr * 16, K, m < a.M, a.o);
         }
     } else {
         for (; base < a.M; base += step, ++turn) {
@@ -335,9 +346,9 @@ f8_norm_kernel(const F8NormArgs a) {
                         q.get(v[h]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * rstd * w[h][i] : 0.f;
+                    for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * w[h][i] : 0.f;
                 }
-                f8_emit<VEC>(v, m, c, K, m < a.M, a.o);
+                f8_emit<VEC>(v, rstd, m, c, K, m < a.M, a.o);
             }
         }
     }
