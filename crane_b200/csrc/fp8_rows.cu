@@ -123,9 +123,9 @@ __device__ __forceinline__ uint32_t f8_quad(float a, float b, float c, float d) 
 }
 // A thread has 16 columns of a block of 128, 8 from 8 (lane % 8) on and 8 from 64 behind those, 8 neighbouring threads the block.
 __device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
-// Scale and codes of y = v rs.  Where y's largest magnitude counts, rs takes no part in the codes: v (448 / max |v|).  Every lane of the warp calls
+// Scale and codes of a thread's 16 columns.  Every lane of the warp calls
 template <bool VEC>
-__device__ __forceinline__ void f8_emit(const float (*v)[8], float rs, long long m, int c, int K, bool row_in, const F8Out& o) {
+__device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c, int K, bool row_in, const F8Out& o) {
     float a = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -133,10 +133,10 @@ __device__ __forceinline__ void f8_emit(const float (*v)[8], float rs, long long
         for (int i = 0; i < 8; ++i) a = fmaxf(a, fabsf(v[h][i]));
 #pragma unroll
     for (int s = 4; s > 0; s >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, s));
-    const bool large = a * rs >= F8_TINY;         // (false for a row's NaN)
-    const float inv = __fdiv_rn(F8_TOP, large ? a : F8_TINY) * (large ? 1.f : rs);
+    a = fmaxf(a, F8_TINY);
+    const float inv = __fdiv_rn(F8_TOP, a);
     if (!row_in || c >= K) return;
-    if ((c & (F8_BLOCK - 1)) == 0) o.scales[(c / F8_BLOCK) * o.lds + m] = __fdiv_rn(large ? a * rs : F8_TINY, F8_TOP);
+    if ((c & (F8_BLOCK - 1)) == 0) o.scales[(c / F8_BLOCK) * o.lds + m] = __fdiv_rn(a, F8_TOP);
     unsigned char* p = o.codes + m * o.ld + c;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -213,7 +213,7 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
                     for (int i = 0; i < 8; ++i) y[h][i] = 0.f;
                 }
             }
-            f8_emit<VEC>(y, 1.f, row[u], col[u], K, true, o);
+            f8_emit<VEC>(y, row[u], col[u], K, true, o);
         }
     }
 }
@@ -308,15 +308,15 @@ f8_norm_kernel(const F8NormArgs a) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) load(m + step, c0 + j * a.tpr * 16, p[j]);
             }
+            const float rstd = row_rstd(s, turn);             // y = (x rstd) w in this order: x w may not have a place in f32 where y has
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
+            for (int j = 0; j < PER; ++j) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[j][h][i] *= w[j][h][i];
-            const float rstd = row_rstd(s, turn);
-#pragma unroll
-            for (int j = 0; j < PER; ++j) f8_emit<VEC>(v[j], rstd, m, c0 + j * a.tpr * 16, K, m < a.M, a.o);
+                    for (int i = 0; i < 8; ++i) v[j][h][i] = v[j][h][i] * rstd * w[j][h][i];
+                f8_emit<VEC>(v[j], m, c0 + j * a.tpr * 16, K, m < a.M, a.o);
+            }
         }
     } else {
         for (; base < a.M; base += step, ++turn) {
@@ -346,9 +346,9 @@ f8_norm_kernel(const F8NormArgs a) {
                         q.get(v[h]);
                     }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * w[h][i] : 0.f;
+                    for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * rstd * w[h][i] : 0.f;
                 }
-                f8_emit<VEC>(v, rstd, m, c, K, m < a.M, a.o);
+                f8_emit<VEC>(v, m, c, K, m < a.M, a.o);
             }
         }
     }
@@ -415,7 +415,7 @@ static int f8_norm_v(cudaStream_t st, F8NormArgs& a, bool pdl) {
     while (a.tpr < 512 && a.tpr * 16 < (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK) a.tpr *= 2;
     const int block = a.tpr < 256 ? 256 : a.tpr;
     if (a.K <= a.tpr * 16) return f8_norm_p<T, R, VEC, 1>(st, a, block, pdl);
-    if (VEC && a.K <= a.tpr * 32) return f8_norm_p<T, R, VEC, VEC ? 2 : 0>(st, a, block, pdl);
+    if (a.K <= a.tpr * 32) return f8_norm_p<T, R, VEC, 2>(st, a, block, pdl);
     return f8_norm_p<T, R, VEC, 0>(st, a, block, pdl);
 }
 template <typename T, typename R>

@@ -278,6 +278,19 @@ def test_norm_of_zeros_and_infinities():
     assert (back[0] == 0).all() and torch.isnan(back[2]).all() and torch.isnan(back[1, 7])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [300, 512, 9001, 9216, 17000])
+def test_norm_whose_rows_times_weights_pass_f32(k):
+    """x w lies outside of f32 where (x / rms) w does not: powers of two throughout, so y is 2^100 times the signs and every code the type's largest value."""
+    from crane_b200 import fp8
+    g = torch.Generator().manual_seed(k)
+    signs = (torch.randint(0, 2, (3, k), generator=g) * 2 - 1).float()
+    x = (signs * torch.tensor([2.0 ** 50, 2.0 ** 40, 2.0 ** -30])[:, None]).cuda()
+    codes, scales = fp8.rms_norm(x, torch.full((k,), 2.0 ** 100, device="cuda"), 0.0)
+    assert torch.equal(codes.float().cpu(), signs * 448)
+    assert ((scales.cpu() * 448 / 2.0 ** 100 - 1).abs() < 2.0 ** -20).all()            # (a rsqrt of 2 ulp, a product and a quotient; the row's sum of equal squares is exact to k 2^-24 / k)
+
+
 # --------------------------------------------------------------------------------------------------------------------- linears
 SHAPES = [(1, 1, 1), (1, 128, 128), (1, 4096, 2048), (2, 130, 16), (3, 200, 256), (8, 1000, 1037), (15, 129, 4096), (16, 256, 1024), (17, 384, 2048), (31, 1001, 129), (32, 512, 640),
           (33, 24576, 256), (48, 127, 12288), (63, 640, 384), (64, 2048, 1040), (65, 640, 512), (77, 4096, 1536), (127, 300, 300), (128, 128, 4096), (129, 256, 128), (130, 1001, 1037),
