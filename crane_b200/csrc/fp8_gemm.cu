@@ -435,72 +435,80 @@ __device__ __forceinline__ F8Item f8_item(const F8PairArgs& a, int i) {
     const int per = F8_BAND * a.tiles_n, b = t / per, r = t - b * per, w = min(F8_BAND, a.tiles_m - b * F8_BAND), nt = r / w;
     return F8Item{b * F8_BAND + r - nt * w, nt * 256 + sub * width, width};
 }
-// 32 rows x up to C columns of a warp (those below N), a row a lane, through a patch of 32 x 128 bytes (16-byte pieces swizzled by the row), so that stores (and the addend's loads) are of whole
-// lines.  The addition is f32: without an addend values are rounded into the patch, with one they go through it in f32.
-template <typename T, int C>
+// 32 rows x up to C columns of a warp (those below N), a row a lane, through a patch of 32 x 128 bytes (16-byte pieces swizzled by the row), so that stores (and the addend's loads)
+// are of whole lines.  The addition is f32: without an addend values are rounded into the patch, with one they go through it in f32.  Rows that lie on no 16-byte boundaries leave
+// a value a lane, a row at a time.
+// Addends are read a few rows at a time, ahead of those rows' stores: result and addend may be the same memory, so the compiler keeps a load behind every store that is written before it.
+template <typename P, typename T, int C>
 __device__ __forceinline__ void f8_store_rows(const F8Epi& e, bool vec, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
-    constexpr int PER = 16 / (int)sizeof(T), W = 8 * PER;          // elements of a piece, columns of a patch
-    const T* add = static_cast<const T*>(e.add);
-    if (!add) {
+    constexpr int PER = 16 / (int)sizeof(P), W = 8 * PER;          // elements of a piece, columns of a patch
+    using V = typename std::conditional<sizeof(T) * PER == 16, uint4, uint2>::type;
+    const T* add = sizeof(P) == 4 ? static_cast<const T*>(e.add) : nullptr;
+    const int rows = min(32, M - m0);
 #pragma unroll
-        for (int c = 0; c < C; c += W) {
-            if (n0 + c >= N) break;
+    for (int c = 0; c < C; c += W) {
+        if (n0 + c >= N) break;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                alignas(16) T h[PER];
+        for (int p = 0; p < 8; ++p) {
+            alignas(16) P h[PER];
 #pragma unroll
-                for (int i = 0; i < PER; ++i) h[i] = f8_round<T>(c + p * PER + i < C ? v[c + p * PER + i < C ? c + p * PER + i : 0] : 0.f);
-                *reinterpret_cast<uint4*>(patch + sw128_off(lane, p)) = *reinterpret_cast<const uint4*>(h);
+            for (int i = 0; i < PER; ++i) h[i] = f8_round<P>(c + p * PER + i < C ? v[c + p * PER + i < C ? c + p * PER + i : 0] : 0.f);
+            *reinterpret_cast<uint4*>(patch + sw128_off(lane, p)) = *reinterpret_cast<const uint4*>(h);
+        }
+        __syncwarp();
+        if (vec) {
+            const int p = lane & 7, n = n0 + c + p * PER;
+            int r = lane >> 3;
+            T* o = static_cast<T*>(e.out) + (long long)(m0 + r) * e.ldo + n;
+            const T* a = add ? add + (long long)(m0 + r) * e.ldadd + n : nullptr;
+            if (n + PER <= N) {
+                constexpr int G = sizeof(T) == 4 ? 2 : 4;
+#pragma unroll 1
+                for (int i = 0; i < 8; i += G) {
+                    V g[G];
+                    if (add) {
+#pragma unroll
+                        for (int j = 0; j < G; ++j, a += 4LL * e.ldadd) if (r + 4 * j < rows) g[j] = *reinterpret_cast<const V*>(a);
+                    }
+#pragma unroll
+                    for (int j = 0; j < G; ++j, r += 4, o += 4LL * e.ldo) {
+                        alignas(16) P h[PER]; alignas(16) T t[PER];
+                        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(patch + sw128_off(r, p));
+                        if (r >= rows) continue;
+                        if (add) *reinterpret_cast<V*>(t) = g[j];
+#pragma unroll
+                        for (int k = 0; k < PER; ++k) t[k] = f8_round<T>(add ? f8_wide(t[k]) + f8_wide(h[k]) : f8_wide(h[k]));
+                        *reinterpret_cast<V*>(o) = *reinterpret_cast<const V*>(t);
+                    }
+                }
+            } else {
+                for (; r < rows; r += 4, o += 4LL * e.ldo) {
+                    const P* h = reinterpret_cast<const P*>(patch + sw128_off(r, p));
+                    for (int k = 0; n + k < N; ++k) o[k] = f8_round<T>(add ? f8_wide(a[k]) + f8_wide(h[k]) : f8_wide(h[k]));
+                    if (add) a += 4LL * e.ldadd;
+                }
             }
-            __syncwarp();
+        } else {
+            for (int q = lane; q < W && n0 + c + q < N; q += 32) {
+                const int at = q * (int)sizeof(P), n = n0 + c + q;
+                T* o = static_cast<T*>(e.out) + (long long)m0 * e.ldo + n;
+                const T* a = add ? add + (long long)m0 * e.ldadd + n : nullptr;
+#pragma unroll 1
+                for (int r = 0; r < rows; r += 8) {
+                    T x[8];
+                    if (add) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3), p = lane & 7, m = m0 + r, n = n0 + c + p * PER;
-                const uint4 u = *reinterpret_cast<const uint4*>(patch + sw128_off(r, p));
-                if (m < M && n < N) {
-                    T* o = static_cast<T*>(e.out) + (long long)m * e.ldo + n;
-                    if (vec && n + PER <= N) *reinterpret_cast<uint4*>(o) = u;
-                    else {
-                        alignas(16) T h[PER];
-                        *reinterpret_cast<uint4*>(h) = u;
+                        for (int i = 0; i < 8; ++i, a += e.ldadd) if (r + i < rows) x[i] = *a;
+                    }
 #pragma unroll
-                        for (int j = 0; j < PER; ++j) if (n + j < N) o[j] = h[j];
+                    for (int i = 0; i < 8; ++i, o += e.ldo) {
+                        const float h = f8_wide(*reinterpret_cast<const P*>(patch + sw128_off(r + i, at >> 4) + (at & 15)));
+                        if (r + i < rows) *o = f8_round<T>(add ? f8_wide(x[i]) + h : h);
                     }
                 }
             }
-            __syncwarp();
         }
-    } else {
-#pragma unroll
-        for (int c = 0; c < C; c += 32) {
-            if (n0 + c >= N) break;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) *reinterpret_cast<float4*>(patch + sw128_off(lane, p)) = make_float4(v[c + 4 * p], v[c + 4 * p + 1], v[c + 4 * p + 2], v[c + 4 * p + 3]);
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3), p = lane & 7, m = m0 + r, n = n0 + c + p * 4;
-                const float4 u = *reinterpret_cast<const float4*>(patch + sw128_off(r, p));
-                if (m < M && n < N) {
-                    T* o = static_cast<T*>(e.out) + (long long)m * e.ldo + n;
-                    const T* a = add + (long long)m * e.ldadd + n;
-                    alignas(16) T h[4];
-                    if (vec && n + 4 <= N) {
-                        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(a);
-                        else *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(a);
-                        h[0] = f8_round<T>(f8_wide(h[0]) + u.x); h[1] = f8_round<T>(f8_wide(h[1]) + u.y);
-                        h[2] = f8_round<T>(f8_wide(h[2]) + u.z); h[3] = f8_round<T>(f8_wide(h[3]) + u.w);
-                        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
-                        else *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(h);
-                    } else {
-                        const float w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) if (n + j < N) o[j] = f8_round<T>(f8_wide(a[j]) + w[j]);
-                    }
-                }
-            }
-            __syncwarp();
-        }
+        __syncwarp();
     }
 }
 
@@ -578,7 +586,8 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensor
     }
     if (lane == 0) tma_store_wait_read<0>();          // (the whole tiles' stores have left the patch)
     __syncwarp();
-    f8_store_rows<T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
+    if (a.ep.add) f8_store_rows<float, T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
+    else f8_store_rows<T, T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
 }
 
 // Registers: 384 threads x 168 at the launch = 128 x 72 (warps 0 - 3) + 256 x 216 (the epilogue: 128 sums and 32 of the next products a thread)
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(F8_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
 f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW32,
                const __grid_constant__ CUtensorMap tmO, const F8PairArgs a) {
     using Cfg = F8PairCfg;
-    constexpr int STAGE = Cfg::STAGE, STAGES = Cfg::STAGES, C = 128;
+    constexpr int STAGE = Cfg::STAGE, STAGES = Cfg::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full[STAGES];                 // of the even CTA: both CTAs' operands of a stage
@@ -755,14 +764,18 @@ static int f8_pair_launch(cudaStream_t st, const F8Linear& p, int M, int N, int 
 //   77 x 4096 x 2048 7.1 / 7.8 / 8.3 / 11.5   77 x 12288 x 2048 15.9 / 11.0 / 12.9 / 13.3   128 x 4096 x 12288 18.2 / 22.6 / 19.0 / 48   128 x 24576 x 4096 42 / 48 / 41 / 39
 //   256 x 4096 x 4096 13.0 / 16.3 / 13.8 / 19.1   256 x 12288 x 2048 25.7 / 21.3 / 25.7 / 14.1   512 x 2048 x 6144 17.2 / 21.8 / 17.5 / 26.8   512 x 4096 x 2048 16.9 / 20.3 / 13.3 / 13.0
 //   700 x 2048 x 6144 - / 22.0 / 28.2 / 29.3   1024 x 4096 x 4096 - / - / 40.7 / 22.2
-// A CTA takes c us a block of K (in two turns a tenth, in more a quarter more), a pair 0.45, whatever the width of its strip: an MMA of 256 rows takes some 125 cycles with 64 to 256
-// columns, so that strips shorten the last turn by their stores and their scales only (1111 x 4096 x 2048 20.5 / 18.7, 256 x 24576 x 4096 38.4 / 37.1, none 400 x 4096 x 4096 19.7 / 20.4).
+//   4096 x 12288 x 128 168 / 134 / 124 / 21.9   4096 x 12288 x 512 200 / 168 / 157 / 40   1500 x 13624 x 116 73 / 59 / 55 / 13.8   82 x 22704 x 1058 22.7 / 18.4 / 21.0 / 15.3
+//   2935 x 560 x 1340 14.5 / 17.4 / 11.7 / 10.7   5512 x 480 x 8249 64 / 55 / 72 / 39   291 x 8344 x 801 19.1 / 16.5 / 17.8 / 9.5   66 x 3616 x 378 5.0 / 5.6 / 6.3 / 6.4
+// Each turn of CTAs takes t0 us, its launch and its stores, and c us a block of K.  Pairs stay: a turn is their blocks of K, 0.45 us each whatever the width of a strip (an MMA of 256 rows
+// takes some 125 cycles with 64 to 256 columns, so that strips shorten the last turn by their stores and their scales only: 1111 x 4096 x 2048 20.5 / 18.7, 256 x 24576 x 4096 38.4 / 37.1,
+// none 400 x 4096 x 4096 19.7 / 20.4), and the part of the stores that the next tile's MMAs do not cover.  Over 48 sizes drawn between 65 x 64 x 64 and 8192 x 24576 x 12288 the choice takes
+// 0.1 % longer than the best of the four.
 template <int CW>
 static double f8_rows_us(int M, int N, int KB, double t0, double c) {
     const long long tiles = (long long)((N + 127) / 128) * ((M + 2 * CW - 1) / (2 * CW));
     const int cl = f8_rows_cluster<CW, 1>(tiles, KB), sms = tc_device_sms();
     const long long turns = cl > 1 ? 1 : (tiles + sms - 1) / sms;
-    return t0 + (cl > 1 ? 0.3 * cl : 0.) + c * (turns > 2 ? 1.25 : turns > 1 ? 1.1 : 1.) * (double)turns * ((KB + cl - 1) / cl);
+    return (double)turns * (t0 + c * ((KB + cl - 1) / cl)) + (cl > 1 ? 0.3 * cl : 0.);
 }
 
 int f8_linear_launch(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
@@ -778,8 +791,8 @@ int f8_linear_launch(cudaStream_t st, const F8Linear& p, int M, int N, int K, bo
         return f8_rows_gemm_t<32, 1>(st, p, M, N, K, pdl);
     }
     const int KB = f8_blocks(K), pairs = tc_device_sms() / 2, turns = (f8_turns(M, N, pairs).items + pairs - 1) / pairs;
-    const double us32 = f8_rows_us<32>(M, N, KB, 4.4, 0.29), us48 = f8_rows_us<48>(M, N, KB, 5.3, 0.40), us64 = f8_rows_us<64>(M, N, KB, 5.9, 0.48);
-    const double us_pair = 5.0 + 0.445 * turns * KB + 3. * (turns - 1), us_rows = std::min(us32, std::min(us48, us64));
+    const double us32 = f8_rows_us<32>(M, N, KB, 4.2, 0.295), us48 = f8_rows_us<48>(M, N, KB, 5.2, 0.38), us64 = f8_rows_us<64>(M, N, KB, 5.9, 0.49);
+    const double us_pair = 4.6 + 0.45 * turns * KB + 1.5 * (turns - 1), us_rows = std::min(us32, std::min(us48, us64));
     if (us_pair < us_rows) return f8_pair_launch(st, p, M, N, K, pdl);
     if (us_rows == us32) return f8_rows_gemm_t<32, 1>(st, p, M, N, K, pdl);
     if (us_rows == us48) return f8_rows_gemm_t<48, 1>(st, p, M, N, K, pdl);
