@@ -39,6 +39,48 @@ __device__ __forceinline__ void f8_unpack(const uint4& u, __half, float* v) {
         v[2 * i] = f.x; v[2 * i + 1] = f.y;
     }
 }
+// A thread has 16 columns of a block of 128, 8 from f8_col on and 8 from 64 behind those, 8 neighbouring threads the block.
+__device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
+// Rows on 16-byte boundaries (VEC) are read and written as that.  Others are read as the aligned pieces that hold them, of which the values are shifted out, and written one element at a
+// time: there the eight threads of a block change values among themselves and take every eighth column, so that an instruction covers whole pieces of a row and not a value of each (all by elements, each thread its own: 8192 x 11001 to codes 113 us from f32, 70 from bf16, 583 f16 behind a norm
+// with a residual; so 69, 62, 277).
+__device__ __forceinline__ int f8_eighth(int c) { return (c & ~63) + ((c >> 3) & 7); }                   // the first of those, 8 to the next
+// 8 threads' 8 values each, transposed: value i of thread t becomes value t of thread i.  Every lane calls
+__device__ __forceinline__ void f8_turn(float* v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int b = 4; b > 0; b >>= 1) {
+        const bool up = lane & b;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i & b) continue;
+            const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + b], b);
+            if (up) v[i] = got; else v[i + b] = got;
+        }
+    }
+}
+template <typename T>                              // 16-bit values
+__device__ __forceinline__ void f8_turn(T* v) {
+    const int lane = threadIdx.x & 31;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(v + 2 * i) | (uint32_t)*reinterpret_cast<const uint16_t*>(v + 2 * i + 1) << 16;
+#pragma unroll
+    for (int b = 2; b > 0; b >>= 1) {
+        const bool up = lane & (2 * b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i & b) continue;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? w[i] : w[i + b], 2 * b);
+            if (up) w[i] = got; else w[i + b] = got;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[i] = __byte_perm(w[i], __shfl_xor_sync(0xffffffffu, w[i], 1), lane & 1 ? 0x3276 : 0x5410);
+        *reinterpret_cast<uint16_t*>(v + 2 * i) = (uint16_t)w[i]; *reinterpret_cast<uint16_t*>(v + 2 * i + 1) = (uint16_t)(w[i] >> 16);
+    }
+}
 // columns c .. c + 7 of a row of K; zeros behind the last.  `vec`: whole chunks of the row lie on 16-byte boundaries
 template <typename T>
 __device__ __forceinline__ void f8_load8(const T* row, int c, int K, bool vec, float* v) {
@@ -62,12 +104,12 @@ __device__ __forceinline__ void f8_load8(const void* base, int type, long long a
 // What a chunk brings, as it is loaded: to be asked for well ahead of its use, it must not be unpacked where it is loaded.  VEC: every chunk is whole and on its boundary.
 template <typename T, bool VEC> struct F8Chunk {
     uint4 q[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* row, int c, int, bool in) {
+    __device__ __forceinline__ void load(const T* row, int c, int, bool in, const T*, const T*) {
         q[0] = in ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0, 0, 0, 0);
         if constexpr (sizeof(T) == 4) q[1] = in ? *reinterpret_cast<const uint4*>(row + c + 4) : make_uint4(0, 0, 0, 0);
         else static_assert(sizeof(q) == 16, "one piece");
     }
-    __device__ __forceinline__ void get(float* v) const {
+    __device__ __forceinline__ void get(float* v, int, int) const {
         if constexpr (sizeof(T) == 4) {
             v[0] = __uint_as_float(q[0].x); v[1] = __uint_as_float(q[0].y); v[2] = __uint_as_float(q[0].z); v[3] = __uint_as_float(q[0].w);
             v[4] = __uint_as_float(q[1].x); v[5] = __uint_as_float(q[1].y); v[6] = __uint_as_float(q[1].z); v[7] = __uint_as_float(q[1].w);
@@ -75,19 +117,57 @@ template <typename T, bool VEC> struct F8Chunk {
     }
 };
 template <typename T> struct F8Chunk<T, false> {
-    T q[8];
-    __device__ __forceinline__ void load(const T* row, int c, int K, bool) {
+    static constexpr int W = sizeof(T) == 4 ? 3 : 2;               // aligned pieces that hold 8 values
+    uint4 q[W];
+    int s;                                                         // bytes ahead of the values
+    // `first`, `end`: of all rows.  A piece may hold values of a neighbouring row, or what lies between the two, but nothing outside of these
+    __device__ __forceinline__ void load(const T* row, int c, int, bool in, const T* first, const T* end) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row + c), w = at & ~(uintptr_t)15;
+        s = (int)(at & 15);
+        if (!in) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = c + i < K ? row[c + i] : T(0.f);
+            for (int j = 0; j < W; ++j) q[j] = make_uint4(0, 0, 0, 0);
+        } else if (w >= reinterpret_cast<uintptr_t>(first) && w + 16 * W <= reinterpret_cast<uintptr_t>(end)) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) q[j] = reinterpret_cast<const uint4*>(w)[j];
+        } else {
+            alignas(16) T t[16 * W / sizeof(T)];
+#pragma unroll
+            for (int j = 0; j < 16 * W / (int)sizeof(T); ++j) {
+                const T* p = reinterpret_cast<const T*>(w) + j;
+                t[j] = p >= first && p < end ? *p : T(0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) q[j] = reinterpret_cast<const uint4*>(t)[j];
+        }
     }
-    __device__ __forceinline__ void get(float* v) const {
+    __device__ __forceinline__ void get(float* v, int c, int K) const {
+        uint32_t w[4 * W];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = f8_float(q[i]);
+        for (int j = 0; j < W; ++j) { w[4 * j] = q[j].x; w[4 * j + 1] = q[j].y; w[4 * j + 2] = q[j].z; w[4 * j + 3] = q[j].w; }
+        constexpr int N = 2 * (int)sizeof(T);                      // words of 8 values
+#pragma unroll
+        for (int j = 0; j < N + 2 && j + 2 < 4 * W; ++j) w[j] = s & 8 ? w[j + 2] : w[j];
+#pragma unroll
+        for (int j = 0; j < N + 1 && j + 1 < 4 * W; ++j) w[j] = s & 4 ? w[j + 1] : w[j];
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+            const uint32_t by = s & 2 ? 0x5432 : 0x3210;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __byte_perm(w[j], w[j + 1], by);
+            f8_unpack(make_uint4(w[0], w[1], w[2], w[3]), T(), v);
+        }
+        if (c + 8 > K) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (c + i >= K) v[i] = 0.f;
+        }
     }
 };
-// h = v rounded to the type, stored and given back in f32
+// h = v rounded to the type, stored where the row is one and given back in f32.  Every lane calls
 template <typename T, bool VEC>
-__device__ __forceinline__ void f8_store8(T* row, int c, int K, float* v) {
+__device__ __forceinline__ void f8_store8(T* row, int c, int K, bool row_in, float* v) {
     alignas(16) T h[8];
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
@@ -108,11 +188,13 @@ __device__ __forceinline__ void f8_store8(T* row, int c, int K, float* v) {
         }
     }
     if constexpr (VEC) {
+        if (!row_in || c >= K) return;
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(h)[i];
     } else {
+        f8_turn(h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) if (c + i < K) row[c + i] = h[i];
+        for (int i = 0; i < 8; ++i) if (row_in && f8_eighth(c) + 8 * i < K) row[f8_eighth(c) + 8 * i] = h[i];
     }
 }
 
@@ -121,8 +203,6 @@ __device__ __forceinline__ uint32_t f8_quad(float a, float b, float c, float d) 
     asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}" : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
-// A thread has 16 columns of a block of 128, 8 from 8 (lane % 8) on and 8 from 64 behind those, 8 neighbouring threads the block.
-__device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
 // Scale and codes of a thread's 16 columns.  Every lane of the warp calls
 template <bool VEC>
 __device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c, int K, bool row_in, const F8Out& o) {
@@ -175,6 +255,7 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
     const int dm = (int)(warps / per), dc = (int)(warps % per);             // a step of all warps: rows and pieces
     long long m = w / per;
     int piece = (int)(w % per);
+    const T* x_end = x + (M - 1) * ldx + (GATED ? 2 : 1) * K;
     pdl_wait();
     pdl_launch_dependents();
     while (m < M) {
@@ -189,8 +270,8 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
             for (int h = 0; h < 2; ++h) {
                 const int c = col[u] + 64 * h;
                 const bool in = m < M && c < K;
-                if constexpr (GATED) g[u][h].load(at, in ? c : 0, K, in);
-                v[u][h].load(at + (GATED ? K : 0), in ? c : 0, K, in);
+                if constexpr (GATED) g[u][h].load(at, in ? c : 0, K, in, x, x_end);
+                v[u][h].load(at + (GATED ? K : 0), in ? c : 0, K, in, x, x_end);
             }
             m += dm; piece += dc;
             if (piece >= per) { piece -= per; ++m; }
@@ -201,16 +282,12 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
             float y[2][8];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                v[u][h].get(y[h]);
+                v[u][h].get(y[h], col[u] + 64 * h, K);
                 if constexpr (GATED) {
                     float gate[8];
-                    g[u][h].get(gate);
+                    g[u][h].get(gate, col[u] + 64 * h, K);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) y[h][i] = f8_silu_mul(gate[i], y[h][i]);
-                }
-                if (!VEC && col[u] + 64 * h >= K) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) y[h][i] = 0.f;
                 }
             }
             f8_emit<VEC>(y, row[u], col[u], K, true, o);
@@ -228,10 +305,12 @@ f8_norm_kernel(const F8NormArgs a) {
     constexpr bool RES = !std::is_same<R, void>::value;
     using RT = typename std::conditional<RES, R, T>::type;
     __shared__ float red[2][16];
-    const int t = threadIdx.x & (a.tpr - 1), sub = threadIdx.x / a.tpr, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K, rpb = blockDim.x / a.tpr;
+    const int rpb = blockDim.x / a.tpr, sub = threadIdx.x / a.tpr, t = threadIdx.x - sub * a.tpr, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, K = a.K;
     const T* x = static_cast<const T*>(a.n.x);
     const RT* res = static_cast<const RT*>(a.n.residual);
     RT* res_out = static_cast<RT*>(a.n.residual_out);
+    const T* x_end = x + (a.M - 1) * a.n.ldx + K;
+    const long long r_len = (a.M - 1) * a.n.ldr + K;
     struct Piece { F8Chunk<T, VEC> x[2]; F8Chunk<RT, VEC> r[2]; };
     auto load = [&](long long m, int c0, Piece& p) {
         const long long at = m < a.M ? m : 0;
@@ -239,27 +318,23 @@ f8_norm_kernel(const F8NormArgs a) {
         for (int h = 0; h < 2; ++h) {
             const int c = c0 + 64 * h;
             const bool in = m < a.M && c < K;
-            p.x[h].load(x + at * a.n.ldx, in ? c : 0, K, in);
-            if constexpr (RES) p.r[h].load(res + at * a.n.ldr, in ? c : 0, K, in);
+            p.x[h].load(x + at * a.n.ldx, in ? c : 0, K, in, x, x_end);
+            if constexpr (RES) p.r[h].load(res + at * a.n.ldr, in ? c : 0, K, in, res, res + r_len);
         }
     };
     auto sum = [&](long long m, int c0, const Piece& p, float (*v)[8]) {       // h of 16 columns, stored where there is a residual -> their squares
+        const long long at = m < a.M ? m : 0;
         float s = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int c = c0 + 64 * h;
-            const bool in = m < a.M && c < K;
-            p.x[h].get(v[h]);
+            p.x[h].get(v[h], c, K);
             if constexpr (RES) {
                 float r[8];
-                p.r[h].get(r);
+                p.r[h].get(r, c, K);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[h][i] += r[i];
-                if (in) f8_store8<RT, VEC>(res_out + m * a.n.ldr, c, K, v[h]);
-            }
-            if (!VEC && !in) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[h][i] = 0.f;
+                f8_store8<RT, VEC>(res_out + at * a.n.ldr, c, K, m < a.M, v[h]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) s += v[h][i] * v[h][i];
@@ -269,7 +344,7 @@ f8_norm_kernel(const F8NormArgs a) {
     auto row_rstd = [&](float s, int turn) {
         s = warp_sum(s);
         if (a.tpr > 32) {
-            const int nw = a.tpr >> 5, w0 = warp & ~(nw - 1);
+            const int nw = a.tpr >> 5, w0 = sub * nw;
             if (lane == 0) red[turn & 1][warp] = s;
             __syncthreads();                        // (the other half of `red` is the next row's: nobody is still reading it)
             s = warp_sum(lane < nw ? red[turn & 1][w0 + lane] : 0.f);
@@ -294,17 +369,24 @@ f8_norm_kernel(const F8NormArgs a) {
     pdl_launch_dependents();
     if constexpr (PER > 0) {
         float w[PER][2][8];
+        constexpr bool AHEAD = VEC || PER == 1 || !RES;       // (the pieces of 32 columns and a residual's would not stay in registers: 2048 x 9290 bf16 and f32 114 us so, 81 without; of 16 columns they do: 8192 x 4099 bf16 112, 124 without)
         Piece p[PER];
+        if (AHEAD) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) load(base + sub, c0 + j * a.tpr * 16, p[j]);
+            for (int j = 0; j < PER; ++j) load(base + sub, c0 + j * a.tpr * 16, p[j]);
+        }
 #pragma unroll
         for (int j = 0; j < PER; ++j) weights(c0 + j * a.tpr * 16, w[j]);
         for (; base < a.M; base += step, ++turn) {
             const long long m = base + sub;
             float v[PER][2][8], s = 0.f;
+            if (!AHEAD) {
+#pragma unroll
+                for (int j = 0; j < PER; ++j) load(m, c0 + j * a.tpr * 16, p[j]);
+            }
 #pragma unroll
             for (int j = 0; j < PER; ++j) s += sum(m, c0 + j * a.tpr * 16, p[j], v[j]);
-            if (base + step < a.M) {
+            if (AHEAD && base + step < a.M) {
 #pragma unroll
                 for (int j = 0; j < PER; ++j) load(m + step, c0 + j * a.tpr * 16, p[j]);
             }
@@ -322,14 +404,14 @@ f8_norm_kernel(const F8NormArgs a) {
         for (; base < a.M; base += step, ++turn) {
             const long long m = base + sub;
             float s = 0.f;
-            for (int c = c0; c < K; c += a.tpr * 16) {
+            for (int i0 = 0; i0 < K; i0 += a.tpr * 16) {        // (all threads alike: shuffles)
                 Piece p;
                 float v[2][8];
-                load(m, c, p);
-                s += sum(m, c, p, v);
+                load(m, i0 + c0, p);
+                s += sum(m, i0 + c0, p, v);
             }
             const float rstd = row_rstd(s, turn);
-            for (int i0 = 0; i0 < K; i0 += a.tpr * 16) {        // (all threads alike: shuffles)
+            for (int i0 = 0; i0 < K; i0 += a.tpr * 16) {
                 const int c = i0 + c0;
                 float v[2][8], w[2][8];
                 weights(c, w);
@@ -338,12 +420,12 @@ f8_norm_kernel(const F8NormArgs a) {
                     const bool in = m < a.M && c + 64 * h < K;
                     if constexpr (RES) {
                         F8Chunk<RT, VEC> q;
-                        q.load(static_cast<const RT*>(res_out) + (in ? m : 0) * a.n.ldr, in ? c + 64 * h : 0, K, in);
-                        q.get(v[h]);
+                        q.load(static_cast<const RT*>(res_out) + (in ? m : 0) * a.n.ldr, in ? c + 64 * h : 0, K, in, res_out, res_out + r_len);
+                        q.get(v[h], c + 64 * h, K);
                     } else {
                         F8Chunk<T, VEC> q;
-                        q.load(x + (in ? m : 0) * a.n.ldx, in ? c + 64 * h : 0, K, in);
-                        q.get(v[h]);
+                        q.load(x + (in ? m : 0) * a.n.ldx, in ? c + 64 * h : 0, K, in, x, x_end);
+                        q.get(v[h], c + 64 * h, K);
                     }
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[h][i] = in ? v[h][i] * rstd * w[h][i] : 0.f;
@@ -404,16 +486,16 @@ int f8_silu_mul_launch(cudaStream_t st, const void* x, int type, long long ldx, 
 
 template <typename T, typename R, bool VEC, int PER>
 static int f8_norm_p(cudaStream_t st, const F8NormArgs& a, int block, bool pdl) {
-    static std::atomic<int> known[2][CB_MAX_DEV];               // by the block's size
+    static std::atomic<int> known[17][CB_MAX_DEV];              // by the block's warps
     const int rows = block / a.tpr;
-    const long long blocks = std::min<long long>((a.M + rows - 1) / rows, f8_resident(f8_norm_kernel<T, R, VEC, PER>, block, known[block > 256]));
+    const long long blocks = std::min<long long>((a.M + rows - 1) / rows, f8_resident(f8_norm_kernel<T, R, VEC, PER>, block, known[block / 32]));
     return launch_k(f8_norm_kernel<T, R, VEC, PER>, dim3((unsigned)blocks), dim3(block), 0, st, pdl, a);
 }
 template <typename T, typename R, bool VEC>
 static int f8_norm_v(cudaStream_t st, F8NormArgs& a, bool pdl) {
-    a.tpr = 32;
-    while (a.tpr < 512 && a.tpr * 16 < (a.K + F8_BLOCK - 1) / F8_BLOCK * F8_BLOCK) a.tpr *= 2;
-    const int block = a.tpr < 256 ? 256 : a.tpr;
+    // whole warps for a row, as few as have its columns (power of two: 8192 x 4099 bf16 and a residual 133 us, so 112); a block of about 256 threads
+    a.tpr = std::min(512, (a.K + F8_BLOCK - 1) / F8_BLOCK * 8 + 31 & ~31);
+    const int block = a.tpr * std::max(1, 256 / a.tpr);
     if (a.K <= a.tpr * 16) return f8_norm_p<T, R, VEC, 1>(st, a, block, pdl);
     if (a.K <= a.tpr * 32) return f8_norm_p<T, R, VEC, 2>(st, a, block, pdl);
     return f8_norm_p<T, R, VEC, 0>(st, a, block, pdl);

@@ -279,6 +279,31 @@ def test_norm_of_zeros_and_infinities():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("k", [1, 7, 8, 130, 519, 2049, 4099, 9001, 17001])
+@pytest.mark.parametrize("dt", TYPES)
+def test_rows_on_every_boundary(dt, k):
+    """Rows from every offset inside 16 bytes, NaN between and around them: the bits of rows that lie together, and nothing between them is written."""
+    from crane_b200 import fp8
+    gen, t = gen_of("boundary", k, dt), TYPES[dt]
+    x, gated, r = (rows_of(gen, 5, n, t) for n in (k, 2 * k, k))
+    w = 1 + 0.2 * torch.randn(k, generator=gen, device="cuda")
+
+    def among(v, off):
+        wide = torch.full((5 * (v.shape[1] + 3) + off + 8,), math.nan, dtype=t, device="cuda")
+        at = wide[off:off + 5 * (v.shape[1] + 3)].view(5, -1)[:, :v.shape[1]]
+        at.copy_(v)
+        return at, wide
+    alike = lambda a, b: torch.equal(a[0].view(torch.uint8), b[0].view(torch.uint8)) and torch.equal(a[1], b[1])  # noqa: E731
+    plain, unit, sums = fp8.quantize(x), fp8.silu_mul(gated), (x.float() + r.float()).to(t)
+    alone, normed = fp8.rms_norm(x, w, 1e-5), fp8.rms_norm(x, w, 1e-5, residual=r.clone())
+    for off in range(8):
+        xo, (ro, room) = among(x, off)[0], among(r, 7 - off)
+        assert alike(fp8.quantize(xo), plain) and alike(fp8.silu_mul(among(gated, off)[0]), unit) and alike(fp8.rms_norm(xo, w, 1e-5), alone)
+        assert alike(fp8.rms_norm(xo, w, 1e-5, residual=ro), normed)
+        assert torch.equal(ro, sums) and int(torch.isnan(room).sum()) == room.numel() - 5 * k
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("k", [300, 512, 9001, 9216, 17000])
 def test_norm_whose_rows_times_weights_pass_f32(k):
     """x w lies outside of f32 where (x / rms) w does not: powers of two throughout, so y is 2^100 times the signs and every code the type's largest value."""
