@@ -416,7 +416,7 @@ struct F8PairArgs {
     long long lds, ldws;
     int M, N, KB, tiles_m, tiles_n, pairs;
     int whole, items, cut;             // tiles 0 .. whole - 1 as they are, then strips of 256 / cut columns: `items` together
-    bool vec, tma, w_static;
+    bool tma, w_static;
     int* err;
 };
 constexpr int F8_BAND = 8;                         // rows of tiles that are walked together: neighbours in time share weights and activations in L2
@@ -435,14 +435,53 @@ __device__ __forceinline__ F8Item f8_item(const F8PairArgs& a, int i) {
     const int per = F8_BAND * a.tiles_n, b = t / per, r = t - b * per, w = min(F8_BAND, a.tiles_m - b * F8_BAND), nt = r / w;
     return F8Item{b * F8_BAND + r - nt * w, nt * 256 + sub * width, width};
 }
-// 32 rows x up to C columns of a warp (those below N), a row a lane, through a patch of 32 x 128 bytes (16-byte pieces swizzled by the row), so that stores (and the addend's loads)
-// are of whole lines.  The addition is f32: without an addend values are rounded into the patch, with one they go through it in f32.  Rows that lie on no 16-byte boundaries leave
-// a value a lane, a row at a time.
-// Addends are read a few rows at a time, ahead of those rows' stores: result and addend may be the same memory, so the compiler keeps a load behind every store that is written before it.
+// 32 rows x up to C columns of a warp (those below N), a row a lane, through a patch of 32 x 32 f32 (16-byte pieces swizzled by the row), so that stores (and the addend's loads) cover
+// pieces of rows.  The addition is f32.  Addends are read ahead of all stores: result and addend may be the same memory, so the compiler keeps a load behind every store that is written
+// before it (8192 x 24576 x 64 f32 669 us so, 345 ahead).
+template <typename T, int C, bool ADD>
+__device__ __forceinline__ void f8_store_rows(const F8Epi& e, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
+    using V = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+    const int r0 = lane >> 3, p0 = lane & 7;
+#pragma unroll
+    for (int c = 0; c < C; c += 32) {
+        if (n0 + c >= N) break;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) *reinterpret_cast<float4*>(patch + sw128_off(lane, p)) = make_float4(v[c + 4 * p], v[c + 4 * p + 1], v[c + 4 * p + 2], v[c + 4 * p + 3]);
+        __syncwarp();
+        const int n = n0 + c + p0 * 4;
+        const T* add = ADD ? static_cast<const T*>(e.add) + n : nullptr;
+        V g[8];
+        if (ADD && n + 4 <= N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (m0 + 4 * i + r0 < M) g[i] = *reinterpret_cast<const V*>(add + (long long)(m0 + 4 * i + r0) * e.ldadd);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = 4 * i + r0, m = m0 + r;
+            const float4 u = *reinterpret_cast<const float4*>(patch + sw128_off(r, p0));
+            if (m >= M || n >= N) continue;
+            T* o = static_cast<T*>(e.out) + (long long)m * e.ldo + n;
+            const float w[4] = {u.x, u.y, u.z, u.w};
+            if (n + 4 <= N) {
+                alignas(16) T h[4];
+                if (ADD) *reinterpret_cast<V*>(h) = g[i];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[j] = f8_round<T>(ADD ? f8_wide(h[j]) + w[j] : w[j]);
+                *reinterpret_cast<V*>(o) = *reinterpret_cast<const V*>(h);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) if (n + j < N) o[j] = f8_round<T>(ADD ? f8_wide(add[(long long)m * e.ldadd + j]) + w[j] : w[j]);
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// The same for rows that lie on no 16-byte boundaries: a value a lane, a row at a time.  Addends are read eight rows at a time, ahead of those rows' stores: result and addend may be the
+// same memory, so the compiler keeps a load behind every store that is written before it.
 template <typename P, typename T, int C>
-__device__ __forceinline__ void f8_store_rows(const F8Epi& e, bool vec, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
-    constexpr int PER = 16 / (int)sizeof(P), W = 8 * PER;          // elements of a piece, columns of a patch
-    using V = typename std::conditional<sizeof(T) * PER == 16, uint4, uint2>::type;
+__device__ __forceinline__ void f8_store_odd(const F8Epi& e, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
+    constexpr int PER = 16 / (int)sizeof(P), W = 8 * PER;
     const T* add = sizeof(P) == 4 ? static_cast<const T*>(e.add) : nullptr;
     const int rows = min(32, M - m0);
 #pragma unroll
@@ -456,55 +495,21 @@ __device__ __forceinline__ void f8_store_rows(const F8Epi& e, bool vec, int M, i
             *reinterpret_cast<uint4*>(patch + sw128_off(lane, p)) = *reinterpret_cast<const uint4*>(h);
         }
         __syncwarp();
-        if (vec) {
-            const int p = lane & 7, n = n0 + c + p * PER;
-            int r = lane >> 3;
-            T* o = static_cast<T*>(e.out) + (long long)(m0 + r) * e.ldo + n;
-            const T* a = add ? add + (long long)(m0 + r) * e.ldadd + n : nullptr;
-            if (n + PER <= N) {
-                constexpr int G = sizeof(T) == 4 ? 2 : 4;
+        for (int q = lane; q < W && n0 + c + q < N; q += 32) {
+            const int at = q * (int)sizeof(P), n = n0 + c + q;
+            T* o = static_cast<T*>(e.out) + (long long)m0 * e.ldo + n;
+            const T* a = add ? add + (long long)m0 * e.ldadd + n : nullptr;
 #pragma unroll 1
-                for (int i = 0; i < 8; i += G) {
-                    V g[G];
-                    if (add) {
+            for (int r = 0; r < rows; r += 8) {
+                T x[8];
+                if (add) {
 #pragma unroll
-                        for (int j = 0; j < G; ++j, a += 4LL * e.ldadd) if (r + 4 * j < rows) g[j] = *reinterpret_cast<const V*>(a);
-                    }
-#pragma unroll
-                    for (int j = 0; j < G; ++j, r += 4, o += 4LL * e.ldo) {
-                        alignas(16) P h[PER]; alignas(16) T t[PER];
-                        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(patch + sw128_off(r, p));
-                        if (r >= rows) continue;
-                        if (add) *reinterpret_cast<V*>(t) = g[j];
-#pragma unroll
-                        for (int k = 0; k < PER; ++k) t[k] = f8_round<T>(add ? f8_wide(t[k]) + f8_wide(h[k]) : f8_wide(h[k]));
-                        *reinterpret_cast<V*>(o) = *reinterpret_cast<const V*>(t);
-                    }
+                    for (int i = 0; i < 8; ++i, a += e.ldadd) if (r + i < rows) x[i] = *a;
                 }
-            } else {
-                for (; r < rows; r += 4, o += 4LL * e.ldo) {
-                    const P* h = reinterpret_cast<const P*>(patch + sw128_off(r, p));
-                    for (int k = 0; n + k < N; ++k) o[k] = f8_round<T>(add ? f8_wide(a[k]) + f8_wide(h[k]) : f8_wide(h[k]));
-                    if (add) a += 4LL * e.ldadd;
-                }
-            }
-        } else {
-            for (int q = lane; q < W && n0 + c + q < N; q += 32) {
-                const int at = q * (int)sizeof(P), n = n0 + c + q;
-                T* o = static_cast<T*>(e.out) + (long long)m0 * e.ldo + n;
-                const T* a = add ? add + (long long)m0 * e.ldadd + n : nullptr;
-#pragma unroll 1
-                for (int r = 0; r < rows; r += 8) {
-                    T x[8];
-                    if (add) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i, a += e.ldadd) if (r + i < rows) x[i] = *a;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i, o += e.ldo) {
-                        const float h = f8_wide(*reinterpret_cast<const P*>(patch + sw128_off(r + i, at >> 4) + (at & 15)));
-                        if (r + i < rows) *o = f8_round<T>(add ? f8_wide(x[i]) + h : h);
-                    }
+                for (int i = 0; i < 8; ++i, o += e.ldo) {
+                    const float h = f8_wide(*reinterpret_cast<const P*>(patch + sw128_off(r + i, at >> 4) + (at & 15)));
+                    if (r + i < rows) *o = f8_round<T>(add ? f8_wide(x[i]) + h : h);
                 }
             }
         }
@@ -537,11 +542,17 @@ __device__ __forceinline__ void f8_store_tma(const CUtensorMap* map, int M, int 
 }
 
 // One tile, or strip, of an epilogue warp: C columns of each lane's row
+// How results leave has a kernel each: with other ways beside its own, the loop over K comes out slower (8192 x 24576 x 4096 bf16 745 us with all three in one, so 711)
+enum { F8_PLAIN, F8_ADD, F8_ODD };                    // rows on 16-byte boundaries without an addend, with one, rows on others
 struct F8Ring { uint64_t *full, *empty; int b; uint32_t phases; };
-template <int C, typename T>
+template <int C, typename T, int WAY>
 __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensorMap* tmO, const float* xs, const float* ws, uint32_t lanes, F8Ring& ring, const TcWait& wait, int m0, int n0, int N,
                                              uint8_t* patch, int lane) {
     constexpr int BUFS = 256 / C;
+    if (WAY != F8_PLAIN && a.ep.add && m0 + lane < a.M) {      // the addend's lines come to L2 while the MMAs run (8192 x 24576 x 64 f32 421 us without, 345 so)
+        const char* row = reinterpret_cast<const char*>(static_cast<const T*>(a.ep.add) + (long long)(m0 + lane) * a.ep.ldadd + n0);
+        for (int c = 0; c < (N - n0) * (int)sizeof(T); c += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + c));
+    }
     float v[C];
 #pragma unroll
     for (int j = 0; j < C; ++j) v[j] = 0.f;
@@ -581,20 +592,21 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensor
         ring.phases ^= 1u << ring.b;
         if (++ring.b == BUFS) ring.b = 0;
     }
-    if constexpr (C * sizeof(T) >= 128) {
+    if constexpr (WAY == F8_PLAIN && C * sizeof(T) >= 128) {
         if (a.tma) { f8_store_tma<T, C>(tmO, a.M, N, m0, n0, v, patch, lane); return; }
     }
     if (lane == 0) tma_store_wait_read<0>();          // (the whole tiles' stores have left the patch)
     __syncwarp();
-    if (a.ep.add) f8_store_rows<float, T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
-    else f8_store_rows<T, T, C>(a.ep, a.vec, a.M, N, m0, n0, v, patch, lane);
+    if constexpr (WAY != F8_ODD) f8_store_rows<T, C, WAY == F8_ADD>(a.ep, a.M, N, m0, n0, v, patch, lane);
+    else if (a.ep.add) f8_store_odd<float, T, C>(a.ep, a.M, N, m0, n0, v, patch, lane);
+    else f8_store_odd<T, T, C>(a.ep, a.M, N, m0, n0, v, patch, lane);
 }
 
 // Registers: 384 threads x 168 at the launch = 128 x 72 (warps 0 - 3) + 256 x 216 (the epilogue: 128 sums and 32 of the next products a thread)
 constexpr int F8_PAIR_THREADS = 128 + 32 * F8_EPI, F8_REGS_LOW = 72, F8_REGS_EPI = 216;
 static_assert(128 * F8_REGS_LOW + 32 * F8_EPI * F8_REGS_EPI <= F8_PAIR_THREADS * 168, "the shares come out of the launch's registers");
 //   warp 0: TMA producer    warp 1: TMEM allocator and (even CTA) MMA issuer    warps 4 - 11: epilogue (32 rows from 32 (warp % 4), half of the columns)
-template <typename T>
+template <typename T, int WAY>
 __global__ void __launch_bounds__(F8_PAIR_THREADS, 1) __cluster_dims__(2, 1, 1)
 f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW32,
                const __grid_constant__ CUtensorMap tmO, const F8PairArgs a) {
@@ -702,9 +714,9 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             const float* xs = a.xs + min(m0 + lane, a.M - 1);
             const float* ws = a.ws + (long long)min(n0 / 128, (a.N - 1) / 128) * a.ldws;
             const int N = min(a.N, n0 + cw);
-            if (width == 256) f8_pair_tile<128, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
-            else if (width == 128) f8_pair_tile<64, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
-            else f8_pair_tile<32, T>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            if (width == 256) f8_pair_tile<128, T, WAY>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            else if (width == 128) f8_pair_tile<64, T, WAY>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
+            else f8_pair_tile<32, T, WAY>(a, &tmO, xs, ws, lanes, ring, wait, m0, n0, N, patch, lane);
         }
         if (lane == 0) tma_store_wait_read<0>();      // (the writes themselves are complete when the grid is)
     }
@@ -725,7 +737,7 @@ static F8Turns f8_turns(int M, int N, int pairs) {       // tiles of a pair, tho
     t.items = t.whole + (tiles - t.whole) * t.cut;
     return t;
 }
-template <typename T>
+template <typename T, int WAY>
 static int f8_pair_t(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
     using Cfg = F8PairCfg;
     F8PairArgs a = {};
@@ -737,25 +749,29 @@ static int f8_pair_t(cudaStream_t st, const F8Linear& p, int M, int N, int K, bo
     const F8Turns turns = f8_turns(M, N, pairs);
     a.whole = turns.whole; a.items = turns.items; a.cut = turns.cut;
     a.pairs = std::min(a.items, pairs);
-    a.vec = f8_vec_out(p);
     if (const int err = f8_err_word(st, &a.err)) return err;
     CUtensorMap tmX, tmW, tmW32, tmO;
     if (!tc_tmap_encode(&tmX, p.x.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K, (uint64_t)p.x.ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmW, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmW32, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
-    a.tma = a.vec && !p.add && (long long)N * (long long)sizeof(T) % 16 == 0;      // (a row that ends inside 16 bytes would be written to their end)
+    a.tma = WAY == F8_PLAIN && (long long)N * (long long)sizeof(T) % 16 == 0;      // (a row that ends inside 16 bytes would be written to their end)
     tmO = tmX;
     if (a.tma && !tc_tmap_encode(&tmO, p.out, std::is_same<T, float>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : std::is_same<T, bf16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                                  (uint64_t)M, (uint64_t)N, (uint64_t)p.ldo, 32, 128 / sizeof(T), CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
     static SmemOptIn seen;
-    if (const int err = ensure_dyn_smem(f8_pair_kernel<T>, (size_t)Cfg::SMEM, seen)) return err;
-    return launch_k(f8_pair_kernel<T>, dim3(2 * a.pairs), dim3(F8_PAIR_THREADS), Cfg::SMEM, st, pdl, tmX, tmW, tmW32, tmO, a);
+    if (const int err = ensure_dyn_smem(f8_pair_kernel<T, WAY>, (size_t)Cfg::SMEM, seen)) return err;
+    return launch_k(f8_pair_kernel<T, WAY>, dim3(2 * a.pairs), dim3(F8_PAIR_THREADS), Cfg::SMEM, st, pdl, tmX, tmW, tmW32, tmO, a);
+}
+template <typename T>
+static int f8_pair_p(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
+    if (!f8_vec_out(p)) return f8_pair_t<T, F8_ODD>(st, p, M, N, K, pdl);
+    return p.add ? f8_pair_t<T, F8_ADD>(st, p, M, N, K, pdl) : f8_pair_t<T, F8_PLAIN>(st, p, M, N, K, pdl);
 }
 static int f8_pair_launch(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
     switch (p.type) {
-        case F8_F32:  return f8_pair_t<float>(st, p, M, N, K, pdl);
-        case F8_BF16: return f8_pair_t<bf16>(st, p, M, N, K, pdl);
-        case F8_F16:  return f8_pair_t<__half>(st, p, M, N, K, pdl);
+        case F8_F32:  return f8_pair_p<float>(st, p, M, N, K, pdl);
+        case F8_BF16: return f8_pair_p<bf16>(st, p, M, N, K, pdl);
+        case F8_F16:  return f8_pair_p<__half>(st, p, M, N, K, pdl);
         default: return -1000;
     }
 }
