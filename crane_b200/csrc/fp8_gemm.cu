@@ -6,7 +6,7 @@
 // f8_rows_gemm_kernel, up to some hundred rows: 128 weight rows are the MMA's M, up to 128 activation rows its N.  All weight rows of a tile share a scale, an activation
 // row's scale is a column's: xs * ws of a warp's columns lies in a patch of shared memory that its lanes fill a stage ahead.  Fewer tiles than SMs: a cluster shares a tile
 // along K and adds its partial tiles through distributed shared memory.
-// f8_pair_kernel, more rows: tiles of 256 x 256 over pairs of CTAs.
+// f8_pair_kernel, more rows: tiles of 256 x 256 over pairs of CTAs, a kernel for each way the results leave.
 #include "fp8.cuh"
 #include "tc.cuh"
 

@@ -297,7 +297,7 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
 
 struct F8NormArgs { F8Norm n; long long M; int K, tpr; bool vec_w; F8Out o; };
 // `tpr` threads have a row (a block several, where it has fewer columns than 16 x 256), PER times 16 columns each, in registers between the sum and the codes; PER = 0: wider rows,
-// read again for the codes (what the thread itself stored, where there is a residual).  A block keeps its weights in registers over the rows it takes in turn, and asks for the
+// read again for the codes (what the block stored ahead of the sum's barrier, where there is a residual).  A block keeps its weights in registers over the rows it takes in turn, and asks for the
 // next row before it finishes one.
 template <typename T, typename R, bool VEC, int PER>
 __global__ void __launch_bounds__(512)

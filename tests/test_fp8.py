@@ -376,6 +376,27 @@ def test_linear_leaves_what_lies_around_its_rows(m, n, k, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("m, n, k", [(60, 1001, 256), (129, 260, 128), (700, 1001, 256), (1300, 2085, 384), (2600, 4198, 130), (4900, 4200, 128)])
+def test_linear_of_added_rows_on_every_boundary(m, n, k, dt):
+    """An addend in rows on 16-byte boundaries, ragged at their ends, in place and apart, gives the bits of one on odd boundaries; nothing around the rows is written."""
+    from crane_b200 import fp8
+    gen = gen_of("added", m, n, k, dt)
+    x, xs = fp8.quantize(rows_of(gen, m, k, torch.float32))
+    w, ws = weights(gen, n, k)
+    add = (3 * torch.randn((m, n), generator=gen, device="cuda")).to(TYPES[dt])
+    want = fp8.linear(x, xs, w, ws, add=strided(add, 1, 1), out=strided(add, 2 + n % 2, 1))
+    check_linear(want, linear_ref(x, xs, w, ws, add))
+    wide = torch.full((m + 2, (n + 15) // 8 * 8), 99.0, device="cuda", dtype=TYPES[dt])
+    rows = wide[1:m + 1, :n]
+    rows.copy_(add)
+    assert torch.equal(fp8.linear(x, xs, w, ws, add=rows, out=torch.empty_like(wide)[:m, :n]), want)
+    assert torch.equal(fp8.linear(x, xs, w, ws, add=rows, out=rows), want)
+    assert (wide[0] == 99).all() and (wide[m + 1] == 99).all() and (wide[:, n:] == 99).all()
+    fp8.status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [1, 40, 100, 700])
 def test_linear_keeps_nan_and_infinity_in_their_rows(m):
     from crane_b200 import fp8
