@@ -43,7 +43,7 @@ __device__ __forceinline__ void f8_unpack(const uint4& u, __half, float* v) {
 __device__ __forceinline__ int f8_col(int thread) { return (thread >> 3) * F8_BLOCK + (thread & 7) * 8; }
 // Rows on 16-byte boundaries (VEC) are read and written as that.  Others are read as the aligned pieces that hold them, of which the values are shifted out, and written one element at a
 // time: there the eight threads of a block change values among themselves and take every eighth column, so that an instruction covers whole pieces of a row and not a value of each (all by elements, each thread its own: 8192 x 11001 to codes 113 us from f32, 70 from bf16, 583 f16 behind a norm
-// with a residual; so 69, 62, 277).
+// with a residual; so 72, 67, 291).
 __device__ __forceinline__ int f8_eighth(int c) { return (c & ~63) + ((c >> 3) & 7); }                   // the first of those, 8 to the next
 // 8 threads' 8 values each, transposed: value i of thread t becomes value t of thread i.  Every lane calls
 __device__ __forceinline__ void f8_turn(float* v) {
@@ -120,8 +120,8 @@ template <typename T> struct F8Chunk<T, false> {
     static constexpr int W = sizeof(T) == 4 ? 3 : 2;               // aligned pieces that hold 8 values
     uint4 q[W];
     int s;                                                         // bytes ahead of the values
-    // `first`, `end`: of all rows.  A piece may hold values of a neighbouring row, or what lies between the two, but nothing outside of these
-    __device__ __forceinline__ void load(const T* row, int c, int, bool in, const T* first, const T* end) {
+    // Pieces that hold a byte of the row: what else is in them, between two rows or of the next, is shifted out.  `first`, `end`: of all rows, nothing outside of these is read
+    __device__ __forceinline__ void load(const T* row, int c, int K, bool in, const T* first, const T* end) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(row + c), w = at & ~(uintptr_t)15;
         s = (int)(at & 15);
         if (!in) {
@@ -129,13 +129,13 @@ template <typename T> struct F8Chunk<T, false> {
             for (int j = 0; j < W; ++j) q[j] = make_uint4(0, 0, 0, 0);
         } else if (w >= reinterpret_cast<uintptr_t>(first) && w + 16 * W <= reinterpret_cast<uintptr_t>(end)) {
 #pragma unroll
-            for (int j = 0; j < W; ++j) q[j] = reinterpret_cast<const uint4*>(w)[j];
+            for (int j = 0; j < W; ++j) q[j] = j == 0 || w + 16 * j < reinterpret_cast<uintptr_t>(row + K) ? reinterpret_cast<const uint4*>(w)[j] : make_uint4(0, 0, 0, 0);
         } else {
             alignas(16) T t[16 * W / sizeof(T)];
 #pragma unroll
             for (int j = 0; j < 16 * W / (int)sizeof(T); ++j) {
                 const T* p = reinterpret_cast<const T*>(w) + j;
-                t[j] = p >= first && p < end ? *p : T(0.f);
+                t[j] = p >= row && p < row + K ? *p : T(0.f);
             }
 #pragma unroll
             for (int j = 0; j < W; ++j) q[j] = reinterpret_cast<const uint4*>(t)[j];
@@ -369,7 +369,7 @@ f8_norm_kernel(const F8NormArgs a) {
     pdl_launch_dependents();
     if constexpr (PER > 0) {
         float w[PER][2][8];
-        constexpr bool AHEAD = VEC || PER == 1 || !RES;       // (the pieces of 32 columns and a residual's would not stay in registers: 2048 x 9290 bf16 and f32 114 us so, 81 without; of 16 columns they do: 8192 x 4099 bf16 112, 124 without)
+        constexpr bool AHEAD = VEC || PER == 1 || !RES;       // (the pieces of 32 columns and a residual's would not stay in registers: 2048 x 9290 bf16 and f32 114 us so, 84 without; of 16 columns they do: 8192 x 4099 bf16 114, 124 without)
         Piece p[PER];
         if (AHEAD) {
 #pragma unroll
@@ -493,7 +493,7 @@ static int f8_norm_p(cudaStream_t st, const F8NormArgs& a, int block, bool pdl) 
 }
 template <typename T, typename R, bool VEC>
 static int f8_norm_v(cudaStream_t st, F8NormArgs& a, bool pdl) {
-    // whole warps for a row, as few as have its columns (power of two: 8192 x 4099 bf16 and a residual 133 us, so 112); a block of about 256 threads
+    // whole warps for a row, as few as have its columns (power of two: 8192 x 4099 bf16 and a residual 133 us, so 114); a block of about 256 threads
     a.tpr = std::min(512, (a.K + F8_BLOCK - 1) / F8_BLOCK * 8 + 31 & ~31);
     const int block = a.tpr * std::max(1, 256 / a.tpr);
     if (a.K <= a.tpr * 16) return f8_norm_p<T, R, VEC, 1>(st, a, block, pdl);
