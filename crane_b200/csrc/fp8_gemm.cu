@@ -8,6 +8,7 @@
 // along K and adds its partial tiles through distributed shared memory.
 // f8_pair_kernel, more rows: tiles of 256 x 256 over pairs of CTAs, a kernel for each way the results leave.
 #include "fp8.cuh"
+#include "fp8_tiles.h"
 #include "tc.cuh"
 
 #include <cooperative_groups.h>
@@ -419,22 +420,11 @@ struct F8PairArgs {
     bool tma, w_static;
     int* err;
 };
-constexpr int F8_BAND = 8;                         // rows of tiles that are walked together: neighbours in time share weights and activations in L2
 struct F8PairCfg {
     static constexpr int A_BYTES = 128 * 128, STAGE = A_BYTES + 128 * 128, PATCH = F8_EPI * 8192;
     static constexpr int STAGES = (226 * 1024 - PATCH - 1024) / STAGE;
     static constexpr int SMEM = STAGES * STAGE + PATCH + 1024;
 };
-struct F8Item { int mt, n0, width; };
-__device__ __forceinline__ F8Item f8_item(const F8PairArgs& a, int i) {
-    int t = i, sub = 0, width = 256;
-    if (i >= a.whole) {
-        const int j = i - a.whole;
-        t = a.whole + j / a.cut; sub = j % a.cut; width = 256 / a.cut;
-    }
-    const int per = F8_BAND * a.tiles_n, b = t / per, r = t - b * per, w = min(F8_BAND, a.tiles_m - b * F8_BAND), nt = r / w;
-    return F8Item{b * F8_BAND + r - nt * w, nt * 256 + sub * width, width};
-}
 // 32 rows x up to C columns of a warp (those below N), a row a lane, through a patch of 32 x 32 f32 (16-byte pieces swizzled by the row), so that stores (and the addend's loads) cover
 // pieces of rows.  The addition is f32.  Addends are read ahead of all stores: result and addend may be the same memory, so the compiler keeps a load behind every store that is written
 // before it (8192 x 24576 x 64 f32 669 us so, 345 ahead).
@@ -520,12 +510,12 @@ __device__ __forceinline__ void f8_store_odd(const F8Epi& e, int M, int N, int m
 // The same rows by TMA, two pieces of 128 bytes a row under way: the tiles of all SMs end together, and what they store then (64 KB each) takes the chip longer than the two blocks
 // of K that the MMAs run ahead.
 template <typename T, int C>
-__device__ __forceinline__ void f8_store_tma(const CUtensorMap* map, int M, int N, int m0, int n0, const float* v, uint8_t* patch, int lane) {
+__device__ __forceinline__ void f8_store_tma(const CUtensorMap* map, int M, int N, int m0, int n0, const float* v, uint8_t* patch, uint32_t& phases, int lane) {
     constexpr int PER = 16 / (int)sizeof(T), W = 8 * PER;
 #pragma unroll
     for (int c = 0; c < C; c += W) {
         if (n0 + c >= N || m0 >= M) break;
-        uint8_t* to = patch + (c / W & 1) * 4096;
+        uint8_t* to = patch + f8_half(phases) * 4096;
         if (lane == 0) tma_store_wait_read<1>();
         __syncwarp();
 #pragma unroll
@@ -538,6 +528,7 @@ __device__ __forceinline__ void f8_store_tma(const CUtensorMap* map, int M, int 
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) { tma_store_2d(map, to, n0 + c, m0); tma_store_commit(); }
+        f8_half_stored(phases);
     }
 }
 
@@ -593,7 +584,7 @@ __device__ __forceinline__ void f8_pair_tile(const F8PairArgs& a, const CUtensor
         if (++ring.b == BUFS) ring.b = 0;
     }
     if constexpr (WAY == F8_PLAIN && C * sizeof(T) >= 128) {
-        if (a.tma) { f8_store_tma<T, C>(tmO, a.M, N, m0, n0, v, patch, lane); return; }
+        if (a.tma) { f8_store_tma<T, C>(tmO, a.M, N, m0, n0, v, patch, ring.phases, lane); return; }
     }
     if (lane == 0) tma_store_wait_read<0>();          // (the whole tiles' stores have left the patch)
     __syncwarp();
@@ -728,15 +719,6 @@ f8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     if (warp == 1) { tc_fence_after(); tmem_dealloc_pair(tmem, 512); }
 }
 
-struct F8Turns { int whole, items, cut; };
-static F8Turns f8_turns(int M, int N, int pairs) {       // tiles of a pair, those of the last turn cut into strips where pairs are free for them
-    const int tiles = ((M + 255) / 256) * ((N + 255) / 256), left = tiles % pairs;
-    F8Turns t;
-    t.cut = left == 0 || 2 * left > pairs ? 1 : 4 * left > pairs ? 2 : 4;
-    t.whole = tiles - (t.cut > 1 ? left : 0);
-    t.items = t.whole + (tiles - t.whole) * t.cut;
-    return t;
-}
 template <typename T, int WAY>
 static int f8_pair_t(cudaStream_t st, const F8Linear& p, int M, int N, int K, bool pdl) {
     using Cfg = F8PairCfg;
