@@ -21,6 +21,7 @@
 #include "decode.cuh"
 #include "decode_ll.cuh"
 #include "fp8.cuh"
+#include "fp8_waits.h"
 #include "host_pool.h"
 #include "gdn.cuh"
 #include "gemm.cuh"

@@ -35,6 +35,7 @@ struct F8Linear {
     void* out; int type; long long ldo;
     const void* add; long long ldadd;
     bool w_static;             // no kernel that may still run writes the weights: their first tiles are fetched ahead of the dependency wait
+    int* err = nullptr;        // word of bounded waits that run out (TcWait); nullptr: the stream's, which calls that read results from that stream look at
 };
 int f8_linear_launch(cudaStream_t st, const F8Linear& a, int M, int N, int K, bool pdl);
 

@@ -374,7 +374,8 @@ static int f8_rows_gemm_t(cudaStream_t st, const F8Linear& p, int M, int N, int 
     a.ep = F8Epi{p.out, p.add, p.ldo, p.ldadd, p.type};
     a.xs = p.x.scales; a.lds = p.x.lds; a.ws = p.ws; a.ldws = p.ldws;
     a.M = M; a.N = N; a.KB = f8_blocks(K); a.w_static = p.w_static; a.vec = f8_vec_out(p);
-    if (const int e = f8_err_word(st, &a.err)) return e;
+    a.err = p.err;
+    if (!a.err) if (const int e = f8_err_word(st, &a.err)) return e;
     CUtensorMap tmW, tmX;
     if (!tc_tmap_encode(&tmW, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmX, p.x.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K, (uint64_t)p.x.ld, Cfg::NT, 128, CU_TENSOR_MAP_SWIZZLE_128B)) return -1001;
@@ -731,7 +732,8 @@ static int f8_pair_t(cudaStream_t st, const F8Linear& p, int M, int N, int K, bo
     const F8Turns turns = f8_turns(M, N, pairs);
     a.whole = turns.whole; a.items = turns.items; a.cut = turns.cut;
     a.pairs = std::min(a.items, pairs);
-    if (const int err = f8_err_word(st, &a.err)) return err;
+    a.err = p.err;
+    if (!a.err) if (const int err = f8_err_word(st, &a.err)) return err;
     CUtensorMap tmX, tmW, tmW32, tmO;
     if (!tc_tmap_encode(&tmX, p.x.codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)M, (uint64_t)K, (uint64_t)p.x.ld, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
         !tc_tmap_encode(&tmW, p.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, (uint64_t)N, (uint64_t)K, (uint64_t)p.ldw, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||

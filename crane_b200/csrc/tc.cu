@@ -82,9 +82,8 @@ __global__ void expire_wait_kernel(int* err) {
     wait(&bar, 0);
     wait(&bar, 0);                  // (given up: returns at once)
 }
-int tc_expire_wait(cudaStream_t st) {
-    int* err = nullptr;
-    if (const int e = tc_err_word(st, &err)) return e;
+int tc_expire_wait(cudaStream_t st, int* err) {
+    if (!err) if (const int e = tc_err_word(st, &err)) return e;
     expire_wait_kernel<<<1, 1, 0, st>>>(err);
     return (int)cudaGetLastError();
 }

@@ -259,7 +259,7 @@ inline bool tc_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint
     return tc_tmap_16(map, base, rows, cols, ld, box_rows, 64, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 // launches a kernel whose wait runs out after about a millisecond (for tests of what follows)
-int tc_expire_wait(cudaStream_t st);
+int tc_expire_wait(cudaStream_t st, int* err = nullptr);      // err: nullptr: the stream's word
 int tc_expire_wait_pair(cudaStream_t st);      // ... one CTA's of a pair, while the other waits for what never comes
 int tc_device_sms();
 // clusters of `cl` (2 .. 8) CTAs that the device runs at the same time when a CTA takes a whole SM

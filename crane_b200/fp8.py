@@ -8,7 +8,7 @@ A model of an fp8 checkpoint (`quantization_config` {"quant_method": "fp8", "wei
     codes, scales = fp8.silu_mul(gate_up)
     stream = fp8.linear(codes, scales, w_down, w_down_scales, add=stream, out=stream)
 
-Calls run on the tensors' device and its current stream, wait for nothing, keep nothing and may be captured into graphs.  Given `out` they allocate nothing.
+Calls run on the tensors' device and its current stream, wait for nothing, keep nothing and may be captured into graphs (`status` waits, and tells of a linear that gave up a wait).  Given `out` they allocate nothing.
 As everywhere in this package there is no CPU path.
 """
 from __future__ import annotations
@@ -204,7 +204,8 @@ def linear(x, x_scales, weight, weight_scales, *, add=None, out=None, dtype=torc
 
 
 def status(device=None):
-    """Waits for the current stream of `device`; raises when its work failed, or when a linear gave up a wait on the GPU."""
+    """Waits for the current stream of `device`; raises when its work failed, or when a linear on the device, captured or not, gave up a wait on the GPU since
+    the last call for that stream (whichever stream it ran on: each is told once)."""
     index = None if device is None else torch.device(device).index
     dev = torch.cuda.current_device() if index is None else index
     rc = _entry("status")(dev, _raw_stream(dev))

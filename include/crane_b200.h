@@ -326,7 +326,8 @@ CRANE_B200_API int crane_b200_decode_path(const crane_b200_model* m);
  * their tensors on the device themselves: activation rows become e4m3 codes with an f32 scale for every 128 columns, weights are codes with a scale for every 128 x 128.
  *   block of a row:  a = max(max |y|, 2^-100), scale = a / 448, code = e4m3(y * (448 / a)), to nearest even (a NaN's code is NaN; an infinity makes its block NaN in use)
  * Every pointer is memory of `device`, `stream` a cudaStream_t of that device (NULL: its default stream); a call enqueues its work there, with no wait and no
- * copy to the host, and may be captured into a graph.  Inputs and results have to stay while that work runs.  Nothing is kept between calls: several threads may make them at once.
+ * copy to the host, and may be captured into a graph.  Inputs and results have to stay while that work runs.  Nothing is kept between calls
+ * but a device's word of waits that ran out (crane_b200_fp8_status): several threads may make them at once.
  * dtype: crane_b200_dtype; a row distance (ld..) counts elements.  Codes: rows start on 16-byte boundaries (base and ld multiples of 16, ld >= columns), any number of
  * columns.  Scales of rows: block by block, that of row i and block b at scales[b * lds + i], lds >= rows.  m = 0 (or n = 0) does nothing; m, n and k go to 2^30.
  * Bytes behind a row's last column and rows behind the last are left as they are.
@@ -347,8 +348,8 @@ CRANE_B200_API int crane_b200_fp8_rms_norm(int device, const void* x, int dtype,
  * w [n, k] codes, w_scales [ceil(n / 128), ceil(k / 128)].  Sums in f32, rounded once to out's type; `add` (NULL: nothing) has that type and may be `out`. */
 CRANE_B200_API int crane_b200_fp8_linear(int device, const uint8_t* x, size_t ldx, const float* x_scales, size_t lds, const uint8_t* w, size_t ldw, const float* w_scales,
                                          size_t ldws, size_t m, size_t n, size_t k, const void* add, size_t ldadd, void* out, int dtype, size_t ldo, void* stream);
-/* Waits for `stream`; CRANE_B200_CUDA_ERROR when its work failed, or when a linear's bounded wait ran out on the GPU since the last such call (its results are
- * worth nothing then). */
+/* Waits for `stream`; CRANE_B200_CUDA_ERROR when its work failed, or when a linear's bounded wait ran out on `device` (its results are worth nothing then) since the last such call
+ * for this stream, or ever if there was none: in whichever stream's work, captured linears of graphs launched on any stream among it.  Every stream is told once. */
 CRANE_B200_API int crane_b200_fp8_status(int device, void* stream);
 
 /* ---- kernel-level test hooks (used by tests/ only; host buffers in, host buffers out) ------------ */
