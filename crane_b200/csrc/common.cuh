@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <cstdio>
 
+#include "smem_optin.h"
+
 namespace cb {
 
 typedef __nv_bfloat16 bf16;
@@ -130,22 +132,6 @@ __device__ __forceinline__ float glu_pair_f(float g, float u, float limit) {
 }
 __device__ __forceinline__ float gelu_erf_f(float x) { return 0.5f * x * (1.f + erff(x * 0.70710678118654752440f)); }
 
-
-// Host: cudaFuncSetAttribute(MaxDynamicSharedMemorySize) is per DEVICE -- one process may drive a handle on every GPU of the box --
-// so each launcher remembers, per device, the largest opt-in it has already made for its kernel instantiation.
-constexpr int CB_MAX_DEV = 64;
-struct SmemOptIn { size_t bytes[CB_MAX_DEV] = {}; };
-template <typename K>
-inline int ensure_dyn_smem(K kernel, size_t bytes, SmemOptIn& seen) {
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= CB_MAX_DEV) return (int)cudaErrorInvalidDevice;
-    if (bytes > seen.bytes[dev]) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-        if (e != cudaSuccess) return (int)e;
-        seen.bytes[dev] = bytes;
-    }
-    return 0;
-}
 
 // Host: launch `kernel` on `st`, as a programmatic dependent of the previous kernel in the stream when `pdl`.
 inline bool& prefill_pdl() { static bool on = true; return on; }

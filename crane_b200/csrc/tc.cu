@@ -1,6 +1,7 @@
 // Host side of the tensor-core kernels.  See tc.cuh.
 #include "tc.cuh"
 
+#include <atomic>
 #include <mutex>
 #include <unordered_map>
 
@@ -65,11 +66,15 @@ bool tc_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType type, uint6
 }
 
 int tc_device_sms() {
-    static int sms[CB_MAX_DEV] = {};
+    static std::atomic<int> sms[CB_MAX_DEV];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= CB_MAX_DEV) return 148;
-    if (!sms[dev]) { int v = 0; cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev); sms[dev] = v > 0 ? v : 148; }
-    return sms[dev];
+    int n = sms[dev].load(std::memory_order_relaxed);
+    if (!n) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) { cudaGetLastError(); n = 148; }
+        sms[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
 }
 
 __global__ void expire_wait_kernel(int* err) {
