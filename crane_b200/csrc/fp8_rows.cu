@@ -230,20 +230,19 @@ __device__ __forceinline__ void f8_emit(const float (*v)[8], long long m, int c,
     }
 }
 
-// SiLU(g) u = g / (1 + z) u, z = exp(-g): 2^t with t = -g log2 e and what its rounding lost (lo) made good to first order, the quotient by rcp.approx and one step of Newton's.
-// The exponent's g is held to +-88: above, z vanishes against 1; below, 1 + z passes 2^126, the reciprocal is zero, and so is the result (|true| < 6e-37 u).
-// Thirteen instructions and errors of an ulp or two, as expf and a division have in thirty, whose form took 166 us where the bytes (8192 x 2 x 12288 bf16) take 78 (these: 97); 104 with
-// expf(-|g|), which needs no bounds.
+// SiLU(g) u = g / (1 + z) u, z = exp(-g).  z / 4 = 2^(t - 2), t = -g log2 e, what t's rounding lost (lo) made good to first order; 4 / (1 + z) by rcp.approx, which an infinite gate stays
+// infinite through.  By quarters, because 1 / (1 + z) would leave the normal numbers, where the reciprocal gives zero, ahead of g / (1 + z); where z itself passes 2^128 (g < -88.72) it
+// does, and the result is zero.  The exponent's g is held to -90 .. 88: above, z vanishes against 1.
+// Fourteen instructions and errors to five ulp (measured over -88.7 .. 88; four with a step of Newton's on the reciprocal), as expf and a division have two in thirty.  8192 x 2 x 12288 bf16, whose
+// bytes take 78 us: 96; with the step 102, with expf and a division 166.
 __device__ __forceinline__ float f8_silu_mul(float g, float u) {
     const float c = 1.44269502162933349609375f;                            // log2 e to f32
-    const float h = fminf(fmaxf(g, -88.f), 88.f), t = h * -c, lo = fmaf(h, -c, -t);
+    const float h = fminf(fmaxf(g, -90.f), 88.f), t = h * -c, lo = fmaf(h, -c, -t);
     float z, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(t));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(z) : "f"(t - 2.f));
     z = fmaf(z, fmaf(h, -1.3349758e-8f, lo * 0.69314718f), z);             // (log2 e - c) ln 2 = 1.3349758e-8
-    const float d = 1.f + z;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-    const float q = g * r;
-    return fmaf(fmaf(-q, d, g), r, q) * u;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(0.25f + z));
+    return g * (r * 0.25f) * u;
 }
 
 // A warp takes 512 columns of a row (four blocks) at a time and asks for U such pieces before it works on the first.

@@ -1,6 +1,7 @@
-"""Linears in 8-bit floating point where they were wrong once: stores of ragged tiles that follow one another, waits that run out in a replayed graph.
-References and tolerances are test_fp8.py's."""
+"""Linears in 8-bit floating point where they were wrong once: stores of ragged tiles that follow one another, waits that run out in a replayed graph,
+infinite gates and far negative ones.  References and tolerances are test_fp8.py's where nothing else is said."""
 import ctypes as C
+import math
 import os
 import subprocess
 
@@ -85,3 +86,48 @@ def test_a_wait_that_ran_out_in_a_replayed_graph_is_reported():
             assert told(s) == (s != on)
             assert not told(s)
     assert torch.equal(out, fp8.linear(x, xs, w, ws))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [128, 300])
+@pytest.mark.parametrize("dt", TYPES)
+def test_infinite_and_nan_gates(dt, k):
+    """An infinite SiLU(g) u makes its block's scale infinite and the block NaN in use; a NaN (that of g = -inf, -inf / inf, and of inf x 0 among them) is its own."""
+    from crane_b200 import fp8
+    inf, nan = math.inf, math.nan
+    gate, up = torch.ones((8, k), device="cuda"), torch.ones((8, k), device="cuda")
+    gate[0, 3], gate[1, 3], gate[2, 3], gate[3, 3] = inf, -inf, nan, inf
+    up[3, 3] = 0
+    up[4, 3], up[5, 3] = inf, nan
+    gate[6, 3], up[6, 3] = inf, -2
+    y = gate.double() / (1 + torch.exp(-gate.double())) * up.double()
+    codes, scales = fp8.silu_mul(torch.cat([gate, up], 1).to(TYPES[dt]))
+    back = codes.double() * scales.double().repeat_interleave(128, 1)[:, :k]
+    others = [i for i in range(k) if i != 3]
+    for r in range(8):
+        if torch.isinf(y[r, 3]):
+            assert r in (0, 4, 6) and torch.isinf(scales[r, 0]) and torch.isnan(back[r, :128]).all() and torch.isfinite(back[r, 128:]).all()
+        else:
+            assert torch.isnan(back[r, 3]) == torch.isnan(y[r, 3]) == (r in (1, 2, 3, 5))
+            assert (codes[r, others].float() == 448).all() and torch.isfinite(scales[r]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lo, hi", [(-8, 8), (8, 89), (-80, -8), (-87.3, -80), (-88.7, -87.3), (-1000, -88.8)])
+def test_gated_units_to_their_last_bits(lo, hi):
+    """One value a block, so that the block's scale is that value / 448 in f32.  In units of 2^-24: the exponential 4 (2^-22 of itself), its argument 1.4 where it is small (ln 2 x 2^-23),
+    its correction 1, 1 + z 1, the reciprocal 2 (an ulp), its quarter 4 where that is no normal number (half of 2^-149 of 2^-128), two products 2, the scale's quotient 1: 16.4; 18 are allowed.
+    Below -88.73 the exponential is infinite in f32 and the unit zero."""
+    from crane_b200 import fp8
+    gen = gen_of("units", lo, hi)
+    n = 1 << 18
+    g = torch.rand(n, generator=gen, device="cuda") * (hi - lo) + lo
+    u = torch.exp2(3 * torch.rand(n, generator=gen, device="cuda")) * 2.0 ** (100 if lo < -80 else 60 if lo < -8 else 0)
+    x = torch.zeros((n, 256), device="cuda")
+    x[:, 0], x[:, 128] = g, u
+    scales = fp8.silu_mul(x)[1][:, 0].double()
+    y = (g.double() / (1 + torch.exp(-g.double())) * u.double()).abs()
+    if hi < -88.73:
+        y.zero_()
+    want = y.clamp_min(2.0 ** -100) / 448
+    assert ((scales - want).abs() <= 18 * 2.0 ** -24 * want).all(), float(((scales - want) / want).abs().max()) * 2 ** 24
