@@ -245,6 +245,10 @@ __device__ __forceinline__ float f8_silu_mul(float g, float u) {
     return g * (r * 0.25f) * u;
 }
 
+// values of an input row (its 2 K pass an int's range where K is the largest that is taken)
+__host__ __device__ constexpr long long f8_row_values(bool gated, int K) { return (gated ? 2LL : 1LL) * K; }
+static_assert(f8_row_values(true, 1 << 30) == 1LL << 31, "counted in 64 bits");
+
 // A warp takes 512 columns of a row (four blocks) at a time and asks for U such pieces before it works on the first.
 template <typename T, bool GATED, bool VEC, int U>
 __global__ void __launch_bounds__(256)
@@ -254,7 +258,7 @@ f8_rows_kernel(const T* x, long long ldx, long long M, int K, F8Out o) {
     const int dm = (int)(warps / per), dc = (int)(warps % per);             // a step of all warps: rows and pieces
     long long m = w / per;
     int piece = (int)(w % per);
-    const T* x_end = x + (M - 1) * ldx + (GATED ? 2 : 1) * K;
+    const T* x_end = x + (M - 1) * ldx + f8_row_values(GATED, K);
     pdl_wait();
     pdl_launch_dependents();
     while (m < M) {

@@ -131,3 +131,18 @@ def test_gated_units_to_their_last_bits(lo, hi):
         y.zero_()
     want = y.clamp_min(2.0 ** -100) / 448
     assert ((scales - want).abs() <= 18 * 2.0 ** -24 * want).all(), float(((scales - want) / want).abs().max()) * 2 ** 24
+
+
+@pytest.mark.gpu
+def test_rows_of_the_largest_width():
+    """2^30 columns of gates and as many ups on an odd boundary: the bits of the same row on a 16-byte boundary."""
+    from crane_b200 import fp8
+    k = 2 ** 30
+    wide = torch.empty(2 * k + 8, dtype=torch.bfloat16, device="cuda")
+    part = rows_of(gen_of("widest"), 1, 2 ** 20, torch.bfloat16)[0]
+    for i in range(0, 2 * k, 2 ** 20):
+        wide[i:i + 2 ** 20] = part.roll(i >> 20)
+    even = fp8.silu_mul(wide[None, :2 * k])
+    wide[1:2 * k + 1] = wide[:2 * k].clone()
+    odd = fp8.silu_mul(wide[None, 1:2 * k + 1])
+    assert torch.equal(even[0].view(torch.uint8), odd[0].view(torch.uint8)) and torch.equal(even[1], odd[1])
