@@ -37,8 +37,8 @@ __device__ __forceinline__ float f8_fetch(const float* p) {
     return v;
 }
 
-// An accumulator has been read (tcgen05.wait::ld, fence::before_thread_sync): no memory of this thread's is handed over with it, so the arrival is a relaxed one.  As a
-// release at cluster scope it waited, once a block of K, for everything the thread had in flight.
+// An accumulator has been read: behind tcgen05.wait::ld its values are in registers, so all that the arrival orders is the next MMAs' writes behind these reads, which have happened.  Nothing
+// that this thread wrote is handed over with it, so it may be a relaxed one; as a release at cluster scope it waited, once a block of K, for everything the thread had in flight.
 __device__ __forceinline__ void f8_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
 struct F8Epi { void* out; const void* add; long long ldo, ldadd; int type; };
@@ -407,10 +407,10 @@ static int f8_rows_gemm_t(cudaStream_t st, const F8Linear& p, int M, int N, int 
 // an epilogue thread has one activation row and half of the columns, so that its scale is one product a block of K.
 // A persistent pair an SM pair takes tiles in turn; MMAs run up to two blocks of K ahead of the epilogue, into the next tile too.  Tiles left over for the last turn, or
 // for the only one, are cut into 2 or 4 strips of columns when that many pairs are free.
-// What bounds it (8192 x 24576 x 4096, 2 310 TFLOP/s; the MMAs and stores alone 2 700 at 1.3 GHz under the power limit): the two accumulators.  A block's MMAs take 512 cycles, its
-// epilogue 440 (TMEM reads and 256 FMA issues a scheduler, next to MMAs that read and write the same TMEM), the hand-overs between them (commit, wait, arrival at
-// the even CTA) some 600 more, so that a block passes every 800.  Measured and left: two MMAs of 128 columns, for four accumulators (1 850 TFLOP/s, an MMA takes 125 cycles all the same),
-// sixteen epilogue warps, 32 columns a read, two producers, two issuing warps (no gain).
+// What bounds it (8192 x 24576 x 4096: 705 - 730 us in some calls, 2 340 TFLOP/s; 843 in seconds of them, 1 960, at the 1.2 - 1.28 GHz that the power limit leaves; the MMAs and stores alone
+// 2 700 at 1.3 GHz): the two accumulators.  A block's MMAs take 512 cycles, its epilogue 440 (TMEM reads and 256 FMA issues a scheduler, next to MMAs that read and write the same TMEM), the
+// hand-overs between them (commit, wait, arrival at the even CTA) some 600 more, so that a block passes every 800.  Measured and left: two MMAs of 128 columns, for four accumulators
+// (1 850 TFLOP/s; by themselves MMAs of 256, 128 and 64 columns take 128, 64 and 43 cycles), sixteen epilogue warps, 32 columns a read, two producers, two issuing warps (no gain).
 // =====================================================================================
 struct F8PairArgs {
     F8Epi ep;
@@ -766,9 +766,8 @@ static int f8_pair_launch(cudaStream_t st, const F8Linear& p, int M, int N, int 
 //   700 x 2048 x 6144 - / 22.0 / 28.2 / 29.3   1024 x 4096 x 4096 - / - / 40.7 / 22.2
 //   4096 x 12288 x 128 168 / 134 / 124 / 21.9   4096 x 12288 x 512 200 / 168 / 157 / 40   1500 x 13624 x 116 73 / 59 / 55 / 13.8   82 x 22704 x 1058 22.7 / 18.4 / 21.0 / 15.3
 //   2935 x 560 x 1340 14.5 / 17.4 / 11.7 / 10.7   5512 x 480 x 8249 64 / 55 / 72 / 39   291 x 8344 x 801 19.1 / 16.5 / 17.8 / 9.5   66 x 3616 x 378 5.0 / 5.6 / 6.3 / 6.4
-// Each turn of CTAs takes t0 us, its launch and its stores, and c us a block of K.  Pairs stay: a turn is their blocks of K, 0.45 us each whatever the width of a strip (an MMA of 256 rows
-// takes some 125 cycles with 64 to 256 columns, so that strips shorten the last turn by their stores and their scales only: 1111 x 4096 x 2048 20.5 / 18.7, 256 x 24576 x 4096 38.4 / 37.1,
-// none 400 x 4096 x 4096 19.7 / 20.4), and the part of the stores that the next tile's MMAs do not cover.  Over 48 sizes drawn between 65 x 64 x 64 and 8192 x 24576 x 12288 the choice takes
+// Each turn of CTAs takes t0 us, its launch and its stores, and c us a block of K.  Pairs stay: a turn is their blocks of K, 0.45 us each whatever the width of a strip (strips
+// shorten the last turn by little: 1111 x 4096 x 2048 20.5 / 18.7, 256 x 24576 x 4096 38.4 / 37.1, none 400 x 4096 x 4096 19.7 / 20.4), and the part of the stores that the next tile's MMAs do not cover.  Over 48 sizes drawn between 65 x 64 x 64 and 8192 x 24576 x 12288 the choice takes
 // 0.1 % longer than the best of the four.
 template <int CW>
 static double f8_rows_us(int M, int N, int KB, double t0, double c) {
