@@ -273,7 +273,7 @@ struct crane_b200_model {
     bool fp8 = false, any_f8 = false;
     F8Rooms f8_dec, f8_pre;
     bool load_f8(LayerW& l, const std::string& n, const std::string& t, int dt, const int64_t* shape, int ndim, const void* data);
-    F8Rooms f8_rooms(int rows);
+    void f8_rooms(F8Rooms& r, int rows);
     void f8_linear(const F8Rooms& r, const unsigned char* w, const float* ws, int N, int K, const float* add, float* y, int rows);
     void f8_qkv(const LayerW& l, const F8Rooms& r, const float* xin, float* y, int rows);            // y = W_qkv norm(x)
     void f8_o(const LayerW& l, const F8Rooms& r, const float* a, float* xio, int rows);              // x += W_o a
@@ -433,6 +433,7 @@ struct crane_b200_model {
         if (it != allocs.end()) allocs.erase(it);
         cudaFree(p);
     }
+    template <typename... P> void dfree_all(P*&... p) { ((dfree(p), p = nullptr), ...); }
     int q_stride() const { return hybrid ? 2 * D : D; }     // Qwen3.5 q_proj emits per-head [query | gate]
     int qkv_dim() const { return nh * q_stride() + 2 * nkv * D; }
     int conv_dim() const { return 2 * nk * dk + nv * dv; }
@@ -1162,14 +1163,12 @@ bool crane_b200_model::load_f8(LayerW& l, const std::string& n, const std::strin
     fail(CRANE_B200_UNSUPPORTED, "tensor %s: e4m3 codes and their scales are the seven projections' of a layer", n.c_str());
 }
 
-crane_b200_model::F8Rooms crane_b200_model::f8_rooms(int rows) {
+void crane_b200_model::f8_rooms(F8Rooms& r, int rows) {
     const int kmax = std::max(std::max(H, I), q_dim());
-    F8Rooms r;
     r.codes = dalloc<unsigned char>((size_t)rows * kmax);
     r.scales = dalloc<float>((size_t)(kmax / F8_BLOCK) * rows);
     r.gu = dalloc<float>((size_t)rows * 2 * I);
     r.rows = rows;
-    return r;
 }
 
 void crane_b200_model::f8_linear(const F8Rooms& r, const unsigned char* w, const float* ws, int N, int K, const float* add, float* y, int rows) {
@@ -1327,7 +1326,7 @@ void crane_b200_model::finalize() {
         TcScratch sc;                               // (taken here, not by the first decode step)
         LAUNCH_OK(tc_scratch_get(stream, (std::max(std::max(V, 2 * I), qkv_dim()) + 127) / 128, &sc));
     }
-    if (any_f8) f8_dec = f8_rooms(B);
+    if (any_f8) f8_rooms(f8_dec, B);
     x_dec = dalloc<float>((size_t)B * H);
     qkv_dec = dalloc<float>((size_t)B * qkv_dim());
     attn_dec = dalloc<float>((size_t)B * q_dim());
@@ -1378,10 +1377,9 @@ void crane_b200_model::finalize() {
 void crane_b200_model::ensure_prefill_ws(int S) {
     if (S <= ws_S) return;
     CUDA_OK(cudaStreamSynchronize(stream));
-    for (void* p : {(void*)x, (void*)qkv, (void*)xn, (void*)q_bf, (void*)attn_bf, (void*)act_bf, (void*)ids_dev, (void*)pos3_dev,
-                    (void*)rows_dev, (void*)embeds_in, (void*)rows_f32, (void*)xqr_buf, (void*)g_proj, (void*)g_conv, (void*)g_qn, (void*)g_kn, (void*)g_gb, (void*)g_y, (void*)g_gl, (void*)g_chunk,
-                    (void*)f8_pre.codes, (void*)f8_pre.scales, (void*)f8_pre.gu})
-        dfree(p);
+    ws_S = 0;                                  // (until all of it is there again: a growth that finds no memory leaves nothing that a later call would take for its own)
+    dfree_all(x, qkv, xn, q_bf, attn_bf, act_bf, ids_dev, pos3_dev, rows_dev, embeds_in, rows_f32, xqr_buf, g_proj, g_conv, g_qn, g_kn, g_gb, g_y, g_gl, g_chunk,
+              f8_pre.codes, f8_pre.scales, f8_pre.gu);
     const int cap = (S + 127) / 128 * 128;
     x = dalloc<float>((size_t)cap * H);
     qkv = dalloc<float>((size_t)cap * qkv_dim());
@@ -1407,7 +1405,7 @@ void crane_b200_model::ensure_prefill_ws(int S) {
     pos3_dev = dalloc<int>((size_t)3 * cap);
     rows_dev = dalloc<int>(cap);
     embeds_in = dalloc<float>((size_t)cap * H);
-    if (any_f8) f8_pre = f8_rooms(cap);
+    if (any_f8) f8_rooms(f8_pre, cap);
     rows_f32 = any_quant || any_f8 ? dalloc<float>((size_t)cap * std::max(I, q_dim())) : nullptr;
     xqr_buf = any_quant ? dalloc<unsigned char>(qrows_bytes(cap, std::max(std::max(H, I), q_dim()))) : nullptr;
     xqr_rows = cap;
@@ -1901,10 +1899,8 @@ void crane_b200_model::prefill(const uint32_t* ids, const float* embeds, size_t 
 void crane_b200_model::ensure_vision_ws(int N) {
     if (N <= vws_N) return;
     CUDA_OK(cudaStreamSynchronize(stream));
-    for (void* p : {(void*)v_x, (void*)v_qkv, (void*)v_pv, (void*)v_cos, (void*)v_sin, (void*)v_w4, (void*)v_pvb, (void*)v_xn, (void*)v_qkvb,
-                    (void*)v_attn, (void*)v_act, (void*)v_m1, (void*)v_idx4, (void*)v_seq_start, (void*)v_seq_len, (void*)img_embeds,
-                    (void*)ds_embeds})
-        dfree(p);
+    vws_N = 0;
+    dfree_all(v_x, v_qkv, v_pv, v_cos, v_sin, v_w4, v_pvb, v_xn, v_qkvb, v_attn, v_act, v_m1, v_idx4, v_seq_start, v_seq_len, img_embeds, ds_embeds);
     v_tab_key.clear();
     const int cap = (N + 127) / 128 * 128;
     const int pk = v_in * v_tpatch * v_patch * v_patch, mh = v_H * v_merge * v_merge, m2 = v_merge * v_merge;
