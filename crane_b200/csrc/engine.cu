@@ -22,6 +22,9 @@
 #include "decode_ll.cuh"
 #include "fp8.cuh"
 #include "fp8_waits.h"
+#include "kv8.cuh"
+#include "lora.cuh"
+#include "draft.cuh"
 #include "host_pool.h"
 #include "gdn.cuh"
 #include "gemm.cuh"
@@ -3203,5 +3206,6 @@ int crane_b200_op_gemm(int device, const uint16_t* a, const uint16_t* a_lo, cons
 
 #include "engine_tts.inc"
 #include "engine_fp8.inc"
+#include "engine_device.inc"
 #include "engine_comm.inc"
 #include "engine_loaders.inc"

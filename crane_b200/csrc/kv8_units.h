@@ -1,0 +1,105 @@
+// How the work over an 8-bit paged cache (kv8.cuh) is found in what device memory says, and dealt out.  Host and device code: tests run it on the CPU.
+#pragma once
+
+#ifdef __CUDACC__
+#define CB_HD __host__ __device__ __forceinline__
+#else
+#define CB_HD inline
+#endif
+
+namespace cb {
+
+struct Kv8Pool { unsigned char* k; unsigned char* v; float* scales; int pages, kv_heads, page, dim; };
+// Sequence b holds lens[b] positions, position i on page table[b * ldt + i / page]; its new rows are rows starts[b] .. starts[b + 1] - 1, at its last positions.
+// Everything here is device memory that the host does not look at: kernels clamp starts to the rows there are and leave out pages and positions that do not exist.
+struct Kv8Seqs { const int* table; long long ldt; int width; const int* lens; const int* starts; int seqs, rows; };
+
+template <typename T> CB_HD T least(T a, T b) { return b < a ? b : a; }
+template <typename T> CB_HD T most(T a, T b) { return a < b ? b : a; }
+
+// What a sequence brings
+struct Kv8Seq { int s0, n, len, first; };                           // first: position of row s0 (negative: rows ahead of position 0 are not in the cache)
+CB_HD int kv8_start(const Kv8Seqs& s, int b) { return least(most(s.starts[b], 0), s.rows); }
+CB_HD Kv8Seq kv8_seq(const Kv8Seqs& s, int b) {
+    Kv8Seq q;
+    q.s0 = kv8_start(s, b);
+    q.n = most(kv8_start(s, b + 1), q.s0) - q.s0;
+    q.len = least(most(s.lens[b], 0), 1 << 30);
+    q.first = q.len - q.n;
+    return q;
+}
+CB_HD int kv8_page(const Kv8Seqs& s, const Kv8Pool& p, int b, int block) {      // -1: none
+    if (block < 0 || block >= s.width) return -1;
+    const int page = s.table[b * s.ldt + block];
+    return (unsigned)page < (unsigned)p.pages ? page : -1;
+}
+
+// ---- rows into pages: the pieces of a sequence's new rows that lie on one page each ------------------------------------------------
+// Piece number `at` is either a row, the first of its page's (by_row), or a number that sequence b has kv8_piece_key(b) and on: n rows touch at most n / page + 2 pages.
+CB_HD int kv8_piece_key(const Kv8Seqs& s, int page, int b, bool by_row) { const int r = kv8_start(s, b); return by_row ? r : r / page + 2 * b; }
+struct Kv8Piece { int block, pos, count; };                        // block of the sequence's table, first position, positions (none: 0)
+CB_HD Kv8Piece kv8_piece(const Kv8Seqs& s, const Kv8Seq& q, int page, int b, int at, bool by_row) {
+    const int begin = most(q.first, 0);
+    int block;
+    if (by_row) {
+        const int pos = q.first + (at - q.s0);
+        if (at < q.s0 || at >= q.s0 + q.n || pos < 0 || (pos != begin && pos % page)) return {0, 0, 0};
+        block = pos / page;
+    } else {
+        block = begin / page + (at - kv8_piece_key(s, page, b, false));
+    }
+    if (block < 0 || (long long)block * page >= q.len) return {0, 0, 0};
+    const int pos = most(begin, block * page);
+    return {block, pos, most((int)least((long long)q.len, (long long)block * page + page) - pos, 0)};
+}
+
+// ---- attention: how the steps are dealt out ----------------------------------------------------------------------------------------
+// A unit is a sequence, a kv head and a group of M rows of its queries (row = token * group + head of the group); its steps are the tiles of TILE positions, one at least.  All
+// steps, unit after unit, are dealt out evenly to the CTAs, whatever the lengths: a unit may lie with several CTAs, which then leave their parts of the sums to be joined.
+template <int M, int TILE>
+struct Kv8Units {
+    int b, head, grp;                          // the unit
+    Kv8Seq q;
+    int tiles, groups;
+    long long first;                           // number of its first step
+    CB_HD void shape(const Kv8Seqs& s, const Kv8Pool& p, int group) {
+        q = kv8_seq(s, b);
+        groups = (int)(((long long)q.n * group + M - 1) / M);
+        tiles = most(1, (int)((least((long long)q.len, (long long)s.width * p.page) + TILE - 1) / TILE));
+    }
+    CB_HD long long steps(const Kv8Pool& p) const { return (long long)groups * p.kv_heads * tiles; }
+    CB_HD bool next(const Kv8Seqs& s, const Kv8Pool& p, int group) {           // false: behind the last
+        first += tiles;
+        if (++grp < groups) return true;
+        grp = 0;
+        if (++head < p.kv_heads) return true;
+        head = 0;
+        do {
+            if (++b >= s.seqs) return false;
+            shape(s, p, group);
+        } while (!groups);
+        return true;
+    }
+    // The unit that holds a step; sequences are counted off from b on, which begins with step `at`
+    CB_HD void seek(const Kv8Seqs& s, const Kv8Pool& p, int group, int from, long long at, long long step) {
+        for (b = from;; ++b) {
+            shape(s, p, group);
+            const long long c = steps(p);
+            if (step < at + c || b + 1 >= s.seqs) break;
+            at += c;
+        }
+        const long long k = (step - at) / tiles;
+        head = (int)(k / most(groups, 1));
+        grp = (int)(k - (long long)head * groups);
+        first = at + k * tiles;
+    }
+};
+CB_HD long long kv8_range(long long total, int ctas, int c) { return total / ctas * c + least((long long)c, total % ctas); }       // a CTA's first step
+CB_HD int kv8_owner(long long total, int ctas, long long step) {
+    const long long base = total / ctas, rem = total % ctas, big = rem * (base + 1);
+    return (int)(step < big ? step / (base + 1) : rem + (step - big) / most(base, 1LL));
+}
+// Where a CTA leaves its part of a unit that it shares: 0 for the one that its range begins with, 1 for the one that it ends with
+CB_HD int kv8_slot(int cta, long long begin, long long part) { return 2 * cta + (part == begin ? 0 : 1); }
+
+}  // namespace cb

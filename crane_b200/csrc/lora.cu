@@ -1,0 +1,453 @@
+// Low-rank adapters of many requests (lora.cuh).  One kernel: a cluster of CTAs has a tile of rows that go through the same adapter.  Its CTAs each take a share of the
+// k columns of T = X A^T, add their shares up in distributed shared memory, and then each take a share of the n columns of out = add + s T B^T.  T never leaves the SMs;
+// there is no workspace and nothing to wait for outside the cluster.
+//
+// T is f32 and multiplied by the adapter's scale before it is split into two parts of the weights' type (bf16: 16 bits; f16: 22, each row moved into f16's range by a power of
+// two of its own), so that the rank's sum loses nothing that a 16-bit result could show.  f32 weights or rows: tf32 parts, hi hi + lo hi + hi lo, 2^-22 of each product.
+//
+// Bound by bytes: for single rows those of A and B, for prompts those of add and out.  Fragments come straight from global memory: which k a place of a fragment stands for is free
+// as long as both operands agree, so a lane takes 16 neighbouring bytes of a row, and the columns of a result are dealt so that a lane leaves eight neighbours.
+#include <cuda_fp16.h>
+
+#include "lora.cuh"
+#include "tc.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int THREADS = 256, WARPS = 8;
+
+template <typename T> constexpr int TYPE = 0;
+template <> constexpr int TYPE<bf16> = 1;
+template <> constexpr int TYPE<__half> = 2;
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<bf16>(bf16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 from_f<bf16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+
+// N neighbouring elements as they lie, `have` of them there (VEC: all or none, aligned); the rest zeros
+template <typename T, int N> struct Piece {
+    static constexpr int W = N * (int)sizeof(T) / 4;
+    uint32_t w[W];
+    __device__ __forceinline__ float at(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else {
+            const unsigned short u = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
+            if constexpr (TYPE<T> == 1) return __uint_as_float((uint32_t)u << 16);
+            else return __half2float(__ushort_as_half(u));
+        }
+    }
+};
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ Piece<T, N> load(const T* p, int have) {
+    Piece<T, N> r;
+#pragma unroll
+    for (int i = 0; i < r.W; ++i) r.w[i] = 0;
+    if constexpr (VEC) {
+        if (have >= N) {
+#pragma unroll
+            for (int i = 0; i < r.W; i += r.W < 4 ? 2 : 4) {
+                if constexpr (Piece<T, N>::W < 4) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); r.w[0] = v.x; r.w[1] = v.y; }
+                else { const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4); r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w; }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i < have) {
+                if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(__ldg(reinterpret_cast<const float*>(p) + i));
+                else r.w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p) + i) << (16 * (i & 1));
+            }
+        }
+    }
+    return r;
+}
+
+template <typename W> __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (TYPE<W> == 1)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tf32(float v) { uint32_t r; asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v)); return r; }
+// what `hi` leaves of v; nothing of an infinity (inf - inf would make a NaN of it)
+__device__ __forceinline__ float rest(float v, float hi) { return fabsf(hi) < INFINITY ? v - hi : 0.f; }
+__device__ __forceinline__ uint32_t tf32_rest(float v, uint32_t hi) { return tf32(rest(v, __uint_as_float(hi))); }
+
+template <typename X, typename W, int MT, int RT>
+struct Shape {
+    static constexpr bool T32 = sizeof(X) == 4;                      // tf32 products; else those of the 16-bit type
+    static constexpr int ROWS = 16 * MT, RP = 8 * RT, LDT = RP + 4;
+    static constexpr int KS = T32 ? RT : RT / 2;                     // MMAs along the rank
+    static constexpr int T_BYTES = ROWS * LDT * 4, FRAG = MT * KS * 32 * 16;
+    static constexpr int SMEM = 2 * T_BYTES + 2 * FRAG;              // shares of T (this CTA's, read by the cluster), T, its two parts
+};
+
+template <typename X, typename W, int MT, int RT, bool VEC>
+__global__ void __launch_bounds__(THREADS)
+lora_kernel(Lora l, bool gather) {
+    using S = Shape<X, W, MT, RT>;
+    constexpr bool T32 = S::T32;
+    constexpr int ROWS = S::ROWS, LDT = S::LDT, KS = S::KS, MW = MT == 4 ? 2 : 1, KW = WARPS / MW, MPW = MT / MW;
+    extern __shared__ __align__(16) unsigned char sm[];
+    float* share = reinterpret_cast<float*>(sm);
+    float* ts = reinterpret_cast<float*>(sm + S::T_BYTES);
+    uint4* hi_s = reinterpret_cast<uint4*>(sm + 2 * S::T_BYTES);
+    uint4* lo_s = hi_s + S::FRAG / 16;
+    __shared__ int rows_s[ROWS], which_s[ROWS];
+    __shared__ float down_s[ROWS];                                   // powers of two that take the rows of T back out of f16's range
+    __shared__ int n_rows_s;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    uint32_t cl;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cl));
+    const int cr = (int)cluster_rank(), nc = (int)cl, tile = blockIdx.x / nc;
+
+    // ---- the tile's rows ----
+    if (gather) {
+        // tile r: rows r and on that go through row r's adapter, if the number of those ahead of r is a multiple of ROWS
+        if (warp == 0) {
+            const int w = __ldg(l.which + tile);
+            int w0 = (unsigned)w < (unsigned)l.adapters ? w : -1, ahead = 0, have = 0;
+            for (int i = 0; i < l.m && have < ROWS; i += 32) {
+                int v = -2;
+                if (i + lane < l.m) { v = __ldg(l.which + i + lane); if ((unsigned)v >= (unsigned)l.adapters) v = -1; }
+                const unsigned same = __ballot_sync(0xffffffffu, v == w0);
+                const unsigned from = i + 31 < tile ? 0u : i >= tile ? 0xffffffffu : 0xffffffffu << (tile - i);      // rows >= tile
+                ahead += __popc(same & ~from);
+                const unsigned mine = same & from;
+                const int at = have + __popc(mine & ((1u << lane) - 1));
+                if ((mine >> lane & 1) && at < ROWS) { rows_s[at] = i + lane; which_s[at] = w0; }
+                have = min(ROWS, have + __popc(mine));
+                if (i + 31 >= tile && ahead % ROWS) break;
+            }
+            if (lane == 0) n_rows_s = ahead % ROWS ? 0 : have;
+        }
+    } else {
+        for (int i = tid; i < ROWS; i += THREADS) {
+            const int r = tile * ROWS + i;
+            rows_s[i] = r;
+            int v = r < l.m ? __ldg(l.which + r) : -1;
+            which_s[i] = (unsigned)v < (unsigned)l.adapters ? v : -1;
+        }
+        if (tid == 0) n_rows_s = min(ROWS, l.m - tile * ROWS);
+    }
+    __syncthreads();
+    const int n_rows = n_rows_s;
+    if (n_rows == 0) return;                                         // (the whole cluster's CTAs alike)
+
+    const X* x = reinterpret_cast<const X*>(l.x);
+    const X* add = reinterpret_cast<const X*>(l.add);
+    X* out = reinterpret_cast<X*>(l.out);
+    const int nb = (l.n + 31) / 32, nb0 = (int)((long long)nb * cr / nc), nb1 = (int)((long long)nb * (cr + 1) / nc);
+    unsigned long long left = n_rows == 64 ? ~0ull : (1ull << n_rows) - 1;
+    while (left) {
+        // ---- the next adapter among the rows that are left ----
+        const int w = which_s[__ffsll(left) - 1];
+        unsigned long long mine = __ballot_sync(0xffffffffu, lane < ROWS && which_s[lane % ROWS] == w);
+        if constexpr (ROWS > 32) mine |= (unsigned long long)__ballot_sync(0xffffffffu, which_s[(lane + 32) % ROWS] == w) << 32;
+        mine &= left;
+        left &= ~mine;
+        float o[MT][4][4];
+        if (w >= 0) {
+            // ---- this CTA's share of T ----
+            const W* A = reinterpret_cast<const W*>(l.a) + (size_t)w * l.rank * l.k;
+            float acc[MPW][RT][4];
+#pragma unroll
+            for (int i = 0; i < MPW; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+            const int mw = warp % MW, kw = warp / MW;
+            const X* xr[MPW][2];
+#pragma unroll
+            for (int i = 0; i < MPW; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = (mw * MPW + i) * 16 + h * 8 + g;
+                    xr[i][h] = r < n_rows && (mine >> r & 1) ? x + (long long)rows_s[r] * l.ldx : nullptr;
+                }
+            const int kc = (l.k + 31) / 32, k0 = (int)((long long)kc * cr / nc), k1 = (int)((long long)kc * (cr + 1) / nc);
+            for (int c = k0 + kw; c < k1; c += KW) {
+                const int at = c * 32 + 8 * t, have = l.k - at;
+                Piece<X, 8> xv[MPW][2];
+#pragma unroll
+                for (int i = 0; i < MPW; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) xv[i][h] = load<X, 8, VEC>(xr[i][h] + at, xr[i][h] ? have : 0);
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const int r = j * 8 + g;
+                    const Piece<W, 8> av = load<W, 8, VEC>(A + (size_t)r * l.k + at, r < l.rank ? have : 0);
+                    if constexpr (!T32) {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int i = 0; i < MPW; ++i) {
+                                const uint32_t f[4] = {xv[i][0].w[2 * s], xv[i][1].w[2 * s], xv[i][0].w[2 * s + 1], xv[i][1].w[2 * s + 1]};
+                                mma16<W>(acc[i][j], f, av.w[2 * s], av.w[2 * s + 1]);
+                            }
+                    } else {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            uint32_t bh[2], bl[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) { bh[e] = tf32(av.at(2 * s + e)); if (sizeof(W) == 4) bl[e] = tf32_rest(av.at(2 * s + e), bh[e]); }
+#pragma unroll
+                            for (int i = 0; i < MPW; ++i) {
+                                uint32_t fh[4], fl[4];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) { const float v = xv[i][e & 1].at(2 * s + (e >> 1)); fh[e] = tf32(v); fl[e] = tf32_rest(v, fh[e]); }
+                                if (sizeof(W) == 4) mma_tf32(acc[i][j], fh, bl[0], bl[1]);
+                                mma_tf32(acc[i][j], fl, bh[0], bh[1]);
+                                mma_tf32(acc[i][j], fh, bh[0], bh[1]);
+                            }
+                        }
+                    }
+                }
+            }
+            // ---- the warps' sums one after the other, then the cluster's: the order is the same every time ----
+            for (int turn = 0; turn < KW; ++turn) {
+                if (kw == turn) {
+#pragma unroll
+                    for (int i = 0; i < MPW; ++i)
+#pragma unroll
+                        for (int j = 0; j < RT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float* p = share + ((mw * MPW + i) * 16 + g + 8 * (e >> 1)) * LDT + j * 8 + 2 * t + (e & 1);
+                                *p = turn ? *p + acc[i][j][e] : acc[i][j][e];
+                            }
+                }
+                __syncthreads();
+            }
+            if (nc > 1) cluster_sync_all();
+            const float s = l.scales ? __ldg(l.scales + w) : 1.f;
+            for (int i = tid; i < ROWS * S::RP; i += THREADS) {
+                const int at = i / S::RP * LDT + i % S::RP;
+                float v = 0.f;
+                for (int c = 0; c < nc; ++c) {
+                    if (nc == 1) { v = share[at]; break; }
+                    float y;
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(peer_smem(share + at, c)) : "memory");
+                    v += y;
+                }
+                ts[at] = s * v;
+            }
+            __syncthreads();
+            if constexpr (TYPE<W> == 2 && !T32) {
+                for (int r = warp; r < ROWS; r += WARPS) {
+                    float top = 0.f;
+                    for (int i = lane; i < S::RP; i += 32) top = fmaxf(top, fabsf(ts[r * LDT + i]));
+                    top = warp_max(top);
+                    const uint32_t e = __float_as_uint(fminf(fmaxf(top, 0x1p-100f), 0x1p120f)) >> 23;
+                    const float up = top < INFINITY ? __uint_as_float((268 - e) << 23) : 1.f;      // the largest of the row to [2^14, 2^15)
+                    for (int i = lane; i < S::RP; i += 32) ts[r * LDT + i] *= up;
+                    if (lane == 0) down_s[r] = top < INFINITY ? __uint_as_float((e - 14) << 23) : 1.f;
+                }
+                __syncthreads();
+            }
+            for (int i = tid; i < MT * KS * 32; i += THREADS) {
+                const int ln = i & 31, ks = i / 32 % KS, mt = i / 32 / KS, gg = ln >> 2, tt = ln & 3;
+                uint32_t h[4], lo[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float* p = ts + (mt * 16 + gg + 8 * (e & 1)) * LDT;
+                    if constexpr (T32) {                             // 16 columns of the rank are two MMAs, lane t has columns 4 t .. 4 t + 3
+                        const float v = p[ks / 2 * 16 + 4 * tt + (ks & 1) * 2 + (e >> 1)];
+                        h[e] = tf32(v);
+                        lo[e] = tf32_rest(v, h[e]);
+                    } else {
+                        const float a = p[ks * 16 + 4 * tt + (e >> 1) * 2], b = p[ks * 16 + 4 * tt + (e >> 1) * 2 + 1];
+                        if constexpr (TYPE<W> == 1) {
+                            h[e] = pack_bf16(a, b);
+                            lo[e] = pack_bf16(rest(a, bf16lo(h[e])), rest(b, bf16hi(h[e])));
+                        } else {
+                            const __half2 hh = __floats2half2_rn(a, b);
+                            const float2 f = __half22float2(hh);
+                            const __half2 ll = __floats2half2_rn(rest(a, f.x), rest(b, f.y));
+                            h[e] = *reinterpret_cast<const uint32_t*>(&hh);
+                            lo[e] = *reinterpret_cast<const uint32_t*>(&ll);
+                        }
+                    }
+                }
+                hi_s[i] = make_uint4(h[0], h[1], h[2], h[3]);
+                lo_s[i] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            }
+            __syncthreads();
+        }
+        // ---- out = add + T B^T: 32 columns a warp at a time ----
+        const W* B = reinterpret_cast<const W*>(l.b) + (size_t)max(w, 0) * l.n * l.rank;
+        if (w >= 0 || add != out)
+            for (int b = nb0 + warp; b < nb1; b += WARPS) {
+                const int n0 = b * 32, col = n0 + t * 8, have = l.n - col;
+                Piece<X, 8> av[MT][2];
+                if (add) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = i * 16 + h * 8 + g;
+                            const bool in = mine >> r & 1;
+                            // (may be out: not through the read-only path)
+                            const X* p = add + (in ? (long long)rows_s[r] * l.ldadd : 0) + col;
+#pragma unroll
+                            for (int q = 0; q < Piece<X, 8>::W; ++q) av[i][h].w[q] = 0;
+                            if constexpr (VEC) {
+                                if (in && have >= 8) {
+#pragma unroll
+                                    for (int q = 0; q < Piece<X, 8>::W; q += 4) {
+                                        const uint4 v = reinterpret_cast<const uint4*>(p)[q / 4];
+                                        av[i][h].w[q] = v.x; av[i][h].w[q + 1] = v.y; av[i][h].w[q + 2] = v.z; av[i][h].w[q + 3] = v.w;
+                                    }
+                                }
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q)
+                                    if (in && q < have) {
+                                        if constexpr (sizeof(X) == 4) av[i][h].w[q] = reinterpret_cast<const uint32_t*>(p)[q];
+                                        else av[i][h].w[q / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[q] << (16 * (q & 1));
+                                    }
+                            }
+                        }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int q = 0; q < Piece<X, 8>::W; ++q) av[i][0].w[q] = av[i][1].w[q] = 0;
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+                if (w >= 0) {
+#pragma unroll 2
+                    for (int ks = 0; ks < RT / 2; ++ks) {
+                        if (ks * 16 >= l.rank) break;
+                        Piece<W, 4> bv[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = n0 + (g >> 1) * 8 + j * 2 + (g & 1), c = ks * 16 + 4 * t;
+                            bv[j] = load<W, 4, VEC>(B + (size_t)r * l.rank + c, r < l.n ? l.rank - c : 0);
+                        }
+                        if constexpr (!T32) {
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) {
+                                const uint4 hv = hi_s[(i * KS + ks) * 32 + lane], lv = lo_s[(i * KS + ks) * 32 + lane];
+                                const uint32_t fh[4] = {hv.x, hv.y, hv.z, hv.w}, fl[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) { mma16<W>(o[i][j], fl, bv[j].w[0], bv[j].w[1]); mma16<W>(o[i][j], fh, bv[j].w[0], bv[j].w[1]); }
+                            }
+                        } else {
+#pragma unroll
+                            for (int s = 0; s < 2; ++s) {
+                                uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) { const float v = bv[j].at(2 * s + e); bh[j][e] = tf32(v); if (sizeof(W) == 4) bl[j][e] = tf32_rest(v, bh[j][e]); }
+#pragma unroll
+                                for (int i = 0; i < MT; ++i) {
+                                    const uint4 hv = hi_s[(i * KS + ks * 2 + s) * 32 + lane], lv = lo_s[(i * KS + ks * 2 + s) * 32 + lane];
+                                    const uint32_t fh[4] = {hv.x, hv.y, hv.z, hv.w}, fl[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        if (sizeof(W) == 4) mma_tf32(o[i][j], fh, bl[j][0], bl[j][1]);
+                                        mma_tf32(o[i][j], fl, bh[j][0], bh[j][1]);
+                                        mma_tf32(o[i][j], fh, bh[j][0], bh[j][1]);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = i * 16 + h * 8 + g;
+                        if (!(mine >> r & 1) || have <= 0) continue;
+                        X* p = out + (long long)rows_s[r] * l.ldo + col;
+                        const float down = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[r] : 1.f;
+                        X y[8];
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[i][q >> 1][2 * h + (q & 1)], down, av[i][h].at(q)));
+                        if constexpr (VEC) {
+                            if (have >= 8)
+#pragma unroll
+                                for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(y)[q];
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
+                        }
+                    }
+            }
+        if (w >= 0) { if (nc > 1) cluster_sync_all(); else __syncthreads(); }      // every CTA has read the shares: they may be written again, or their owner may leave
+    }
+}
+
+template <typename X, typename W, int MT, int RT, bool VEC>
+int launch(cudaStream_t st, const Lora& l, bool gather, int cluster, bool pdl) {
+    using S = Shape<X, W, MT, RT>;
+    static SmemOptIn seen;
+    auto kernel = lora_kernel<X, W, MT, RT, VEC>;
+    if (const int e = ensure_dyn_smem(kernel, (size_t)S::SMEM, seen)) return e;
+    const int tiles = gather ? l.m : (l.m + S::ROWS - 1) / S::ROWS;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)tiles * cluster); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, l, gather);
+}
+template <typename X, typename W, int MT, bool VEC>
+int launch_rank(cudaStream_t st, const Lora& l, bool gather, int cluster, bool pdl) {
+    if (l.rank <= 16) return launch<X, W, MT, 2, VEC>(st, l, gather, cluster, pdl);
+    if (l.rank <= 32) return launch<X, W, MT, 4, VEC>(st, l, gather, cluster, pdl);
+    if (l.rank <= 64) return launch<X, W, MT, 8, VEC>(st, l, gather, cluster, pdl);
+    return launch<X, W, MT, 16, VEC>(st, l, gather, cluster, pdl);
+}
+template <typename X, typename W>
+int launch_types(cudaStream_t st, const Lora& l, bool vec, bool pdl) {
+    const bool gather = l.m <= 256;
+    const int tiles = gather ? (l.m + 7) / 8 : (l.m + 63) / 64, sms = tc_device_sms();
+    int cluster = 1;
+    while (cluster < 8 && tiles * cluster * 2 <= 2 * sms) cluster *= 2;
+    if (gather) return vec ? launch_rank<X, W, 1, true>(st, l, true, cluster, pdl) : launch_rank<X, W, 1, false>(st, l, true, cluster, pdl);
+    return vec ? launch_rank<X, W, 4, true>(st, l, false, cluster, pdl) : launch_rank<X, W, 4, false>(st, l, false, cluster, pdl);
+}
+
+}  // namespace
+
+int lora_linear_launch(cudaStream_t st, const Lora& l, bool pdl) {
+    if (l.m == 0 || l.n == 0) return 0;
+    if (l.rank < 1 || l.rank > LORA_MAX_RANK) return -1000;
+    const int xe = l.type == LORA_F32 ? 4 : 2, we = l.w_type == LORA_F32 ? 4 : 2;
+    auto on16 = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
+    const bool vec = on16(l.x) && on16(l.a) && on16(l.b) && on16(l.out) && (!l.add || on16(l.add)) && (l.ldx * xe) % 16 == 0 && (l.ldo * xe) % 16 == 0 &&
+                     (!l.add || (l.ldadd * xe) % 16 == 0) && l.k % 8 == 0 && l.n % 8 == 0 && (l.rank * we) % 16 == 0 && l.rank % 4 == 0 && ((long long)l.k * we) % 16 == 0;
+    if (l.type == LORA_F32) {
+        if (l.w_type == LORA_F32) return launch_types<float, float>(st, l, vec, pdl);
+        if (l.w_type == LORA_BF16) return launch_types<float, bf16>(st, l, vec, pdl);
+        if (l.w_type == LORA_F16) return launch_types<float, __half>(st, l, vec, pdl);
+    } else if (l.type == l.w_type) {
+        if (l.type == LORA_BF16) return launch_types<bf16, bf16>(st, l, vec, pdl);
+        if (l.type == LORA_F16) return launch_types<__half, __half>(st, l, vec, pdl);
+    }
+    return -1000;
+}
+
+}  // namespace cb

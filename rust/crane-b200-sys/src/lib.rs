@@ -121,6 +121,13 @@ extern "C" {
     pub fn crane_b200_fp8_rms_norm(device: c_int, x: *const c_void, dtype: c_int, ldx: usize, residual: *const c_void, residual_out: *mut c_void, res_dtype: c_int, ldr: usize, weight: *const c_void, w_dtype: c_int, eps: f32, m: usize, k: usize, codes: *mut u8, ld: usize, scales: *mut f32, lds: usize, stream: *mut c_void) -> c_int;
     pub fn crane_b200_fp8_linear(device: c_int, x: *const u8, ldx: usize, x_scales: *const f32, lds: usize, w: *const u8, ldw: usize, w_scales: *const f32, ldws: usize, m: usize, n: usize, k: usize, add: *const c_void, ldadd: usize, out: *mut c_void, dtype: c_int, ldo: usize, stream: *mut c_void) -> c_int;
     pub fn crane_b200_fp8_status(device: c_int, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_device_last_error() -> *const c_char;
+    pub fn crane_b200_kv8_append(device: c_int, k: *const c_void, ldk: usize, ldkh: usize, v: *const c_void, ldv: usize, ldvh: usize, dtype: c_int, k_codes: *mut u8, v_codes: *mut u8, scales: *mut f32, pages: usize, kv_heads: usize, page: usize, dim: usize, table: *const i32, ldt: usize, width: usize, lens: *const i32, starts: *const i32, seqs: usize, rows: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_kv8_attention_bytes(device: c_int, heads: usize, kv_heads: usize, dim: usize, seqs: usize, rows: usize, max_rows: usize, bytes: *mut usize) -> c_int;
+    pub fn crane_b200_kv8_attention(device: c_int, q: *const c_void, ldq: usize, ldqh: usize, out: *mut c_void, ldo: usize, ldoh: usize, dtype: c_int, heads: usize, scale: f32, k_codes: *const u8, v_codes: *const u8, scales: *const f32, pages: usize, kv_heads: usize, page: usize, dim: usize, table: *const i32, ldt: usize, width: usize, lens: *const i32, starts: *const i32, seqs: usize, rows: usize, max_rows: usize, work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_lora_linear(device: c_int, x: *const c_void, ldx: usize, dtype: c_int, a: *const c_void, b: *const c_void, w_dtype: c_int, adapters: usize, rank: usize, which: *const i32, scales: *const f32, add: *const c_void, ldadd: usize, out: *mut c_void, ldo: usize, m: usize, n: usize, k: usize, stream: *mut c_void) -> c_int;
+    pub fn crane_b200_draft_verify_bytes(device: c_int, vocab: usize, seqs: usize, drafts: usize, with_draft_logits: c_int, bytes: *mut usize) -> c_int;
+    pub fn crane_b200_draft_verify(device: c_int, logits: *const c_void, ld: usize, draft_logits: *const c_void, ldd: usize, dtype: c_int, vocab: usize, tokens: *const i32, starts: *const i32, seqs: usize, drafts: usize, temperatures: *const f32, uniforms: *const f32, noise: *const f32, ldn: usize, accepted: *mut i32, next: *mut i32, work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn crane_b200_op_gemm(device: c_int, a: *const u16, a_lo: *const u16, w: *const u16, M: c_int, N: c_int, K: c_int, mode: c_int, bias: *const f32, out_inout: *mut c_void, use_simt: c_int) -> c_int;
     pub fn crane_b200_op_gemm_epi(device: c_int, a: *const u16, a_lo: *const u16, w: *const u16, M: c_int, N: c_int, K: c_int, mode: c_int, bias: *const f32, col_scale: *const f32, gate: *const f32, gate_bias: *const f32, glu_limit: f32, out_inout: *mut c_void, out_lo: *mut u16) -> c_int;
     pub fn crane_b200_op_qlinear(device: c_int, x: *const f32, m: usize, k: usize, raw: *const c_void, raw_bytes: usize, ggml_type: c_int, n: usize, norm_w: *const f32, eps: f32, y: *mut f32) -> c_int;
