@@ -22,45 +22,12 @@ struct Args {
     const void* q; long long ldq, ldqh;
     void* out; long long ldo, ldoh;
     float scale2, scale2_rest;                 // scale * log2 e, and what f32 leaves of it
-    int heads, group;                          // query heads; those that share a kv head
-    Kv8Pool pool;
-    Kv8Seqs s;
+    Kv8Deal d;
     float* work;                               // [2 * CTAs][rows of a group of rows][D + 2]
     int* err;
 };
 
 template <int M> using Units = Kv8Units<M, TILE>;
-// Every thread of the block: the steps of all sequences (kv8_units.h), and, by thread share, those ahead of each share.  `sums` [threads + 1].
-template <int M>
-__device__ __forceinline__ long long count_steps(const Args& a, long long* sums, int threads) {
-    const int tid = threadIdx.x, per = (a.s.seqs + threads - 1) / threads;
-    long long mine = 0;
-    if (tid < threads)
-        for (int i = tid * per; i < min(a.s.seqs, tid * per + per); ++i) {
-            Units<M> u; u.b = i; u.shape(a.s, a.pool, a.group);
-            mine += u.steps(a.pool);
-        }
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const long long t = __shfl_up_sync(0xffffffffu, incl, o); if ((tid & 31) >= o) incl += t; }
-    __shared__ long long wsum[32];
-    if ((tid & 31) == 31) wsum[tid >> 5] = incl;
-    __syncthreads();
-    long long before = 0, all = 0;
-    for (int w = 0; w < (int)(blockDim.x + 31) / 32; ++w) { if (w < (tid >> 5)) before += wsum[w]; all += wsum[w]; }
-    if (tid < threads) sums[tid] = before + incl - mine;
-    if (tid == 0) sums[threads] = all;
-    __syncthreads();
-    return all;
-}
-template <int M>
-__device__ __forceinline__ Units<M> find_unit(const Args& a, const long long* sums, int threads, long long step) {
-    int lo = 0, n = threads;                   // the last share that begins at or ahead of the step
-    while (n > 1) { const int h = n / 2; if (sums[lo + h] <= step) { lo += h; n -= h; } else n = h; }
-    Units<M> u;
-    u.seek(a.s, a.pool, a.group, lo * ((a.s.seqs + threads - 1) / threads), sums[lo], step);
-    return u;
-}
 
 // ---- fragments -------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void lds16(uint32_t a, uint32_t* r) { asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a)); }
@@ -129,7 +96,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     uint32_t* qs = reinterpret_cast<uint32_t*>(sm + STAGES * St::BYTES + S::JOIN);
     __shared__ uint64_t full[STAGES], empty[STAGES];
     __shared__ float4 meta[STAGES][4];                       // of each 16 positions: ks, log2 vs, 1 / vs, and whether there is a page
-    __shared__ long long sums[129];
+    __shared__ long long sums[KV8_SHARES + 1];
     __shared__ int gave_up;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
@@ -140,15 +107,15 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     }
     const TcWait wait{&gave_up, a.err};
     pdl_wait();
-    const long long total = count_steps<M>(a, sums, 128);
+    const long long total = kv8_count<Units<M>>(a.d, sums);
     const long long begin = kv8_range(total, gridDim.x, blockIdx.x), end = kv8_range(total, gridDim.x, blockIdx.x + 1);
     pdl_launch_dependents();
     if (begin >= end) return;
-    Units<M> u = find_unit<M>(a, sums, 128, begin);
+    Units<M> u = kv8_find<Units<M>>(a.d, sums, begin);
 
     if (warp == S::WARPS) {
         // ---- copies: a box per page (64 positions of it at most) and plane ----
-        const int P = a.pool.page, rows = min(P, TILE), boxes = TILE / rows;
+        const int P = a.d.p.page, rows = min(P, TILE), boxes = TILE / rows;
         int stage = 0;
         uint32_t parity = 1;
         for (long long step = begin; step < end;) {
@@ -158,10 +125,10 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 int row = -1;
                 float4 sc = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (base + lane < n) {
-                    const int pos = t0 * TILE + (base + lane) * rows, page = pos < u.q.len ? kv8_page(a.s, a.pool, u.b, pos / P) : -1;
+                    const int pos = t0 * TILE + (base + lane) * rows, page = pos < u.q.len ? kv8_page(a.d.s, a.d.p, u.b, pos / P) : -1;
                     if (page >= 0) {
-                        row = (page * a.pool.kv_heads + u.head) * P + pos % P;
-                        const float2 kv = *reinterpret_cast<const float2*>(a.pool.scales + ((size_t)page * a.pool.kv_heads + u.head) * 2);
+                        row = (page * a.d.p.kv_heads + u.head) * P + pos % P;
+                        const float2 kv = *reinterpret_cast<const float2*>(a.d.p.scales + ((size_t)page * a.d.p.kv_heads + u.head) * 2);
                         const float vs = fmaxf(kv.y, 0x1p-120f);
                         sc = make_float4(kv.x, log2f(vs), __frcp_rn(vs), 1.f);
                     }
@@ -179,7 +146,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     __syncwarp();
                     for (int j = 0; j < boxes; ++j) {
                         int r = __shfl_sync(0xffffffffu, row, i - base + j);
-                        if (r < 0) r = a.pool.pages * a.pool.kv_heads * P;       // behind the pool: zeros come
+                        if (r < 0) r = a.d.p.pages * a.d.p.kv_heads * P;       // behind the pool: zeros come
                         if (lane < 2 * St::PLANES) {
                             const int pl = lane >> 1;
                             tma_load_2d(st + (lane & 1) * St::PLANES * St::PLANE + pl * St::PLANE + j * rows * St::BOX, lane & 1 ? &map_v : &map_k, &full[stage], pl * St::BOX, r);
@@ -189,7 +156,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 }
             }
             step = u.first + t1;
-            if (step < end && !u.next(a.s, a.pool, a.group)) break;
+            if (step < end && !u.next(a.d)) break;
         }
         __syncwarp();
         // (the last copies have landed when the consumers' last waits return)
@@ -213,7 +180,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 row[r] = u.grp * M + mg * 16 + g + r * 8;
-                const int tok = row[r] / a.group, h = u.head * a.group + row[r] % a.group;
+                const int tok = row[r] / a.d.group, h = u.head * a.d.group + row[r] % a.d.group;
                 const bool in = tok < u.q.n;
                 pmax[r] = in ? u.q.first + tok : -1;
                 if (in) wmin = min(wmin, pmax[r]);
@@ -460,7 +427,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             const bool whole = t0 == 0 && t1 == u.tiles;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const int row = mg * 16 + g + r * 8, tok = (u.grp * M + row) / a.group, h = u.head * a.group + (u.grp * M + row) % a.group;
+                const int row = mg * 16 + g + r * 8, tok = (u.grp * M + row) / a.d.group, h = u.head * a.d.group + (u.grp * M + row) % a.d.group;
                 if (whole) {
                     if (tok >= u.q.n) continue;
                     T* dst = reinterpret_cast<T*>(a.out) + (long long)(u.q.s0 + tok) * a.ldo + (long long)h * a.ldoh;
@@ -487,26 +454,27 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             }
         }
         step = u.first + t1;
-        if (step < end && !u.next(a.s, a.pool, a.group)) break;
+        if (step < end && !u.next(a.d)) break;
     }
     if (tid == 0) wait.drain();
 }
 
 // Adds up the parts of the units that lie with several CTAs.  Block x: unit boundaries between CTAs x and x + 1, if the unit does not reach back to CTA x - 1's steps.
-template <int D, typename T, int M>
+template <int D, typename T, int M, int TILE>
 __global__ void __launch_bounds__(128)
 join_kernel(Args a, int ctas) {
-    __shared__ long long sums[129];
+    using Units = Kv8Units<M, TILE>;
+    __shared__ long long sums[KV8_SHARES + 1];
     pdl_wait();
     pdl_launch_dependents();
-    const long long total = count_steps<M>(a, sums, 128);
+    const long long total = kv8_count<Units>(a.d, sums);
     const int c = blockIdx.x;
     const long long begin = kv8_range(total, ctas, c), end = kv8_range(total, ctas, c + 1);
     if (begin >= end || end >= total) return;
-    const Units<M> u = find_unit<M>(a, sums, 128, end - 1);          // the last unit of CTA c
+    const Units u = kv8_find<Units>(a.d, sums, end - 1);          // the last unit of CTA c
     if (u.first + u.tiles <= end || u.first < begin) return;         // ... ends there, or begins ahead of it
     const int last = kv8_owner(total, ctas, u.first + u.tiles - 1);
-    const int rows = (int)min((long long)M, (long long)u.q.n * a.group - (long long)u.grp * M);
+    const int rows = (int)min((long long)M, (long long)u.q.n * a.d.group - (long long)u.grp * M);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for (int row = blockIdx.y * 4 + warp; row < rows; row += 4 * gridDim.y) {
         float o[D / 32], m = -INFINITY, l = 0.f;
@@ -522,7 +490,7 @@ join_kernel(Args a, int ctas) {
 #pragma unroll
             for (int j = 0; j < D / 32; ++j) o[j] = o[j] * c0 + src[j * 32 + lane] * c1;
         }
-        const int rr = u.grp * M + row, tok = rr / a.group, h = u.head * a.group + rr % a.group;
+        const int rr = u.grp * M + row, tok = rr / a.d.group, h = u.head * a.d.group + rr % a.d.group;
         T* dst = reinterpret_cast<T*>(a.out) + (long long)(u.q.s0 + tok) * a.ldo + (long long)h * a.ldoh;
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -530,10 +498,18 @@ join_kernel(Args a, int ctas) {
     }
 }
 
-// Rows of a group of queries: 16 where no sequence brings more, else 32 or 64
-int rows_of(int group, int dim, int max_rows) {
+// Rows of a kv head from which on a sequence goes through kv8_flash.cu: 16-bit ones of 64 and 128 columns.
+constexpr int FLASH_FROM = 65;
+bool flash_takes(int type, int dim, int group, int max_rows) { return type != KV8_F32 && dim <= 128 && (long long)group * max_rows >= FLASH_FROM; }
+// Rows of a group of queries: 16 where no sequence brings more, else 32 or 64.  (Beside kv8_flash.cu 16: most of what is left are decoded tokens.)
+int rows_of(int group, int dim, int max_rows, bool flash) {
     const long long r = (long long)group * max_rows;
-    return r <= 16 ? 16 : r <= 32 || dim == 256 ? 32 : 64;
+    return r <= 16 || flash ? 16 : r <= 32 || dim == 256 ? 32 : 64;
+}
+template <typename T>
+int join_flash(cudaStream_t st, const Args& a) {
+    auto k = a.d.p.dim == 64 ? join_kernel<64, T, KV8_FLASH_ROWS, 128> : join_kernel<128, T, KV8_FLASH_ROWS, 128>;
+    return launch_k(k, dim3(tc_device_sms() - 1, 16), dim3(128), 0, st, true, a, tc_device_sms());
 }
 
 template <int D, typename T, int TG, int MG>
@@ -543,7 +519,7 @@ int launch(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const 
     if (const int e = ensure_dyn_smem(small_kernel<D, T, TG, MG>, (size_t)S::SMEM, seen)) return e;
     const int ctas = tc_device_sms() * S::CTAS;
     if (const int e = launch_k(small_kernel<D, T, TG, MG>, dim3(ctas), dim3(S::THREADS), S::SMEM, st, pdl, mk, mv, a)) return e;
-    return launch_k(join_kernel<D, T, S::M>, dim3(ctas - 1, S::M / 16), dim3(128), 0, st, true, a, ctas);
+    return launch_k(join_kernel<D, T, S::M, TILE>, dim3(ctas - 1, S::M / 16), dim3(128), 0, st, true, a, ctas);
 }
 template <int D, typename T>
 int launch_rows(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int rows, bool pdl) {
@@ -554,7 +530,7 @@ int launch_rows(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, c
 }
 template <typename T>
 int launch_dim(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int rows, bool pdl) {
-    switch (a.pool.dim) {
+    switch (a.d.p.dim) {
         case 64: return launch_rows<64, T>(st, mk, mv, a, rows, pdl);
         case 128: return launch_rows<128, T>(st, mk, mv, a, rows, pdl);
         case 256: return launch_rows<256, T>(st, mk, mv, a, rows, pdl);
@@ -564,14 +540,18 @@ int launch_dim(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, co
 
 }  // namespace
 
-size_t kv8_attention_bytes(int heads, int kv_heads, int dim, int rows, int seqs, int max_rows) {
+size_t kv8_attention_bytes(int type, int heads, int kv_heads, int dim, int rows, int seqs, int max_rows) {
     if (!rows || !seqs) return 0;
-    return (size_t)tc_device_sms() * 2 * 2 * rows_of(heads / kv_heads, dim, max_rows) * (dim + 2) * 4;
+    const bool flash = flash_takes(type, dim, heads / kv_heads, max_rows);
+    const size_t small = (size_t)tc_device_sms() * 2 * 2 * rows_of(heads / kv_heads, dim, max_rows, flash), large = flash ? (size_t)tc_device_sms() * 2 * KV8_FLASH_ROWS : 0;
+    return (small > large ? small : large) * (dim + 2) * 4;
 }
 
 int kv8_attention_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Pool& pool, const Kv8Seqs& s, bool pdl) {
     if (s.rows == 0 || s.seqs == 0) return 0;
-    const int rows = rows_of(k.heads / pool.kv_heads, pool.dim, k.max_rows), box = pool.dim < 128 ? pool.dim : 128;
+    const int group = k.heads / pool.kv_heads;
+    const bool flash = flash_takes(k.q.type, pool.dim, group, k.max_rows);
+    const int rows = rows_of(group, pool.dim, k.max_rows, flash), box = pool.dim < 128 ? pool.dim : 128;
     const uint64_t n = (uint64_t)pool.pages * pool.kv_heads * pool.page;
     CUtensorMap mk, mv;
     const CUtensorMapSwizzle sw = box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -579,13 +559,15 @@ int kv8_attention_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Pool& 
     if (!tc_tmap(&mk, pool.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, pool.dim, pool.dim, box_rows, box, sw) ||
         !tc_tmap(&mv, pool.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, pool.dim, pool.dim, box_rows, box, sw)) return (int)cudaErrorInvalidValue;
     const double scale2 = (double)k.scale * 1.4426950408889634074;
-    const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)scale2, (float)(scale2 - (double)(float)scale2), k.heads, k.heads / pool.kv_heads, pool, s, reinterpret_cast<float*>(k.work), k.err};
-    switch (k.q.type) {
-        case KV8_F32: return launch_dim<float>(st, mk, mv, a, rows, pdl);
-        case KV8_BF16: return launch_dim<bf16>(st, mk, mv, a, rows, pdl);
-        case KV8_F16: return launch_dim<__half>(st, mk, mv, a, rows, pdl);
-    }
-    return -1000;
+    const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)scale2, (float)(scale2 - (double)(float)scale2), Kv8Deal{s, pool, group, 0, flash ? FLASH_FROM - 1 : 1LL << 62}, reinterpret_cast<float*>(k.work), k.err};
+    if (k.q.type == KV8_F32) return launch_dim<float>(st, mk, mv, a, rows, pdl);
+    if (const int e = k.q.type == KV8_BF16 ? launch_dim<bf16>(st, mk, mv, a, rows, pdl) : launch_dim<__half>(st, mk, mv, a, rows, pdl)) return e;
+    if (!flash) return 0;
+    Args f = a;
+    f.d.lo = FLASH_FROM;
+    f.d.hi = 1LL << 62;
+    if (const int e = kv8_flash_launch(st, k, f.d, true)) return e;
+    return k.q.type == KV8_BF16 ? join_flash<bf16>(st, f) : join_flash<__half>(st, f);
 }
 
 }  // namespace cb

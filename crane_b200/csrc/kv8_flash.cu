@@ -1,0 +1,496 @@
+// Attention over an 8-bit paged cache (kv8.cuh) for sequences that bring many rows: 16-bit queries, tcgen05.  The mathematics is kv8_attention.cu's.
+//
+// Bound by the MMAs and, as much, by the exponentials: 256 query rows x 128 positions x D = 128 are 2 048 cycles of MMAs and as many of the SM's 16 exponentials a cycle.
+// A CTA has 256 query rows (two tiles of 128, each with its own softmax warps, scores and output in TMEM): while one tile's softmax runs, the other's MMAs do.  Codes come in by TMA
+// as they lie; four warps turn them into f16 operands once for both tiles (e4m3 is exact in f16; 32 K codes a step are 256 cvts a thread, under the MMAs), keys K-major, values
+// MN-major.  The alternative, codes as operands with queries and weights in two e4m3 parts each, needs no conversion but loses weights below 2^-19 of a row's
+// largest, and a first token that takes nearly everything is common.  Weights replace their scores in TMEM and are the A operand from there.
+// Work is dealt out by the 128-position step (kv8_units.h): persistent CTAs, whatever the lengths.
+#include <cuda_fp16.h>
+
+#include <climits>
+
+#include "kv8.cuh"
+#include "tc.cuh"
+
+namespace cb {
+namespace {
+
+constexpr int M = KV8_FLASH_ROWS, BN = 128, THREADS = 512;
+constexpr float P_SHIFT = 6.f;                 // weights run up to 2^14: the reference trails a row's maximum by up to 8
+using Units = Kv8Units<M, BN>;
+
+struct Args {
+    const void* q; long long ldq, ldqh;
+    void* out; long long ldo, ldoh;
+    float scale2, sign;                        // |scale| log2 e; the scale's sign goes with the queries
+    Kv8Deal d;
+    float* work;                               // [2 * CTAs][M][D + 2]
+    int* err;
+};
+template <int D> struct Cfg {
+    static constexpr int Q_TILE = 128 * D * 2, SLOT = BN * D * 2, RAW = BN * D;
+    static constexpr int NF = D == 128 ? 3 : 5, NR = D == 128 ? 3 : 4;      // operands (K and V of a step by turns), codes
+    static constexpr int SMEM = 2 * Q_TILE + NF * SLOT + NR * RAW + 1024;
+    static constexpr int C_S = 2 * D;                                       // TMEM columns: two outputs, two tiles of scores
+    static_assert(C_S + 2 * BN <= 512 && SMEM <= 218 * 1024, "");
+};
+constexpr int METAS = 8;      // steps whose scales are kept: the softmax is at most four behind the copies (three operand slots, three of codes)
+
+__device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t half2_of(uint32_t codes, int which) {
+    uint32_t r;
+    const uint16_t c = (uint16_t)(which ? codes >> 16 : codes);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) { uint32_t r; asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a)); return r; }
+template <typename T> __device__ __forceinline__ void pair(uint32_t w, float& a, float& b);
+template <> __device__ __forceinline__ void pair<bf16>(uint32_t w, float& a, float& b) { a = bf16lo(w); b = bf16hi(w); }
+template <> __device__ __forceinline__ void pair<__half>(uint32_t w, float& a, float& b) { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w)); a = f.x; b = f.y; }
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<bf16>(float a, float b) { return pack_bf16(a, b); }
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) { return pack_f16(a, b); }
+// MN-major operand, SWIZZLE_128B: 64 columns (128 B) x 8 positions per 1 KB atom; `lbo` bytes between 64-column groups, 1 KB between groups of 8 positions
+__device__ __forceinline__ uint64_t make_smem_desc_mn128(uint32_t smem_addr, uint32_t lbo) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(lbo >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+__device__ __forceinline__ bool has_nan(uint32_t codes) { return (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; }
+// bytes of a word that are NaN codes -> 0
+__device__ __forceinline__ uint32_t without_nan(uint32_t codes) {
+    const uint32_t n = (((codes & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+    return codes & ~(n * 255u);
+}
+
+template <int D, typename T, bool VEC>
+__global__ void __launch_bounds__(THREADS, 1)
+flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Args a) {
+    using C = Cfg<D>;
+    constexpr int NF = C::NF, NR = C::NR;
+    extern __shared__ uint8_t raw_sm[];
+    uint8_t* sm = raw_sm + (1024 - (smem_u32(raw_sm) & 1023)) % 1024;
+    uint8_t* ring = sm + 2 * C::Q_TILE;
+    uint8_t* codes = ring + NF * C::SLOT;
+    __shared__ uint64_t raw_full[NR], raw_empty[NR], full[NF], empty[NF], q_full[2], s_full[2], p_full[2], o_done[2];
+    __shared__ float4 meta[METAS][BN / 16];                  // of each 16 positions: ks, log2 vs, 1 / vs, and whether there is a page
+    __shared__ float factor_s[M];
+    __shared__ long long sums[KV8_SHARES + 1];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int gave_up, nan_part[METAS];                 // (a part has a step at least, so the converters are fewer parts ahead)
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        gave_up = 0;
+        for (int i = 0; i < METAS; ++i) nan_part[i] = -1;
+        for (int i = 0; i < NR; ++i) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+        for (int i = 0; i < NF; ++i) { mbar_init(&full[i], 4); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 4); mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 4); mbar_init(&o_done[i], 1); }
+        fence_barrier_init();
+        tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v);
+    }
+    pdl_wait();
+    const long long total = kv8_count<Units>(a.d, sums);
+    const long long begin = kv8_range(total, gridDim.x, blockIdx.x), end = kv8_range(total, gridDim.x, blockIdx.x + 1);
+    pdl_launch_dependents();
+    if (begin >= end) return;
+    if (warp == 2) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const TcWait wait{&gave_up, a.err};
+    Units u = kv8_find<Units>(a.d, sums, begin);
+    const int P = a.d.p.page, group = a.d.group;
+
+    if (warp == 0) {
+        // ---- codes: a box per page (64 positions of it at most) ----
+        const int rows = min(P, 64), boxes = BN / rows;
+        int st = 0, seq = 0;
+        uint32_t ph = 1;
+        for (long long step = begin; step < end;) {
+            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first), n = (t1 - t0) * boxes;
+            for (int base = 0; base < n; base += 32) {
+                int row = a.d.p.pages * a.d.p.kv_heads * P;                  // behind the pool: zeros come
+                float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);
+                if (base + lane < n) {
+                    const int pos = t0 * BN + (base + lane) * rows, page = pos < u.q.len ? kv8_page(a.d.s, a.d.p, u.b, pos / P) : -1;
+                    if (page >= 0) {
+                        row = (page * a.d.p.kv_heads + u.head) * P + pos % P;
+                        const float2 kv = *reinterpret_cast<const float2*>(a.d.p.scales + ((size_t)page * a.d.p.kv_heads + u.head) * 2);
+                        const float vs = fmaxf(kv.y, 0x1p-120f);
+                        sc = make_float4(kv.x, log2f(vs), __frcp_rn(vs), 1.f);
+                    }
+                }
+                for (int i = base; i < min(n, base + 32); i += boxes, ++seq) {
+                    for (int half = 0; half < 2; ++half) {
+                        wait(&raw_empty[st], ph);
+                        if (half == 0) {
+                            const int from = (i - base + (lane & 7) * 16 / rows) & 31;
+                            float4 m;
+                            m.x = __shfl_sync(0xffffffffu, sc.x, from); m.y = __shfl_sync(0xffffffffu, sc.y, from);
+                            m.z = __shfl_sync(0xffffffffu, sc.z, from); m.w = __shfl_sync(0xffffffffu, sc.w, from);
+                            if (lane < BN / 16) meta[seq % METAS][lane] = m;
+                        }
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive_expect_tx(&raw_full[st], C::RAW);
+                        __syncwarp();
+                        const int r = __shfl_sync(0xffffffffu, row, (i - base + lane) & 31);
+                        if (lane < boxes)
+#pragma unroll
+                            for (int pl = 0; pl < (D + 127) / 128; ++pl) tma_load_2d(codes + st * C::RAW + lane * rows * D, half ? &map_v : &map_k, &raw_full[st], pl * 128, r);
+                        if (++st == NR) { st = 0; ph ^= 1; }
+                    }
+                }
+            }
+            step = u.first + t1;
+            if (step < end && !u.next(a.d)) break;
+        }
+    } else if (warp == 1) {
+        // ---- MMAs ----
+        constexpr uint32_t id_s = make_idesc_f16(128, BN), id_o = make_idesc_f16(128, D) | (1u << 16);      // (B of P V: MN-major)
+        int st = 0, part = 0;
+        uint32_t ph = 0, p_ph = 0;
+        auto scores = [&](int w) {                           // of tile w, with the keys of slot st
+            if (elect_one()) {
+                const uint64_t qd = make_smem_desc_sw128(smem_u32(sm + w * C::Q_TILE)), kd = make_smem_desc_sw128(smem_u32(ring + st * C::SLOT));
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    umma_bf16(tmem + C::C_S + w * BN, qd + (uint64_t)((k >> 2) * 1024 + 2 * (k & 3)), kd + (uint64_t)((k >> 2) * 1024 + 2 * (k & 3)), id_s, (uint32_t)(k != 0));
+                umma_commit(&s_full[w]);
+            }
+            __syncwarp();
+        };
+        auto output = [&](int w, int slot, bool first, bool last) {
+            if (elect_one()) {
+                const uint64_t vd = make_smem_desc_mn128(smem_u32(ring + slot * C::SLOT), BN * 128);
+#pragma unroll
+                for (int k = 0; k < BN / 16; ++k)
+                    umma_ts(tmem + w * D, tmem + C::C_S + (uint32_t)(w * BN + (k >> 1) * 32 + (k & 1) * 8), vd + (uint64_t)(k * 128), id_o, (uint32_t)!(first && k == 0));
+                if (last) umma_commit(&o_done[w]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](int slot) { if (elect_one()) umma_commit(&empty[slot]); __syncwarp(); };
+        auto step_on = [&]() { if (++st == NF) { st = 0; ph ^= 1; } };
+        for (long long step = begin; step < end; ++part) {
+            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            wait(&full[st], ph);
+            for (int w = 0; w < 2; ++w) {
+                wait(&q_full[w], part & 1);
+                tc_fence_after();
+                scores(w);
+            }
+            release(st);
+            step_on();
+            for (int t = t0; t < t1; ++t) {
+                const bool last = t + 1 == t1;
+                const int v = st;
+                wait(&full[v], ph);
+                step_on();
+                for (int w = 0; w < 2; ++w) {
+                    wait(&p_full[w], p_ph);
+                    tc_fence_after();
+                    output(w, v, t == t0, last);
+                    if (w == 1) release(v);
+                    if (!last) {
+                        if (w == 0) wait(&full[st], ph);
+                        tc_fence_after();
+                        scores(w);
+                    }
+                }
+                p_ph ^= 1;
+                if (!last) { release(st); step_on(); }
+            }
+            step = u.first + t1;
+            if (step < end && !u.next(a.d)) break;
+        }
+    } else if (warp >= 12) {
+        // ---- codes to operands ----
+        const int ct = tid - 384;
+        int rs = 0, fs = 0, seq = 0, part = 0;
+        uint32_t r_ph = 0, f_ph = 1;
+        for (long long step = begin; step < end; ++part) {
+            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            const int seen = u.q.first + (int)((long long)u.grp * M / group);      // last position that all rows see
+            for (int t = t0; t < t1; ++t, ++seq) {
+                const bool edge = t * BN + BN - 1 > seen;
+                for (int half = 0; half < 2; ++half) {
+                    wait(&raw_full[rs], r_ph);
+                    wait(&empty[fs], f_ph);
+                    const uint8_t* src = codes + rs * C::RAW;
+                    uint8_t* dst = ring + fs * C::SLOT;
+                    bool there = true;
+#pragma unroll
+                    for (int i = 0; i < BN / 16; ++i) there = there && meta[seq % METAS][i].w != 0.f;
+                    const bool clean = half && (edge || !there);             // values that some row does not see: nothing of them may reach it
+#pragma unroll 4
+                    for (int e = 0; e < D / 16; ++e) {
+                        const int at = e * 128 + ct, row = at / (D / 16), j = at % (D / 16);
+                        uint4 c = *reinterpret_cast<const uint4*>(src + at * 16);
+                        if (clean) {
+                            const int pos = t * BN + row;
+                            if (pos >= u.q.len || meta[seq % METAS][row / 16].w == 0.f) c = make_uint4(0, 0, 0, 0);
+                            else if (pos > seen && (has_nan(c.x) || has_nan(c.y) || has_nan(c.z) || has_nan(c.w))) {
+                                c.x = without_nan(c.x); c.y = without_nan(c.y); c.z = without_nan(c.z); c.w = without_nan(c.w);
+                                nan_part[part % METAS] = part;                          // (the rows that do see it look for it themselves)
+                            }
+                        }
+                        const uint4 lo = make_uint4(half2_of(c.x, 0), half2_of(c.x, 1), half2_of(c.y, 0), half2_of(c.y, 1));
+                        const uint4 hi = make_uint4(half2_of(c.z, 0), half2_of(c.z, 1), half2_of(c.w, 0), half2_of(c.w, 1));
+                        uint8_t* p = dst + (j >> 2) * (BN * 128);
+                        // (lanes of the second 64 columns store their halves the other way round: no two lanes of a store share banks)
+                        const int swap = j >> 2;
+                        *reinterpret_cast<uint4*>(p + sw128_off(row, (j & 3) * 2 + swap)) = swap ? hi : lo;
+                        *reinterpret_cast<uint4*>(p + sw128_off(row, (j & 3) * 2 + (swap ^ 1))) = swap ? lo : hi;
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) { mbar_arrive(&full[fs]); mbar_arrive(&raw_empty[rs]); }
+                    if (++rs == NR) { rs = 0; r_ph ^= 1; }
+                    if (++fs == NF) { fs = 0; f_ph ^= 1; }
+                }
+            }
+            step = u.first + t1;
+            if (step < end && !u.next(a.d)) break;
+        }
+    } else if (warp >= 4) {
+        // ---- softmax and results: a row a thread ----
+        const int w = (warp - 4) >> 2, qd = warp & 3, r = w * 128 + qd * 32 + lane;
+        const uint32_t lanes = (uint32_t)(qd * 32) << 16;
+        const uint32_t sa = tmem + lanes + C::C_S + w * BN, oa = tmem + lanes + w * D;
+        int seq = 0, part = 0;
+        uint32_t s_ph = 0;
+        for (long long step = begin; step < end; ++part) {
+            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            // ---- the queries of this warp's rows, D / 8 lanes a row: f16, each row's largest moved to [2^14, 2^15) by a power of two ----
+            constexpr int LR = D / 8, RW = 32 / LR;          // lanes a row, rows at a time
+#pragma unroll 4
+            for (int i = 0; i < 32 / RW; ++i) {
+                const int rr = w * 128 + qd * 32 + i * RW + lane / LR, c = lane % LR;
+                const long long row = (long long)u.grp * M + rr;
+                const int tok = (int)(row / group), h = u.head * group + (int)(row % group);
+                uint32_t v[4] = {0, 0, 0, 0};
+                if (tok < u.q.n) {
+                    const T* src = reinterpret_cast<const T*>(a.q) + (long long)(u.q.s0 + tok) * a.ldq + (long long)h * a.ldqh + c * 8;
+                    if constexpr (VEC) { const uint4 x = __ldg(reinterpret_cast<const uint4*>(src)); v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+                    else {
+                        const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) v[k] = __ldg(s + 2 * k) | (uint32_t)__ldg(s + 2 * k + 1) << 16;
+                    }
+                }
+                float x[8], top = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) pair<T>(v[k], x[2 * k], x[2 * k + 1]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) top = x[k] != x[k] ? INFINITY : fmaxf(top, fabsf(x[k]));
+#pragma unroll
+                for (int o = 1; o < LR; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const uint32_t ex = __float_as_uint(fmaxf(top, 0x1p-100f)) >> 23;
+                const float up = top < INFINITY ? a.sign * __uint_as_float((268 - ex) << 23) : NAN;      // (a row with an infinity or a NaN gives NaN)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = pack_f16(x[2 * k] * up, x[2 * k + 1] * up);
+                const int ri = rr & 127;
+                *reinterpret_cast<uint4*>(sm + w * C::Q_TILE + (c >> 3) * 16384 + sw128_off(ri, c & 7)) = make_uint4(v[0], v[1], v[2], v[3]);
+                if (c == 0) factor_s[rr] = fmaxf(a.scale2 * __uint_as_float((ex - 14) << 23), 0x1p-120f);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[w]);
+            const float factor = factor_s[r];
+            const long long row = (long long)u.grp * M + r;
+            const int tok = (int)(row / group), h = u.head * group + (int)(row % group);
+            const bool in = tok < u.q.n;
+            const int pmax = in ? u.q.first + tok : INT_MAX;                 // last position that the row sees
+            const int wmin = __reduce_min_sync(0xffffffffu, pmax);
+            float m = -INFINITY, l = 0.f;                                    // reference of the exponents (a whole number, not always the running maximum), sum
+            for (int t = t0; t < t1; ++t, ++seq) {
+                const float4* mt = meta[seq % METAS];
+                wait(&s_full[w], s_ph);
+                s_ph ^= 1;
+                tc_fence_after();
+                const int kv0 = t * BN;
+                bool there = true;
+#pragma unroll
+                for (int i = 0; i < BN / 16; ++i) there = there && mt[i].w != 0.f;
+                if (kv0 + BN - 1 > wmin || !there) {                         // in place, for the code's size
+#pragma unroll 1
+                    for (int c = 0; c < BN; c += 16) {
+                        uint32_t x[16];
+                        tmem_ld16_async(sa + c, x);
+                        const bool page = mt[c / 16].w != 0.f;
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) if (!page || kv0 + c + j > pmax) x[j] = 0xff800000u;
+                        tmem_st16(sa + c, x);
+                    }
+                    tmem_st_wait();
+                }
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c0 = 0; c0 < BN; c0 += 64) {
+                    uint32_t x[64];
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16) tmem_ld16_async(sa + c0 + c, x + c);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 64; c += 16) {
+                        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) y[j & 3] = fmaxf(y[j & 3], __uint_as_float(x[c + j]));
+                        const float4 sc = mt[(c0 + c) / 16];
+                        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(factor * sc.x, 0x1p-126f), sc.y));
+                    }
+                }
+                const bool grow = mx > m + 8.f || (m == -INFINITY && mx > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float mn = fmaxf(m, ceilf(mx)), f = m == -INFINITY ? 0.f : m == mn ? 1.f : ex2(m - mn);
+                    l *= f;
+                    m = mn;
+                    if (t > t0) {                                            // (the scores are there: the MMAs ahead of theirs, the last step's output among them, are done)
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16_async(oa + c, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            tmem_st16(oa + c, o);
+                        }
+                    }
+                }
+                // scores whose last bit is worth more than a weight: their exponents are differences of rounded numbers
+                const bool far = __any_sync(0xffffffffu, fabsf(m) > 0x1p20f && fabsf(m) < INFINITY);
+                if (far) {
+#pragma unroll 1
+                    for (int c = 0; c < BN; c += 16) {
+                        uint32_t x[16];
+                        tmem_ld16_async(sa + c, x);
+                        tmem_ld_wait();
+                        const float4 sc = mt[c / 16];
+                        const float f = fmaxf(factor * sc.x, 0x1p-126f);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(fmaf(__uint_as_float(x[j]), f, sc.y) - (m == -INFINITY ? 0.f : m));
+                        tmem_st16(sa + c, x);
+                    }
+                    tmem_st_wait();
+                }
+                const float ref = (m == -INFINITY ? 0.f : m) - P_SHIFT;
+#pragma unroll 1
+                for (int c0 = 0; c0 < BN; c0 += 32) {
+                    uint32_t x[32], p[16];
+                    tmem_ld16_async(sa + c0, x);
+                    tmem_ld16_async(sa + c0 + 16, x + 16);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; c += 16) {
+                        const float4 sc = mt[(c0 + c) / 16];
+                        const float f = far ? 1.f : fmaxf(factor * sc.x, 0x1p-126f), b = far ? P_SHIFT : sc.y - ref;
+                        float sum[2] = {0.f, 0.f};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float p0 = ex2(fmaf(__uint_as_float(x[c + 2 * j]), f, b)), p1 = ex2(fmaf(__uint_as_float(x[c + 2 * j + 1]), f, b));
+                            sum[0] += p0; sum[1] += p1;
+                            p[c / 2 + j] = pack_f16(p0, p1);
+                        }
+                        l = fmaf(sum[0] + sum[1], sc.z, l);
+                    }
+                    tmem_st16(sa + c0, p);                                   // in place of the 32 scores
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[w]);
+            }
+            wait(&o_done[w], part & 1);
+            tc_fence_after();
+            // a NaN among values that only some rows see was left out of the products: the rows that see it look it up
+            uint32_t odd[D / 32];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) odd[i] = 0;
+            if (nan_part[part % METAS] == part && in) {
+                const int from = max(u.q.first + (int)((long long)u.grp * M / group) + 1, t0 * BN), to = min(min(pmax, u.q.len - 1), t1 * BN - 1);
+                for (int pos = max(from, 0); pos <= to; ++pos) {
+                    const int page = kv8_page(a.d.s, a.d.p, u.b, pos / P);
+                    if (page < 0) continue;
+                    const unsigned char* v = a.d.p.v + (((size_t)page * a.d.p.kv_heads + u.head) * P + pos % P) * D;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        for (int j = 0; j < 32; ++j) if ((v[i * 32 + j] & 0x7f) == 0x7f) odd[i] |= 1u << j;
+                }
+            }
+            const bool whole = t0 == 0 && t1 == u.tiles;
+            const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            T* dst = reinterpret_cast<T*>(a.out) + (long long)(u.q.s0 + (in ? tok : 0)) * a.ldo + (long long)h * a.ldoh;
+            float* part_dst = a.work + ((size_t)kv8_slot(blockIdx.x, begin, step) * M + r) * (D + 2);
+#pragma unroll
+            for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                tmem_ld16_async(oa + c, o);
+                tmem_ld_wait();
+                float y[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    y[j] = __uint_as_float(o[j]) * inv;
+                    if (odd[c / 32] >> (c % 32 + j) & 1) y[j] = NAN;
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) *reinterpret_cast<float2*>(part_dst + c + j) = make_float2(y[j], y[j + 1]);
+                } else if (in) {
+                    uint32_t k[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) k[j] = pack<T>(y[2 * j], y[2 * j + 1]);
+                    if constexpr (VEC) {
+                        *reinterpret_cast<uint4*>(dst + c) = make_uint4(k[0], k[1], k[2], k[3]);
+                        *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(k[4], k[5], k[6], k[7]);
+                    } else {
+                        unsigned short* s = reinterpret_cast<unsigned short*>(dst + c);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) { s[2 * j] = (unsigned short)k[j]; s[2 * j + 1] = (unsigned short)(k[j] >> 16); }
+                    }
+                }
+            }
+            if (!whole) { part_dst[D] = m; part_dst[D + 1] = l; }
+            tc_fence_before();
+            step = u.first + t1;
+            if (step < end && !u.next(a.d)) break;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+    if (tid == 0) wait.drain();
+}
+
+template <int D, typename T>
+int launch(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, bool vec, bool pdl) {
+    static SmemOptIn seen[2];
+    auto kernel = vec ? flash_kernel<D, T, true> : flash_kernel<D, T, false>;
+    if (const int e = ensure_dyn_smem(kernel, (size_t)Cfg<D>::SMEM, seen[vec])) return e;
+    return launch_k(kernel, dim3(tc_device_sms()), dim3(THREADS), Cfg<D>::SMEM, st, pdl, mk, mv, a);
+}
+
+}  // namespace
+
+// Sequences that bring `lo` rows of a kv head and more; parts of units that lie with several CTAs are left in a.work
+int kv8_flash_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Deal& d, bool pdl) {
+    const int D = d.p.dim;
+    const uint64_t n = (uint64_t)d.p.pages * d.p.kv_heads * d.p.page;
+    CUtensorMap mk, mv;
+    const uint32_t rows = d.p.page < 64 ? d.p.page : 64;
+    if (!tc_tmap(&mk, d.p.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, D, D, rows, D, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !tc_tmap(&mv, d.p.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, D, D, rows, D, CU_TENSOR_MAP_SWIZZLE_NONE)) return (int)cudaErrorInvalidValue;
+    const bool vec = (reinterpret_cast<uintptr_t>(k.q.p) | reinterpret_cast<uintptr_t>(k.out)) % 16 == 0 && (k.q.ld | k.q.ldh | k.ldo | k.ldoh) % 8 == 0;
+    const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)(fabs((double)k.scale) * 1.4426950408889634074), k.scale < 0.f ? -1.f : 1.f, d,
+                    reinterpret_cast<float*>(k.work), k.err};
+    if (k.q.type == KV8_BF16) return D == 64 ? launch<64, bf16>(st, mk, mv, a, vec, pdl) : launch<128, bf16>(st, mk, mv, a, vec, pdl);
+    return D == 64 ? launch<64, __half>(st, mk, mv, a, vec, pdl) : launch<128, __half>(st, mk, mv, a, vec, pdl);
+}
+
+}  // namespace cb

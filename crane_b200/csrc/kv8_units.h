@@ -54,44 +54,58 @@ CB_HD Kv8Piece kv8_piece(const Kv8Seqs& s, const Kv8Seq& q, int page, int b, int
 }
 
 // ---- attention: how the steps are dealt out ----------------------------------------------------------------------------------------
-// A unit is a sequence, a kv head and a group of M rows of its queries (row = token * group + head of the group); its steps are the tiles of TILE positions, one at least.  All
-// steps, unit after unit, are dealt out evenly to the CTAs, whatever the lengths: a unit may lie with several CTAs, which then leave their parts of the sums to be joined.
+// A unit is a sequence, a kv head and a group of M rows of its queries (row = token * group + head of the group); its steps are the tiles of TILE positions that the group's last
+// row sees, one at least.  All steps, unit after unit, are dealt out evenly to the CTAs, whatever the lengths: a unit may lie with several CTAs, which then leave their parts of
+// the sums to be joined.  A kernel takes the sequences that bring from `lo` to `hi` rows.
+struct Kv8Deal { Kv8Seqs s; Kv8Pool p; int group; long long lo, hi; };
 template <int M, int TILE>
 struct Kv8Units {
     int b, head, grp;                          // the unit
     Kv8Seq q;
-    int tiles, groups;
+    int tiles, groups;                         // its tiles, the sequence's groups
     long long first;                           // number of its first step
-    CB_HD void shape(const Kv8Seqs& s, const Kv8Pool& p, int group) {
-        q = kv8_seq(s, b);
-        groups = (int)(((long long)q.n * group + M - 1) / M);
-        tiles = most(1, (int)((least((long long)q.len, (long long)s.width * p.page) + TILE - 1) / TILE));
+    CB_HD void shape(const Kv8Deal& d) {
+        q = kv8_seq(d.s, b);
+        const long long rows = (long long)q.n * d.group;
+        groups = rows < d.lo || rows > d.hi ? 0 : (int)((rows + M - 1) / M);
     }
-    CB_HD long long steps(const Kv8Pool& p) const { return (long long)groups * p.kv_heads * tiles; }
-    CB_HD bool next(const Kv8Seqs& s, const Kv8Pool& p, int group) {           // false: behind the last
+    CB_HD int tiles_of(const Kv8Deal& d, int g) const {
+        const long long last = least((long long)q.n, (((long long)g + 1) * M - 1) / d.group + 1);      // tokens up to the group's last
+        const long long seen = least(q.first + last, (long long)d.s.width * d.p.page);
+        return most(1, (int)((seen + TILE - 1) / TILE));
+    }
+    CB_HD long long head_steps(const Kv8Deal& d) const {
+        long long n = 0;
+        for (int g = 0; g < groups; ++g) n += tiles_of(d, g);
+        return n;
+    }
+    CB_HD bool next(const Kv8Deal& d) {        // false: behind the last
         first += tiles;
-        if (++grp < groups) return true;
-        grp = 0;
-        if (++head < p.kv_heads) return true;
-        head = 0;
-        do {
-            if (++b >= s.seqs) return false;
-            shape(s, p, group);
-        } while (!groups);
+        if (++grp >= groups) {
+            grp = 0;
+            if (++head >= d.p.kv_heads) {
+                head = 0;
+                do {
+                    if (++b >= d.s.seqs) return false;
+                    shape(d);
+                } while (!groups);
+            }
+        }
+        tiles = tiles_of(d, grp);
         return true;
     }
-    // The unit that holds a step; sequences are counted off from b on, which begins with step `at`
-    CB_HD void seek(const Kv8Seqs& s, const Kv8Pool& p, int group, int from, long long at, long long step) {
+    // The unit that holds a step; sequences are counted off from `from` on, which begins with step `at`
+    CB_HD void seek(const Kv8Deal& d, int from, long long at, long long step) {
+        long long each;
         for (b = from;; ++b) {
-            shape(s, p, group);
-            const long long c = steps(p);
-            if (step < at + c || b + 1 >= s.seqs) break;
-            at += c;
+            shape(d);
+            each = head_steps(d);
+            if (step < at + each * d.p.kv_heads || b + 1 >= d.s.seqs) break;
+            at += each * d.p.kv_heads;
         }
-        const long long k = (step - at) / tiles;
-        head = (int)(k / most(groups, 1));
-        grp = (int)(k - (long long)head * groups);
-        first = at + k * tiles;
+        head = (int)((step - at) / most(each, 1LL));
+        first = at + head * each;
+        for (grp = 0; tiles = tiles_of(d, grp), first + tiles <= step && grp + 1 < groups; ++grp) first += tiles;
     }
 };
 CB_HD long long kv8_range(long long total, int ctas, int c) { return total / ctas * c + least((long long)c, total % ctas); }       // a CTA's first step

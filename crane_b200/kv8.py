@@ -99,7 +99,7 @@ def attention(q, cache, table, lens, starts, *, scale: float = None, max_rows: i
     op, ldo, ldoh = _rows("out", out, dev, rows, heads, dim, q.dtype)
     stream = _raw_stream(dev)
     need = C.c_size_t()
-    rc = _entry("kv8_attention_bytes")(dev, heads, c[4], dim, seqs, rows, max_rows, C.byref(need))
+    rc = _entry("kv8_attention_bytes")(dev, _DTYPES[q.dtype], heads, c[4], dim, seqs, rows, max_rows, C.byref(need))
     if rc:
         _failed(rc)
     work = torch.empty(need.value, dtype=torch.uint8, device=q.device)

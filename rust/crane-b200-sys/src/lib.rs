@@ -123,7 +123,7 @@ extern "C" {
     pub fn crane_b200_fp8_status(device: c_int, stream: *mut c_void) -> c_int;
     pub fn crane_b200_device_last_error() -> *const c_char;
     pub fn crane_b200_kv8_append(device: c_int, k: *const c_void, ldk: usize, ldkh: usize, v: *const c_void, ldv: usize, ldvh: usize, dtype: c_int, k_codes: *mut u8, v_codes: *mut u8, scales: *mut f32, pages: usize, kv_heads: usize, page: usize, dim: usize, table: *const i32, ldt: usize, width: usize, lens: *const i32, starts: *const i32, seqs: usize, rows: usize, stream: *mut c_void) -> c_int;
-    pub fn crane_b200_kv8_attention_bytes(device: c_int, heads: usize, kv_heads: usize, dim: usize, seqs: usize, rows: usize, max_rows: usize, bytes: *mut usize) -> c_int;
+    pub fn crane_b200_kv8_attention_bytes(device: c_int, dtype: c_int, heads: usize, kv_heads: usize, dim: usize, seqs: usize, rows: usize, max_rows: usize, bytes: *mut usize) -> c_int;
     pub fn crane_b200_kv8_attention(device: c_int, q: *const c_void, ldq: usize, ldqh: usize, out: *mut c_void, ldo: usize, ldoh: usize, dtype: c_int, heads: usize, scale: f32, k_codes: *const u8, v_codes: *const u8, scales: *const f32, pages: usize, kv_heads: usize, page: usize, dim: usize, table: *const i32, ldt: usize, width: usize, lens: *const i32, starts: *const i32, seqs: usize, rows: usize, max_rows: usize, work: *mut c_void, work_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn crane_b200_lora_linear(device: c_int, x: *const c_void, ldx: usize, dtype: c_int, a: *const c_void, b: *const c_void, w_dtype: c_int, adapters: usize, rank: usize, which: *const i32, scales: *const f32, add: *const c_void, ldadd: usize, out: *mut c_void, ldo: usize, m: usize, n: usize, k: usize, stream: *mut c_void) -> c_int;
     pub fn crane_b200_draft_verify_bytes(device: c_int, vocab: usize, seqs: usize, drafts: usize, with_draft_logits: c_int, bytes: *mut usize) -> c_int;

@@ -68,12 +68,19 @@ static void pieces(const Case& c, bool wild) {
 }
 
 template <int M, int TILE>
-static void units(const Case& c, int group, int ctas) {
+static void units(const Case& c, int group, int ctas, long long lo, long long hi) {
     using U = Kv8Units<M, TILE>;
+    const Kv8Deal d = {c.s, c.p, group, lo, hi};
     long long total = 0;
-    for (int b = 0; b < c.s.seqs; ++b) { U u; u.b = b; u.shape(c.s, c.p, group); CHECK(u.tiles >= 1 && u.groups >= 0); total += u.steps(c.p); }
+    for (int b = 0; b < c.s.seqs; ++b) {
+        U u; u.b = b; u.shape(d);
+        CHECK(u.groups >= 0 && (long long)u.groups * M < (long long)u.q.n * group + M);
+        CHECK(!u.groups == (u.q.n == 0 || (long long)u.q.n * group < lo || (long long)u.q.n * group > hi));
+        total += u.head_steps(d) * c.p.kv_heads;
+    }
     if (total > 2000000) return;
     std::map<std::tuple<int, int, int>, std::vector<std::pair<int, std::pair<int, int>>>> parts;      // unit -> (slot, tiles), in order; slot -1: whole
+    std::map<std::tuple<int, int, int>, int> tiles;
     long long next = 0;
     std::set<int> slots;
     for (int k = 0; k < ctas; ++k) {
@@ -83,16 +90,21 @@ static void units(const Case& c, int group, int ctas) {
         if (begin == end) continue;
         CHECK(kv8_owner(total, ctas, begin) == k && kv8_owner(total, ctas, end - 1) == k);
         U u;
-        u.seek(c.s, c.p, group, 0, 0, begin);
+        u.seek(d, 0, 0, begin);
         for (long long step = begin; step < end;) {
             CHECK(u.first <= step && step < u.first + u.tiles && u.head >= 0 && u.head < c.p.kv_heads && u.grp >= 0 && u.grp < u.groups && u.b < c.s.seqs);
+            CHECK(u.tiles >= 1 && (long long)(u.tiles - 1) * TILE < (long long)c.s.width * c.p.page);
+            const long long row = least((long long)u.q.n * group, (u.grp + 1LL) * M) - 1;            // the group's last row and what it sees
+            const long long seen = least((long long)u.q.first + row / group + 1, (long long)c.s.width * c.p.page);
+            CHECK((long long)u.tiles * TILE >= seen && ((long long)(u.tiles - 1) * TILE < seen || u.tiles == 1));
             const int t0 = (int)(step - u.first), t1 = (int)least((long long)u.tiles, end - u.first);
             const bool whole = t0 == 0 && t1 == u.tiles;
             const int slot = whole ? -1 : kv8_slot(k, begin, step);
             if (!whole) CHECK(slot < 2 * ctas && slots.insert(slot).second);
             parts[{u.b, u.head, u.grp}].push_back({slot, {t0, t1}});
+            tiles[{u.b, u.head, u.grp}] = u.tiles;
             step = u.first + t1;
-            if (step < end) CHECK(u.next(c.s, c.p, group));
+            if (step < end) CHECK(u.next(d));
         }
     }
     CHECK(next == total);
@@ -102,7 +114,7 @@ static void units(const Case& c, int group, int ctas) {
         const long long begin = kv8_range(total, ctas, k), end = kv8_range(total, ctas, k + 1);
         if (begin >= end || end >= total) continue;
         U u;
-        u.seek(c.s, c.p, group, 0, 0, end - 1);
+        u.seek(d, 0, 0, end - 1);
         if (u.first + u.tiles <= end || u.first < begin) continue;
         const auto& p = parts.at({u.b, u.head, u.grp});
         const int last = kv8_owner(total, ctas, u.first + u.tiles - 1);
@@ -113,9 +125,13 @@ static void units(const Case& c, int group, int ctas) {
     for (const auto& e : parts) {
         int at = 0;
         for (const auto& p : e.second) { CHECK(p.second.first == at); at = p.second.second; }
+        CHECK(at == tiles.at(e.first));
         CHECK((e.second.size() > 1) == (joined.count(e.first) == 1));
         if (e.second.size() == 1) CHECK(e.second[0].first == -1);
     }
+    size_t want = 0;
+    for (int b = 0; b < c.s.seqs; ++b) { U u; u.b = b; u.shape(d); want += (size_t)u.groups * c.p.kv_heads; }
+    CHECK(parts.size() == want);                                    // every unit once
 }
 
 int main() {
@@ -125,9 +141,12 @@ int main() {
         pieces(tame, false);
         pieces(wild, true);
         for (int ctas : {1, 3, 148, 296}) {
-            units<16, 64>(tame, 1 + i % 7, ctas);
-            units<64, 64>(tame, 1 + i % 7, ctas);
-            units<16, 64>(wild, 1 + i % 7, ctas);
+            const int group = 1 + i % 7;
+            units<16, 64>(tame, group, ctas, 0, 1LL << 62);
+            units<16, 64>(tame, group, ctas, 0, 64);
+            units<64, 64>(wild, group, ctas, 0, 1LL << 62);
+            units<256, 128>(tame, group, ctas, 65, 1LL << 62);
+            units<256, 128>(wild, group, ctas, 65, 1LL << 62);
         }
     }
     std::puts("ok");

@@ -73,8 +73,8 @@ def test_attention_is_refused_by_its_numbers(change, said):
 def test_sizes_of_workspaces_are_refused():
     n = C.c_size_t()
     for heads, kv, dim, p in ((3, 2, 128, n), (4, 0, 128, n), (4, 2, 100, n)):
-        assert lib().crane_b200_kv8_attention_bytes(0, heads, kv, dim, 1, 1, 0, C.byref(p)) in (crane_b200.INVALID_ARG, crane_b200.UNSUPPORTED)
-    assert lib().crane_b200_kv8_attention_bytes(0, 4, 2, 128, 1, 1, 0, None) == crane_b200.INVALID_ARG
+        assert lib().crane_b200_kv8_attention_bytes(0, 1, heads, kv, dim, 1, 1, 0, C.byref(p)) in (crane_b200.INVALID_ARG, crane_b200.UNSUPPORTED)
+    assert lib().crane_b200_kv8_attention_bytes(0, 1, 4, 2, 128, 1, 1, 0, None) == crane_b200.INVALID_ARG
 
 
 def test_tensors_are_refused():
