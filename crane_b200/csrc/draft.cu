@@ -17,10 +17,10 @@
 namespace cb {
 namespace {
 
-constexpr int THREADS = 256, CLUSTER = 8;
+constexpr int THREADS = 256, RACERS = 512, CLUSTER = 8;
 constexpr double LOG2E = 1.4426950408889634;
 
-struct Part { float top; int at; double sum; };         // of a stretch: its largest logit, the first place of it, the sum of exp((x - top) / T)
+struct Part { float top; int at; double sum; };         // of a stretch: its largest logit; greedy: the first place of it; else the sum of exp((x - top) / T)
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 template <typename T> __device__ __forceinline__ float to_f(T v);
@@ -48,22 +48,42 @@ __device__ __forceinline__ int start_of(const Draft& d, int b) { return min(max(
 
 __host__ __device__ __forceinline__ int stretch_of(int vocab, int parts) { return ((vocab + parts - 1) / parts + 7) / 8 * 8; }
 
-// f(i, x) for i in [lo, hi), 16 bytes at a time where the row's address allows
-template <typename T, typename F>
-__device__ __forceinline__ void each(const T* row, int lo, int hi, F f) {
-    constexpr int N = 16 / (int)sizeof(T);
-    const int skew = (int)(reinterpret_cast<uintptr_t>(row + lo) % 16) / (int)sizeof(T);
-    const int a = min(hi, lo + (skew ? N - skew : 0)), b = a + (hi - a) / N * N;
-    for (int i = lo + threadIdx.x; i < a; i += THREADS) f(i, clean(to_f<T>(row[i])));
-#pragma unroll 4
-    for (int i = a + threadIdx.x * N; i < b; i += THREADS * N) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + i));
+// N neighbouring values, 16 bytes (f32: 4, else 8) or one
+template <typename T, int N> __device__ __forceinline__ void get(const T* p, float* x) {
+    if constexpr (N == 1) x[0] = clean(to_f<T>(*p));
+    else {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
         const T* e = reinterpret_cast<const T*>(&v);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f(i + j, clean(to_f<T>(e[j])));
+        for (int j = 0; j < N; ++j) x[j] = clean(to_f<T>(e[j]));
     }
-    for (int i = b + threadIdx.x; i < hi; i += THREADS) f(i, clean(to_f<T>(row[i])));
 }
+// A running maximum and the sum of exp2((x - top) c) below it, B values at a time
+struct Sum {
+    float top = -INFINITY, s[2] = {0.f, 0.f};
+    template <int B> __device__ __forceinline__ void take(const float* x, float c) {
+        float m = x[0];
+#pragma unroll
+        for (int j = 1; j < B; ++j) m = fmaxf(m, x[j]);
+        if (m > top) {
+            const float f = top == -INFINITY ? 0.f : ex2((top - m) * c);
+            s[0] *= f; s[1] *= f;
+            top = m;
+        }
+        if (fabsf(top) < INFINITY) {
+#pragma unroll
+            for (int j = 0; j < B; ++j) s[j & 1] += ex2((x[j] - top) * c);
+        } else if (top > 0.f) {                         // +inf: those share
+#pragma unroll
+            for (int j = 0; j < B; ++j) s[0] += x[j] == top ? 1.f : 0.f;
+        }
+    }
+};
+struct First {                                          // a running maximum and its first place; values come in ascending order of their places
+    float top = -INFINITY;
+    int at = INT_MAX;
+    __device__ __forceinline__ void take(float x, int i) { if (x > top) { top = x; at = i; } }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
@@ -79,16 +99,39 @@ stretch_kernel(Draft d, int parts) {
     const T* x = reinterpret_cast<const T*>(target ? d.logits : d.q) + (long long)r * (target ? d.ld : d.ldq);
     const int len = stretch_of(d.vocab, parts), lo = (int)min((long long)d.vocab, (long long)part * len), hi = min(d.vocab, lo + len);
     const float c = temp > 0.f ? rate(temp) : 1.f;
-    float top = -INFINITY, sum = 0.f;
+    constexpr int N = 16 / (int)sizeof(T), U = 4;
+    const int skew = (int)(reinterpret_cast<uintptr_t>(x + lo) % 16) / (int)sizeof(T);
+    const int a0 = min(hi, lo + (skew ? N - skew : 0)), a1 = a0 + (hi - a0) / N * N;        // what 16-byte loads reach
+    float top, sum = 0.f;
     int at = INT_MAX;
-    each<T>(x, lo, hi, [&](int i, float v) {
-        if (v > top) {
-            sum = top == -INFINITY ? 0.f : sum * ex2((top - v) * c);
-            top = v;
-            at = i;
+    if (temp > 0.f) {
+        Sum z;
+        float v[U * N];
+        if (lo + (int)threadIdx.x < a0) { get<T, 1>(x + lo + threadIdx.x, v); z.take<1>(v, c); }
+        int i = a0 + threadIdx.x * N;
+        for (; i + (U - 1) * THREADS * N < a1; i += U * THREADS * N) {
+#pragma unroll
+            for (int k = 0; k < U; ++k) get<T, N>(x + i + k * THREADS * N, v + k * N);
+            z.take<U * N>(v, c);
         }
-        sum += v == -INFINITY ? 0.f : ex2(below(v, top) * c);
-    });
+        for (; i < a1; i += THREADS * N) { get<T, N>(x + i, v); z.take<N>(v, c); }
+        if (a1 + (int)threadIdx.x < hi) { get<T, 1>(x + a1 + threadIdx.x, v); z.take<1>(v, c); }
+        top = z.top;
+        sum = z.s[0] + z.s[1];
+    } else {
+        First z;
+        float v[N];
+        if (lo + (int)threadIdx.x < a0) { get<T, 1>(x + lo + threadIdx.x, v); z.take(v[0], lo + threadIdx.x); }
+#pragma unroll 4
+        for (int i = a0 + threadIdx.x * N; i < a1; i += THREADS * N) {
+            get<T, N>(x + i, v);
+#pragma unroll
+            for (int j = 0; j < N; ++j) z.take(v[j], i + j);
+        }
+        if (a1 + (int)threadIdx.x < hi) { get<T, 1>(x + a1 + threadIdx.x, v); z.take(v[0], a1 + threadIdx.x); }
+        top = z.top;
+        at = z.at;
+    }
     // ---- the block's ----
     __shared__ float wt[THREADS / 32];
     __shared__ int wa[THREADS / 32];
@@ -119,37 +162,34 @@ stretch_kernel(Draft d, int parts) {
 __device__ __forceinline__ Part whole(const Part* p, int parts, double inv_t) {
     const int lane = threadIdx.x & 31;
     Part r = {-INFINITY, INT_MAX, 0.0};
-    auto join = [&](const Part& q) {
-        const float m = fmaxf(r.top, q.top);
-        r.sum = (r.sum > 0.0 ? r.sum * exp((double)below(r.top, m) * inv_t) : 0.0) + (q.sum > 0.0 ? q.sum * exp((double)below(q.top, m) * inv_t) : 0.0);
-        r.at = r.top > q.top ? r.at : q.top > r.top ? q.at : min(r.at, q.at);
-        r.top = m;
-    };
-    for (int i = lane; i < parts; i += 32) join(p[i]);
+    for (int i = lane; i < parts; i += 32) { const float top = p[i].top; if (top > r.top) { r.top = top; r.at = p[i].at; } }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        Part q;
-        q.top = __shfl_xor_sync(0xffffffffu, r.top, o);
-        q.at = __shfl_xor_sync(0xffffffffu, r.at, o);
-        q.sum = __shfl_xor_sync(0xffffffffu, r.sum, o);
-        join(q);
+        const float top = __shfl_xor_sync(0xffffffffu, r.top, o);
+        const int at = __shfl_xor_sync(0xffffffffu, r.at, o);
+        r.at = r.top > top ? r.at : top > r.top ? at : min(r.at, at);
+        r.top = fmaxf(r.top, top);
     }
+    for (int i = lane; i < parts; i += 32) if (p[i].sum > 0.0) r.sum += p[i].sum * exp((double)below(p[i].top, r.top) * inv_t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) r.sum += __shfl_xor_sync(0xffffffffu, r.sum, o);
     return r;
 }
 __device__ __forceinline__ double share(float x, const Part& p, double inv_t) { return p.sum > 0.0 && x > -INFINITY ? exp((double)below(x, p.top) * inv_t) / p.sum : 0.0; }
 
 // A cluster for each sequence: the drafts, then the race
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(RACERS)
 race_kernel(Draft d, int parts) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ int first_s;
     __shared__ Part rows_s[2];
-    __shared__ double key_s[THREADS / 32];
-    __shared__ int at_s[THREADS / 32];
+    __shared__ double key_s[RACERS / 32];
+    __shared__ int at_s[RACERS / 32];
     __shared__ double best_s;
     __shared__ int best_at_s;
+    __shared__ float bar_s, bars_s[RACERS / 32];
     const int b = blockIdx.x / CLUSTER, rank = (int)cluster_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int s0 = start_of(d, b), n = max(start_of(d, b + 1), s0) - s0;
     const float temp = d.temperatures ? __ldg(d.temperatures + b) : 1.f;
@@ -160,7 +200,7 @@ race_kernel(Draft d, int parts) {
     const T* y0 = reinterpret_cast<const T*>(d.q) + (d.q ? (long long)s0 * d.ldq : 0);
     if (threadIdx.x == 0) first_s = n;
     __syncthreads();
-    for (int j = warp; j < n; j += THREADS / 32) {
+    for (int j = warp; j < n; j += RACERS / 32) {
         const Part p = whole(parts_p + (long long)(s0 + b + j) * parts, parts, inv_t);
         Part q = {};
         if (d.q && !greedy) q = whole(parts_p + (long long)(d.total + d.seqs + s0 + j) * parts, parts, inv_t);
@@ -196,22 +236,74 @@ race_kernel(Draft d, int parts) {
     const float* u = d.noise + (long long)b * d.ldn;
     const float c = rate(temp), pz = (float)(1.0 / p.sum), qz = q.sum > 0.0 ? (float)(1.0 / q.sum) : 0.f;
     const int len = stretch_of(d.vocab, CLUSTER), lo = (int)min((long long)d.vocab, (long long)rank * len), hi = min(d.vocab, lo + len);
+    constexpr int N = 16 / (int)sizeof(T);
+    const bool wide = ((reinterpret_cast<uintptr_t>(x + lo) | (y ? reinterpret_cast<uintptr_t>(y + lo) : 0) | reinterpret_cast<uintptr_t>(u + lo)) & 15) == 0;
     for (int pass = 0; pass < 2; ++pass) {              // the second only where p exceeds q nowhere: the race over p itself
-        // f32 tells which places cannot win (its p and q are 1e-5 of themselves off at most, a tenth of what is allowed for); the others' keys are computed in 64 bits
-        double best = 0.0;
-        float bar = 0.f;
-        int at = INT_MAX;
-        each<T>(x, lo, hi, [&](int i, float xv) {
-            if (xv == -INFINITY || (pass == 0 && i == sure)) return;
-            const float yv = y && pass == 0 ? clean(to_f<T>(y[i])) : -INFINITY;
-            const float pi = ex2(below(xv, p.top) * c) * pz, qi = yv == -INFINITY ? 0.f : ex2(below(yv, q.top) * c) * qz;
-            const float ui = fminf(fmaxf(__ldg(u + i), 0x1p-126f), 0x1.fffffep-1f), clock = -logf(ui);
-            if ((pi - qi) + 1e-4f * (pi + qi) <= bar * clock) return;
-            const double w = share(xv, p, inv_t) - (yv == -INFINITY ? 0.0 : share(yv, q, inv_t));
-            if (!(w > 0.0)) return;
-            const double key = w / -log((double)ui);
-            if (key > best || (key == best && i < at)) { best = key; at = i; bar = (float)best * 0.9999f; }
+        // f32 brackets every key (its p and q are 1e-5 of themselves off at most, a tenth of what is allowed for).  Places whose upper end stays below the best lower end of the
+        // whole row cannot win; the few others' keys are computed in 64 bits.
+        float low = 0.f, high = 0.f;                    // best lower and upper ends among this thread's places
+        auto bracket = [&](int i, float xv, float yv, float uv, float& lo_key, float& hi_key) {
+            const float pi = xv == -INFINITY || (pass == 0 && i == sure) ? 0.f : ex2(below(xv, p.top) * c) * pz, qi = yv == -INFINITY ? 0.f : ex2(below(yv, q.top) * c) * qz;
+            const float slack = 1e-4f * (pi + qi), inv = __fdividef(1.f, -logf(fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f)));
+            lo_key = (pi - qi - slack) * inv * 0.9999f;
+            hi_key = (pi - qi + slack) * inv * 1.0001f;
+        };
+        auto all = [&](auto&& f) {                      // f(i, x, y, u) over this thread's places
+            if (wide) {
+                const int end = lo + (hi - lo) / N * N;
+#pragma unroll 2
+                for (int i = lo + threadIdx.x * N; i < end; i += RACERS * N) {
+                    float xv[N], yv[N], uv[N];
+                    get<T, N>(x + i, xv);
+                    if (y && pass == 0) get<T, N>(y + i, yv);
+                    else {
+#pragma unroll
+                        for (int k = 0; k < N; ++k) yv[k] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int k = 0; k < N; k += 4) { const float4 v = __ldg(reinterpret_cast<const float4*>(u + i + k)); uv[k] = v.x; uv[k + 1] = v.y; uv[k + 2] = v.z; uv[k + 3] = v.w; }
+#pragma unroll
+                    for (int k = 0; k < N; ++k) f(i + k, xv[k], yv[k], uv[k]);
+                }
+                const int i = end + threadIdx.x;
+                if (i < hi) f(i, clean(to_f<T>(x[i])), y && pass == 0 ? clean(to_f<T>(y[i])) : -INFINITY, __ldg(u + i));
+            } else {
+#pragma unroll 4
+                for (int i = lo + threadIdx.x; i < hi; i += RACERS) f(i, clean(to_f<T>(x[i])), y && pass == 0 ? clean(to_f<T>(y[i])) : -INFINITY, __ldg(u + i));
+            }
+        };
+        all([&](int i, float xv, float yv, float uv) {
+            float a, z;
+            bracket(i, xv, yv, uv, a, z);
+            low = fmaxf(low, a);
+            high = fmaxf(high, z);
         });
+        float bar = warp_max(low);
+        if (lane == 0) bars_s[warp] = bar;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < RACERS / 32; ++w) bar = fmaxf(bar, bars_s[w]);
+            bar_s = bar;
+        }
+        cluster_sync_all();
+        bar = 0.f;
+        for (int r = 0; r < CLUSTER; ++r) {
+            float v;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_smem(&bar_s, r)) : "memory");
+            bar = fmaxf(bar, v);
+        }
+        double best = 0.0;
+        int at = INT_MAX;
+        if (high > 0.f && high >= bar)
+            all([&](int i, float xv, float yv, float uv) {
+                float a, z;
+                bracket(i, xv, yv, uv, a, z);
+                if (!(z > 0.f && z >= bar)) return;
+                const double w = share(xv, p, inv_t) - (yv == -INFINITY ? 0.0 : share(yv, q, inv_t));
+                if (!(w > 0.0)) return;
+                const double key = w / -log((double)fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f));
+                if (key > best || (key == best && i < at)) { best = key; at = i; }
+            });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double k2 = __shfl_xor_sync(0xffffffffu, best, o);
@@ -221,7 +313,7 @@ race_kernel(Draft d, int parts) {
         if (lane == 0) { key_s[warp] = best; at_s[warp] = at; }
         __syncthreads();
         if (threadIdx.x == 0) {
-            for (int w = 1; w < THREADS / 32; ++w)
+            for (int w = 1; w < RACERS / 32; ++w)
                 if (key_s[w] > best || (key_s[w] == best && at_s[w] < at)) { best = key_s[w]; at = at_s[w]; }
             best_s = best;
             best_at_s = at;
@@ -238,7 +330,7 @@ race_kernel(Draft d, int parts) {
         }
         cluster_sync_all();                             // (read: it may be written again, or its owner leave)
         if (best > 0.0 || pass == 1) {
-            if (rank == 0 && threadIdx.x == 0) { d.accepted[b] = j; d.next[b] = best > 0.0 ? at : p.at; }
+            if (rank == 0 && threadIdx.x == 0) { d.accepted[b] = j; d.next[b] = best > 0.0 ? at : -1; }      // (a row's largest logit always has a key)
             return;
         }
     }
@@ -254,7 +346,7 @@ int launch(cudaStream_t st, const Draft& d, bool pdl) {
     const int rows = d.total + d.seqs + (d.q ? d.total : 0), parts = parts_of(rows, d.vocab);
     if (const int e = launch_k(stretch_kernel<T>, dim3(rows, parts), dim3(THREADS), 0, st, pdl, d, parts)) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)d.seqs * CLUSTER); cfg.blockDim = dim3(THREADS); cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)d.seqs * CLUSTER); cfg.blockDim = dim3(RACERS); cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
