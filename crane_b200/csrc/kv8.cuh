@@ -20,7 +20,10 @@ int kv8_attention_launch(cudaStream_t st, const Kv8Attention& a, const Kv8Pool& 
 
 // Sequences with many rows of 16 bits, D up to 128 (kv8_flash.cu); kv8_attention_launch's business
 constexpr int KV8_FLASH_ROWS = 256;
-int kv8_flash_launch(cudaStream_t st, const Kv8Attention& a, const Kv8Deal& d, bool pdl);
+int kv8_flash_launch(cudaStream_t st, const Kv8Attention& a, const Kv8Deal& d, Kv8Join* joins, float* parts, bool pdl);
+
+// `work` begins with a Kv8Join for each CTA, the parts follow
+constexpr size_t kv8_joins(int ctas) { return (size_t)ctas * sizeof(Kv8Join); }
 
 #ifdef __CUDACC__
 // The steps of all sequences (kv8_units.h) and, in `sums`, those ahead of each of the KV8_SHARES equal shares of the sequences.  Every thread of the block.

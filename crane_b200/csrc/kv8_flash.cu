@@ -25,7 +25,8 @@ struct Args {
     void* out; long long ldo, ldoh;
     float scale2, sign;                        // |scale| log2 e; the scale's sign goes with the queries
     Kv8Deal d;
-    float* work;                               // [2 * CTAs][M][D + 2]
+    Kv8Join* joins;                            // [CTAs]
+    float* work;                               // parts [2 * CTAs][M][D + 2]
     int* err;
 };
 template <int D> struct Cfg {
@@ -97,6 +98,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     const long long total = kv8_count<Units>(a.d, sums);
     const long long begin = kv8_range(total, gridDim.x, blockIdx.x), end = kv8_range(total, gridDim.x, blockIdx.x + 1);
     pdl_launch_dependents();
+    if (tid == 128) a.joins[blockIdx.x].rows = 0;
     if (begin >= end) return;
     if (warp == 2) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
     tc_fence_before();
@@ -457,6 +459,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 }
             }
             if (!whole) { part_dst[D] = m; part_dst[D + 1] = l; }
+            if (tid == 128 && t0 == 0 && t1 < u.tiles) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
             tc_fence_before();
             step = u.first + t1;
             if (step < end && !u.next(a.d)) break;
@@ -478,8 +481,8 @@ int launch(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const 
 
 }  // namespace
 
-// Sequences that bring `lo` rows of a kv head and more; parts of units that lie with several CTAs are left in a.work
-int kv8_flash_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Deal& d, bool pdl) {
+// Sequences that bring `lo` rows of a kv head and more; parts of units that lie with several CTAs are left in `parts`
+int kv8_flash_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Deal& d, Kv8Join* joins, float* parts, bool pdl) {
     const int D = d.p.dim;
     const uint64_t n = (uint64_t)d.p.pages * d.p.kv_heads * d.p.page;
     CUtensorMap mk, mv;
@@ -488,7 +491,7 @@ int kv8_flash_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Deal& d, b
         !tc_tmap(&mv, d.p.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, n, D, D, rows, D, CU_TENSOR_MAP_SWIZZLE_NONE)) return (int)cudaErrorInvalidValue;
     const bool vec = (reinterpret_cast<uintptr_t>(k.q.p) | reinterpret_cast<uintptr_t>(k.out)) % 16 == 0 && (k.q.ld | k.q.ldh | k.ldo | k.ldoh) % 8 == 0;
     const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)(fabs((double)k.scale) * 1.4426950408889634074), k.scale < 0.f ? -1.f : 1.f, d,
-                    reinterpret_cast<float*>(k.work), k.err};
+                    joins, parts, k.err};
     if (k.q.type == KV8_BF16) return D == 64 ? launch<64, bf16>(st, mk, mv, a, vec, pdl) : launch<128, bf16>(st, mk, mv, a, vec, pdl);
     return D == 64 ? launch<64, __half>(st, mk, mv, a, vec, pdl) : launch<128, __half>(st, mk, mv, a, vec, pdl);
 }

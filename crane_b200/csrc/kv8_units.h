@@ -17,6 +17,12 @@ struct Kv8Seqs { const int* table; long long ldt; int width; const int* lens; co
 template <typename T> CB_HD T least(T a, T b) { return b < a ? b : a; }
 template <typename T> CB_HD T most(T a, T b) { return a < b ? b : a; }
 
+// a / b for numbers that are not negative, by 32 bits where they do (64-bit division is a hundred instructions one behind the other)
+CB_HD long long quotient(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return (long long)((unsigned)a / (unsigned)b);
+    return a / b;
+}
+
 // What a sequence brings
 struct Kv8Seq { int s0, n, len, first; };                           // first: position of row s0 (negative: rows ahead of position 0 are not in the cache)
 CB_HD int kv8_start(const Kv8Seqs& s, int b) { return least(most(s.starts[b], 0), s.rows); }
@@ -67,12 +73,12 @@ struct Kv8Units {
     CB_HD void shape(const Kv8Deal& d) {
         q = kv8_seq(d.s, b);
         const long long rows = (long long)q.n * d.group;
-        groups = rows < d.lo || rows > d.hi ? 0 : (int)((rows + M - 1) / M);
+        groups = rows < d.lo || rows > d.hi ? 0 : (int)quotient(rows + M - 1, M);
     }
     CB_HD int tiles_of(const Kv8Deal& d, int g) const {
-        const long long last = least((long long)q.n, (((long long)g + 1) * M - 1) / d.group + 1);      // tokens up to the group's last
+        const long long last = least((long long)q.n, quotient(((long long)g + 1) * M - 1, d.group) + 1);      // tokens up to the group's last
         const long long seen = least(q.first + last, (long long)d.s.width * d.p.page);
-        return most(1, (int)((seen + TILE - 1) / TILE));
+        return most(1, (int)(seen + TILE - 1) / TILE);
     }
     CB_HD long long head_steps(const Kv8Deal& d) const {
         long long n = 0;
@@ -103,17 +109,24 @@ struct Kv8Units {
             if (step < at + each * d.p.kv_heads || b + 1 >= d.s.seqs) break;
             at += each * d.p.kv_heads;
         }
-        head = (int)((step - at) / most(each, 1LL));
+        head = (int)quotient(step - at, most(each, 1LL));
         first = at + head * each;
         for (grp = 0; tiles = tiles_of(d, grp), first + tiles <= step && grp + 1 < groups; ++grp) first += tiles;
     }
 };
-CB_HD long long kv8_range(long long total, int ctas, int c) { return total / ctas * c + least((long long)c, total % ctas); }       // a CTA's first step
+CB_HD long long kv8_range(long long total, int ctas, int c) { const long long base = quotient(total, ctas); return base * c + least((long long)c, total - base * ctas); }       // a CTA's first step
 CB_HD int kv8_owner(long long total, int ctas, long long step) {
-    const long long base = total / ctas, rem = total % ctas, big = rem * (base + 1);
-    return (int)(step < big ? step / (base + 1) : rem + (step - big) / most(base, 1LL));
+    const long long base = quotient(total, ctas), rem = total - base * ctas, big = rem * (base + 1);
+    return (int)(step < big ? quotient(step, base + 1) : rem + quotient(step - big, most(base, 1LL)));
 }
 // Where a CTA leaves its part of a unit that it shares: 0 for the one that its range begins with, 1 for the one that it ends with
 CB_HD int kv8_slot(int cta, long long begin, long long part) { return 2 * cta + (part == begin ? 0 : 1); }
+
+// A unit that a CTA begins and does not end: what is needed to add up its parts, which lie with this CTA and those up to `last` (none: rows = 0)
+struct Kv8Join { int s0, head, grp, rows, last, slot, pad[2]; };
+template <typename U>
+CB_HD Kv8Join kv8_join(const Kv8Deal& d, const U& u, int m, long long total, int ctas, int c, long long begin) {
+    return Kv8Join{u.q.s0, u.head, u.grp, (int)least((long long)m, (long long)u.q.n * d.group - (long long)u.grp * m), kv8_owner(total, ctas, u.first + u.tiles - 1), kv8_slot(c, begin, u.first), {0, 0}};
+}
 
 }  // namespace cb

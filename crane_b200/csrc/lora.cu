@@ -88,22 +88,66 @@ template <typename X, typename W, int MT, int RT>
 struct Shape {
     static constexpr bool T32 = sizeof(X) == 4;                      // tf32 products; else those of the 16-bit type
     static constexpr int ROWS = 16 * MT, RP = 8 * RT, LDT = RP + 4;
+    static constexpr int MPW = MT == 1 || RT == 16 ? 1 : 2, MW = MT / MPW, KW = WARPS / MW;      // X A^T: row tiles of a warp, warps along the rows, along k
+    static constexpr int EM = MT == 1 ? 1 : 2, EW = MT / EM, CW = WARPS / EW;                    // T B^T: the same, along n
+    static constexpr int EB = MT > 1 ? 1 : T32 && RT > 4 ? 1 : 2;    // blocks of 32 columns a warp has under way
     static constexpr int KS = T32 ? RT : RT / 2;                     // MMAs along the rank
     static constexpr int T_BYTES = ROWS * LDT * 4, FRAG = MT * KS * 32 * 16;
-    static constexpr int SMEM = 2 * T_BYTES + 2 * FRAG;              // shares of T (this CTA's, read by the cluster), T, its two parts
+    // Many rows: the columns of a step, add and B, come in through a ring of stages
+    static constexpr int NC = CW * 32, ADD = ROWS * NC * (int)sizeof(X), STAGE = ADD + NC * RP * (int)sizeof(W);
+    static constexpr int CTAS = MT == 1 ? 2 : 2 * FRAG + 3 * STAGE <= 112 * 1024 ? 2 : 1;            // resident on an SM
+    static constexpr int FITS = ((CTAS == 2 ? 112 : 222) * 1024 - 2 * FRAG) / STAGE, STAGES = MT == 1 || FITS < 2 ? 0 : FITS > 4 ? 4 : FITS;
+    static constexpr int ROOM = STAGES * STAGE > 2 * T_BYTES ? STAGES * STAGE : 2 * T_BYTES;         // shares of T (this CTA's, read by the cluster) and T; later the stages
+    static constexpr int SMEM = 2 * FRAG + ROOM;                     // ahead of those the two parts of T
 };
 
+// o += T B^T over 16 of the rank: EM row tiles from `er` on, 32 columns
+template <typename X, typename W, int EM, int KS>
+__device__ __forceinline__ void multiply(float (&o)[EM][4][4], const Piece<W, 4> (&bv)[4], const uint4* hi_s, const uint4* lo_s, int er, int ks, int lane) {
+    if constexpr (sizeof(X) != 4) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)                 // (all of the lower parts first: no product waits for the one ahead of it)
+#pragma unroll
+            for (int i = 0; i < EM; ++i) {
+                const uint4 v = (half ? hi_s : lo_s)[((er + i) * KS + ks) * 32 + lane];
+                const uint32_t f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma16<W>(o[i][j], f, bv[j].w[0], bv[j].w[1]);
+            }
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) { const float v = bv[j].at(2 * s + e); bh[j][e] = tf32(v); if (sizeof(W) == 4) bl[j][e] = tf32_rest(v, bh[j][e]); }
+#pragma unroll
+            for (int i = 0; i < EM; ++i) {
+                const uint4 hv = hi_s[((er + i) * KS + ks * 2 + s) * 32 + lane], lv = lo_s[((er + i) * KS + ks * 2 + s) * 32 + lane];
+                const uint32_t fh[4] = {hv.x, hv.y, hv.z, hv.w}, fl[4] = {lv.x, lv.y, lv.z, lv.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (sizeof(W) == 4) mma_tf32(o[i][j], fh, bl[j][0], bl[j][1]);
+                    mma_tf32(o[i][j], fl, bh[j][0], bh[j][1]);
+                    mma_tf32(o[i][j], fh, bh[j][0], bh[j][1]);
+                }
+            }
+        }
+    }
+}
+
 template <typename X, typename W, int MT, int RT, bool VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, Shape<X, W, MT, RT>::CTAS)
 lora_kernel(Lora l, bool gather) {
     using S = Shape<X, W, MT, RT>;
     constexpr bool T32 = S::T32;
-    constexpr int ROWS = S::ROWS, LDT = S::LDT, KS = S::KS, MW = MT == 4 ? 2 : 1, KW = WARPS / MW, MPW = MT / MW;
+    constexpr int ROWS = S::ROWS, LDT = S::LDT, KS = S::KS, MW = S::MW, KW = S::KW, MPW = S::MPW, EM = S::EM, EW = S::EW, CW = S::CW, EB = S::EB;
     extern __shared__ __align__(16) unsigned char sm[];
-    float* share = reinterpret_cast<float*>(sm);
-    float* ts = reinterpret_cast<float*>(sm + S::T_BYTES);
-    uint4* hi_s = reinterpret_cast<uint4*>(sm + 2 * S::T_BYTES);
+    uint4* hi_s = reinterpret_cast<uint4*>(sm);
     uint4* lo_s = hi_s + S::FRAG / 16;
+    float* share = reinterpret_cast<float*>(sm + 2 * S::FRAG);
+    float* ts = share + S::T_BYTES / 4;
     __shared__ int rows_s[ROWS], which_s[ROWS];
     __shared__ float down_s[ROWS];                                   // powers of two that take the rows of T back out of f16's range
     __shared__ int n_rows_s;
@@ -159,7 +203,6 @@ lora_kernel(Lora l, bool gather) {
         if constexpr (ROWS > 32) mine |= (unsigned long long)__ballot_sync(0xffffffffu, which_s[(lane + 32) % ROWS] == w) << 32;
         mine &= left;
         left &= ~mine;
-        float o[MT][4][4];
         if (w >= 0) {
             // ---- this CTA's share of T ----
             const W* A = reinterpret_cast<const W*>(l.a) + (size_t)w * l.rank * l.k;
@@ -178,6 +221,7 @@ lora_kernel(Lora l, bool gather) {
                     xr[i][h] = r < n_rows && (mine >> r & 1) ? x + (long long)rows_s[r] * l.ldx : nullptr;
                 }
             const int kc = (l.k + 31) / 32, k0 = (int)((long long)kc * cr / nc), k1 = (int)((long long)kc * (cr + 1) / nc);
+#pragma unroll(RT <= 4 ? 4 : RT == 8 && MT == 1 ? 2 : 1)
             for (int c = k0 + kw; c < k1; c += KW) {
                 const int at = c * 32 + 8 * t, have = l.k - at;
                 Piece<X, 8> xv[MPW][2];
@@ -233,18 +277,22 @@ lora_kernel(Lora l, bool gather) {
             }
             if (nc > 1) cluster_sync_all();
             const float s = l.scales ? __ldg(l.scales + w) : 1.f;
-            for (int i = tid; i < ROWS * S::RP; i += THREADS) {
-                const int at = i / S::RP * LDT + i % S::RP;
-                float v = 0.f;
-                for (int c = 0; c < nc; ++c) {
-                    if (nc == 1) { v = share[at]; break; }
-                    float y;
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(y) : "r"(peer_smem(share + at, c)) : "memory");
-                    v += y;
+#pragma unroll 1
+            for (int i = tid; i < ROWS * S::RP / 4; i += THREADS) {
+                const int at = i / (S::RP / 4) * LDT + i % (S::RP / 4) * 4;
+                float4 v = *reinterpret_cast<const float4*>(share + at), y[8];
+                if (nc > 1) {                                        // (all on their way before the first is added)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < nc) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[c].x), "=f"(y[c].y), "=f"(y[c].z), "=f"(y[c].w) : "r"(peer_smem(share + at, c)));
+                    v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        if (c < nc) { v.x += y[c].x; v.y += y[c].y; v.z += y[c].z; v.w += y[c].w; }
                 }
-                ts[at] = s * v;
+                *reinterpret_cast<float4*>(ts + at) = make_float4(s * v.x, s * v.y, s * v.z, s * v.w);
             }
-            __syncthreads();
+            if (nc > 1) cluster_sync_all(); else __syncthreads();    // every CTA has read the shares: their room is free, and their owner may leave
             if constexpr (TYPE<W> == 2 && !T32) {
                 for (int r = warp; r < ROWS; r += WARPS) {
                     float top = 0.f;
@@ -286,113 +334,194 @@ lora_kernel(Lora l, bool gather) {
             }
             __syncthreads();
         }
-        // ---- out = add + T B^T: 32 columns a warp at a time ----
+        // ---- out = add + T B^T: EB blocks of 32 columns a warp at a time ----
         const W* B = reinterpret_cast<const W*>(l.b) + (size_t)max(w, 0) * l.n * l.rank;
-        if (w >= 0 || add != out)
-            for (int b = nb0 + warp; b < nb1; b += WARPS) {
-                const int n0 = b * 32, col = n0 + t * 8, have = l.n - col;
-                Piece<X, 8> av[MT][2];
-                if (add) {
+        const int er = warp % EW * EM;                               // this warp's first row tile
+        if constexpr (VEC && S::STAGES > 0) {
+            constexpr int ST = S::STAGES, NC = S::NC, CX = NC * (int)sizeof(X) / 16, CB = S::RP * (int)sizeof(W) / 16, EX = 16 / (int)sizeof(X), EWT = 16 / (int)sizeof(W);
+            // (16-byte pieces of a row change places by row, so that what a warp reads of several rows lies in banks of its own)
+            auto add_at = [](int row, int c) { return (row * CX + (c ^ (sizeof(X) == 4 ? row & 1 : (row & 1) << 2))) * 16; };
+            auto b_at = [](int row, int c) { return (row * CB + (c ^ ((sizeof(W) == 4 ? (row & 1) << 2 : ((row & 1) | (row >> 2 & 2)) << 1) & (CB - 1)))) * 16; };
+            unsigned char* ring = sm + 2 * S::FRAG;
+            const int c0 = nb0 * 32, c1 = min(nb1 * 32, l.n), steps = (c1 - c0 + NC - 1) / NC;
+            // A thread fetches the same piece of every AR-th row of add and of every BR-th row of B, whatever the step: addresses only advance
+            constexpr int AR = THREADS / CX, AK = ROWS / AR, BR = THREADS / CB, BK = NC / BR;
+            const int ac = tid % CX, bc = tid % CB, a_dst = add_at(tid / CX, ac), b_dst = S::ADD + b_at(tid / CB, bc);
+            const X* a_src[AK];
+            uint32_t a_in = 0;
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+            for (int k = 0; k < AK; ++k) {
+                const int row = tid / CX + k * AR;
+                const bool in = add && (mine >> row & 1);
+                a_in |= (uint32_t)in << k;
+                a_src[k] = add + (in ? (long long)rows_s[row] * l.ldadd + c0 + ac * EX : 0);
+            }
+            const bool b_in = bc * EWT < l.rank;
+            const W* b_src = B + (b_in ? (size_t)(c0 + tid / CB) * l.rank + bc * EWT : 0);
+            auto copy = [](uint32_t dst, const void* src, bool in) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); };
+            const uint32_t ring32 = smem_u32(ring);
+            auto fetch = [&](int step) {
+                const uint32_t st = ring32 + step % ST * S::STAGE;
+                const int off = step * NC;
+                if (add) {
+                    const bool here = c0 + off + ac * EX < c1;
+#pragma unroll
+                    for (int k = 0; k < AK; ++k) { const bool in = here && (a_in >> k & 1); copy(st + a_dst + k * (THREADS * 16), a_src[k] + (in ? off : 0), in); }
+                }
+                if (w >= 0) {
+                    const W* src = b_src + (size_t)off * l.rank;
+#pragma unroll
+                    for (int k = 0; k < BK; ++k) { const bool in = b_in && c0 + off + tid / CB + k * BR < c1; copy(st + b_dst + k * (THREADS * 16), in ? src + (size_t)(k * BR) * l.rank : B, in); }
+                }
+            };
+            const int cw = warp / EW * 32;
+            const bool idle = !(mine >> (er * 16) & ((1ull << (16 * EM)) - 1));      // none of this warp's rows
+            X* dst[EM][2];
+            uint32_t row_in = 0;
+            float downs[EM][2];
+#pragma unroll
+            for (int i = 0; i < EM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = (er + i) * 16 + h * 8 + g;
+                    const bool in = mine >> row & 1;
+                    row_in |= (uint32_t)in << (2 * i + h);
+                    dst[i][h] = out + (in ? (long long)rows_s[row] * l.ldo : 0) + c0 + cw + t * 8;
+                    downs[i][h] = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[row] : 1.f;
+                }
+            if (w >= 0 || add != out) {
+                for (int i = 0; i < ST - 1; ++i) { if (i < steps) fetch(i); asm volatile("cp.async.commit_group;" ::: "memory"); }
+#pragma unroll 1
+                for (int step = 0; step < steps; ++step) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
+                    __syncthreads();                                 // the step is there, the one before it read
+                    if (step + ST - 1 < steps) fetch(step + ST - 1);
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (idle) continue;
+                    const unsigned char* st = ring + step % ST * S::STAGE;
+                    float o[EM][4][4];
+#pragma unroll
+                    for (int i = 0; i < EM; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+                    if (w >= 0) {
+#pragma unroll
+                        for (int ks = 0; ks < RT / 2; ++ks) {
+                            if (ks * 16 >= l.rank) break;
+                            Piece<W, 4> bv[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const int row = cw + (g >> 1) * 8 + j * 2 + (g & 1);
+                                if constexpr (sizeof(W) == 4) {
+                                    const uint4 v = *reinterpret_cast<const uint4*>(st + S::ADD + b_at(row, ks * 4 + t));
+                                    bv[j].w[0] = v.x; bv[j].w[1] = v.y; bv[j].w[Piece<W, 4>::W - 2] = v.z; bv[j].w[Piece<W, 4>::W - 1] = v.w;
+                                } else {
+                                    const uint2 v = *reinterpret_cast<const uint2*>(st + S::ADD + b_at(row, ks * 2 + (t >> 1)) + (t & 1) * 8);
+                                    bv[j].w[0] = v.x; bv[j].w[1] = v.y;
+                                }
+                            }
+                            multiply<X, W, EM, KS>(o, bv, hi_s, lo_s, er, ks, lane);
+                        }
+                    }
+                    if (c0 + step * NC + cw + t * 8 < c1)
+#pragma unroll
+                        for (int i = 0; i < EM; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                if (!(row_in >> (2 * i + h) & 1)) continue;
+                                Piece<X, 8> av;
+#pragma unroll
+                                for (int q = 0; q < Piece<X, 8>::W; q += 4) {
+                                    const uint4 v = add ? *reinterpret_cast<const uint4*>(st + add_at((er + i) * 16 + h * 8 + g, (cw + t * 8) / EX + q / 4)) : make_uint4(0, 0, 0, 0);
+                                    av.w[q] = v.x; av.w[q + 1] = v.y; av.w[q + 2] = v.z; av.w[q + 3] = v.w;
+                                }
+                                __align__(16) X y[8];
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[i][q >> 1][2 * h + (q & 1)], downs[i][h], av.at(q)));
+#pragma unroll
+                                for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(dst[i][h] + step * NC)[q] = reinterpret_cast<const uint4*>(y)[q];
+                            }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+            }
+        } else if (w >= 0 || add != out)
+            for (int b0 = nb0 + warp / EW; b0 < nb1; b0 += CW * EB) {
+                Piece<X, 8> av[EB][EM][2];
+                float o[EB][EM][4][4];
+#pragma unroll
+                for (int b = 0; b < EB; ++b) {
+                    const int blk = b0 + b * CW, col = blk * 32 + t * 8, have = blk < nb1 ? l.n - col : 0;
+#pragma unroll
+                    for (int i = 0; i < EM; ++i)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const int r = i * 16 + h * 8 + g;
-                            const bool in = mine >> r & 1;
-                            // (may be out: not through the read-only path)
-                            const X* p = add + (in ? (long long)rows_s[r] * l.ldadd : 0) + col;
+                            const int r = (er + i) * 16 + h * 8 + g;
+                            const bool in = add && (mine >> r & 1);
 #pragma unroll
-                            for (int q = 0; q < Piece<X, 8>::W; ++q) av[i][h].w[q] = 0;
+                            for (int q = 0; q < Piece<X, 8>::W; ++q) av[b][i][h].w[q] = 0;
+                            const X* p = add + (in ? (long long)rows_s[r] * l.ldadd : 0) + col;      // (may be out: not through the read-only path)
                             if constexpr (VEC) {
                                 if (in && have >= 8) {
 #pragma unroll
                                     for (int q = 0; q < Piece<X, 8>::W; q += 4) {
                                         const uint4 v = reinterpret_cast<const uint4*>(p)[q / 4];
-                                        av[i][h].w[q] = v.x; av[i][h].w[q + 1] = v.y; av[i][h].w[q + 2] = v.z; av[i][h].w[q + 3] = v.w;
+                                        av[b][i][h].w[q] = v.x; av[b][i][h].w[q + 1] = v.y; av[b][i][h].w[q + 2] = v.z; av[b][i][h].w[q + 3] = v.w;
                                     }
                                 }
                             } else {
 #pragma unroll
                                 for (int q = 0; q < 8; ++q)
                                     if (in && q < have) {
-                                        if constexpr (sizeof(X) == 4) av[i][h].w[q] = reinterpret_cast<const uint32_t*>(p)[q];
-                                        else av[i][h].w[q / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[q] << (16 * (q & 1));
+                                        if constexpr (sizeof(X) == 4) av[b][i][h].w[q] = reinterpret_cast<const uint32_t*>(p)[q];
+                                        else av[b][i][h].w[q / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[q] << (16 * (q & 1));
                                     }
                             }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) o[b][i][j][2 * h] = o[b][i][j][2 * h + 1] = 0.f;
                         }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int q = 0; q < Piece<X, 8>::W; ++q) av[i][0].w[q] = av[i][1].w[q] = 0;
                 }
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
                 if (w >= 0) {
 #pragma unroll 2
                     for (int ks = 0; ks < RT / 2; ++ks) {
                         if (ks * 16 >= l.rank) break;
-                        Piece<W, 4> bv[4];
+                        Piece<W, 4> bv[EB][4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = n0 + (g >> 1) * 8 + j * 2 + (g & 1), c = ks * 16 + 4 * t;
-                            bv[j] = load<W, 4, VEC>(B + (size_t)r * l.rank + c, r < l.n ? l.rank - c : 0);
-                        }
-                        if constexpr (!T32) {
+                        for (int b = 0; b < EB; ++b)
 #pragma unroll
-                            for (int i = 0; i < MT; ++i) {
-                                const uint4 hv = hi_s[(i * KS + ks) * 32 + lane], lv = lo_s[(i * KS + ks) * 32 + lane];
-                                const uint32_t fh[4] = {hv.x, hv.y, hv.z, hv.w}, fl[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) { mma16<W>(o[i][j], fl, bv[j].w[0], bv[j].w[1]); mma16<W>(o[i][j], fh, bv[j].w[0], bv[j].w[1]); }
+                            for (int j = 0; j < 4; ++j) {
+                                const int blk = b0 + b * CW, r = blk * 32 + (g >> 1) * 8 + j * 2 + (g & 1), c = ks * 16 + 4 * t;
+                                bv[b][j] = load<W, 4, VEC>(B + (size_t)r * l.rank + c, blk < nb1 && r < l.n ? l.rank - c : 0);
                             }
-                        } else {
 #pragma unroll
-                            for (int s = 0; s < 2; ++s) {
-                                uint32_t bh[4][2], bl[4][2];
-#pragma unroll
-                                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) { const float v = bv[j].at(2 * s + e); bh[j][e] = tf32(v); if (sizeof(W) == 4) bl[j][e] = tf32_rest(v, bh[j][e]); }
-#pragma unroll
-                                for (int i = 0; i < MT; ++i) {
-                                    const uint4 hv = hi_s[(i * KS + ks * 2 + s) * 32 + lane], lv = lo_s[(i * KS + ks * 2 + s) * 32 + lane];
-                                    const uint32_t fh[4] = {hv.x, hv.y, hv.z, hv.w}, fl[4] = {lv.x, lv.y, lv.z, lv.w};
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        if (sizeof(W) == 4) mma_tf32(o[i][j], fh, bl[j][0], bl[j][1]);
-                                        mma_tf32(o[i][j], fl, bh[j][0], bh[j][1]);
-                                        mma_tf32(o[i][j], fh, bh[j][0], bh[j][1]);
-                                    }
-                                }
-                            }
-                        }
+                        for (int b = 0; b < EB; ++b) multiply<X, W, EM, KS>(o[b], bv[b], hi_s, lo_s, er, ks, lane);
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                for (int b = 0; b < EB; ++b) {
+                    const int blk = b0 + b * CW, col = blk * 32 + t * 8, have = blk < nb1 ? l.n - col : 0;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = i * 16 + h * 8 + g;
-                        if (!(mine >> r & 1) || have <= 0) continue;
-                        X* p = out + (long long)rows_s[r] * l.ldo + col;
-                        const float down = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[r] : 1.f;
-                        X y[8];
+                    for (int i = 0; i < EM; ++i)
 #pragma unroll
-                        for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[i][q >> 1][2 * h + (q & 1)], down, av[i][h].at(q)));
-                        if constexpr (VEC) {
-                            if (have >= 8)
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = (er + i) * 16 + h * 8 + g;
+                            if (!(mine >> r & 1) || have <= 0) continue;
+                            X* p = out + (long long)rows_s[r] * l.ldo + col;
+                            const float down = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[r] : 1.f;
+                            X y[8];
 #pragma unroll
-                                for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(y)[q];
-                        } else {
+                            for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[b][i][q >> 1][2 * h + (q & 1)], down, av[b][i][h].at(q)));
+                            if constexpr (VEC) {
+                                if (have >= 8)
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
+                                    for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(y)[q];
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
+                            }
                         }
-                    }
+                }
             }
-        if (w >= 0) { if (nc > 1) cluster_sync_all(); else __syncthreads(); }      // every CTA has read the shares: they may be written again, or their owner may leave
+        __syncthreads();                                             // (T's parts and the stages may be written again)
     }
 }
 
@@ -425,7 +554,7 @@ int launch_types(cudaStream_t st, const Lora& l, bool vec, bool pdl) {
     const bool gather = l.m <= 256;
     const int tiles = gather ? (l.m + 7) / 8 : (l.m + 63) / 64, sms = tc_device_sms();
     int cluster = 1;
-    while (cluster < 8 && tiles * cluster * 2 <= 2 * sms) cluster *= 2;
+    while (cluster < 8 && (!gather || tiles * cluster * 2 <= 2 * sms)) cluster *= 2;
     if (gather) return vec ? launch_rank<X, W, 1, true>(st, l, true, cluster, pdl) : launch_rank<X, W, 1, false>(st, l, true, cluster, pdl);
     return vec ? launch_rank<X, W, 4, true>(st, l, false, cluster, pdl) : launch_rank<X, W, 4, false>(st, l, false, cluster, pdl);
 }

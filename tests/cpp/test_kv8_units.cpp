@@ -108,19 +108,27 @@ static void units(const Case& c, int group, int ctas, long long lo, long long hi
         }
     }
     CHECK(next == total);
-    // what joins them: a CTA looks at the last unit of its range, if that began there and goes on
+    // what joins them: the unit that a CTA began and did not end
     std::set<std::tuple<int, int, int>> joined;
     for (int k = 0; k < ctas; ++k) {
         const long long begin = kv8_range(total, ctas, k), end = kv8_range(total, ctas, k + 1);
-        if (begin >= end || end >= total) continue;
+        if (begin == end) continue;
         U u;
-        u.seek(d, 0, 0, end - 1);
-        if (u.first + u.tiles <= end || u.first < begin) continue;
-        const auto& p = parts.at({u.b, u.head, u.grp});
-        const int last = kv8_owner(total, ctas, u.first + u.tiles - 1);
-        CHECK((int)p.size() == last - k + 1);
-        for (int i = k; i <= last; ++i) CHECK(p[i - k].first == (i == k ? kv8_slot(k, begin, u.first) : kv8_slot(i, 0, 0)));
-        CHECK(joined.insert({u.b, u.head, u.grp}).second);
+        u.seek(d, 0, 0, begin);
+        int here = 0;
+        for (long long step = begin; step < end;) {
+            const int t0 = (int)(step - u.first), t1 = (int)least((long long)u.tiles, end - u.first);
+            if (t0 == 0 && t1 < u.tiles) {
+                const Kv8Join j = kv8_join(d, u, M, total, ctas, k, begin);
+                CHECK(!here++ && j.rows >= 1 && j.rows <= M && j.last > k && j.last < ctas);
+                const auto& p = parts.at({u.b, u.head, u.grp});
+                CHECK((int)p.size() == j.last - k + 1);
+                for (int i = k; i <= j.last; ++i) CHECK(p[i - k].first == (i == k ? j.slot : kv8_slot(i, 0, 0)));
+                CHECK(joined.insert({u.b, u.head, u.grp}).second);
+            }
+            step = u.first + t1;
+            if (step < end) CHECK(u.next(d));
+        }
     }
     for (const auto& e : parts) {
         int at = 0;
