@@ -95,21 +95,22 @@ template <int BOX> __device__ __forceinline__ uint32_t piece(int r, int c) { ret
 template <int D> __device__ __forceinline__ int pos8(int n) { return D == 64 ? n : (n & 1) * 4 + (n >> 1); }
 __device__ __forceinline__ int col8(int n) { return (n & 1) * 4 + (n >> 1); }
 
-// Four warps and a fifth that copies, three such CTAs an SM (f32: two): the warps share rows (MG), columns of the result (CW) and positions (TG)
+// Four warps, a fifth that copies and a sixth that brings the queries of the next unit while they work, two such CTAs an SM: the four share rows (MG), columns of the result (CW)
+// and positions (TG)
 template <int D, typename T, int MG>
 struct Small {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int TILE = Step<D>::TILE, DC = D < 128 ? D : 128, CW = D / DC, TG = 4 / (MG * CW), M = 16 * MG, WARPS = 4, THREADS = 160;
+    static constexpr int TILE = Step<D>::TILE, DC = D < 128 ? D : 128, CW = D / DC, TG = 4 / (MG * CW), M = 16 * MG, WARPS = 4, THREADS = 192;
     static constexpr int SL = TILE / 16 / TG;                               // slices of a tile that a warp has: one (it takes those of two tiles together) or more
     static constexpr int AT_ONCE = SL == 1 ? 2 : 1;                         // tiles
     static constexpr int NT = DC / 8;                                       // MMAs across the columns
     static constexpr int KS = D / 16;                                       // ... along them
-    static constexpr int QBYTES = MG * KS * 512 * (F32 ? 2 : 1);            // query fragments
-    static constexpr int JT = NT / 4, JOIN = (TG > 1 ? TG / 2 : 0) * MG * CW * 32 * (JT * 4 + 4) * 4;      // sums on their way between warps, a quarter at a time
+    static constexpr int QBYTES = MG * KS * 512 * (F32 ? 2 : 1), QB = QBYTES > 16 * 1024 ? 1 : 2;          // query fragments, and for how many units
+    static constexpr int JOIN = (TG > 1 ? TG / 2 : 0) * MG * CW * 32 * (NT * 4 + 4) * 4;                   // sums on their way between warps
     static constexpr int CTAS = 2;                                          // resident on an SM (three, of 128 registers a thread: 189 us for a round of 64 sequences, two 145)
-    static constexpr int ROOM = (227 * 1024) / CTAS - 1024 - 2816 - JOIN - QBYTES - 1024;
+    static constexpr int ROOM = (227 * 1024) / CTAS - 1024 - 2816 - JOIN - QB * QBYTES - 1024;
     static constexpr int STAGES = ROOM / Step<D>::BYTES > 8 ? 8 : ROOM / Step<D>::BYTES;
-    static constexpr int SMEM = STAGES * Step<D>::BYTES + JOIN + QBYTES + 1024;
+    static constexpr int SMEM = STAGES * Step<D>::BYTES + JOIN + QB * QBYTES + 1024;
     static_assert(STAGES >= 3 && MG * CW * TG == 4 && SL * TG * 16 == TILE && (SL == 1 || SL % 2 == 0), "");
 };
 
@@ -120,12 +121,13 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     using St = Step<D>;
     constexpr int M = S::M, NT = S::NT, KS = S::KS, STAGES = S::STAGES, TILE = S::TILE, TG = S::TG, CW = S::CW;
     constexpr bool F32 = S::F32;
-    using Units = Kv8Units<M, TILE>;
+    using Units = Kv8Units<M, TILE, 4>;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
     float* join = reinterpret_cast<float*>(sm + STAGES * St::BYTES);
     uint32_t* qs = reinterpret_cast<uint32_t*>(sm + STAGES * St::BYTES + S::JOIN);
-    __shared__ uint64_t full[STAGES], empty[STAGES];
+    __shared__ uint64_t full[STAGES], empty[STAGES], q_full[2], q_empty[2];
+    __shared__ float down_s[2][M];                           // what takes a row's scaled queries back
     __shared__ float4 meta[STAGES][TILE / 16];               // of each 16 positions: ks, log2 vs, 1 / vs, and whether there is a page
     __shared__ long long sums[KV8_SHARES + 1];
     __shared__ int gave_up;
@@ -133,6 +135,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     if (tid == 0) {
         gave_up = 0;
         for (int i = 0; i < STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], S::WARPS); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&q_full[i], 1); mbar_init(&q_empty[i], S::WARPS); }
         fence_barrier_init();
         tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v);
     }
@@ -152,7 +155,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         int stage = 0;
         uint32_t parity = 1;
         for (long long step = begin; step < end;) {
-            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first), n = (t1 - t0) * boxes;
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end)), n = (t1 - t0) * boxes;
             for (int base = 0; base < n; base += 32) {
                 // a lane looks up one box: its row in the pool and its scales
                 int row = a.d.p.pages * a.d.p.kv_heads * P;                  // behind the pool: zeros come
@@ -186,7 +189,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     if (++stage == STAGES) { stage = 0; parity ^= 1; }
                 }
             }
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
         __syncwarp();
@@ -194,54 +197,75 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         return;
     }
 
-    // ---- products ----
-    const int g = lane >> 2, t = lane & 3, mg = warp % MG, cw = warp / MG % CW, tg = warp / (MG * CW);
-    int stage = 0;
-    uint32_t parity = 0;
-    for (long long step = begin; step < end;) {
-        const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
-        // ---- the unit's queries: fragments, and the factor that a row's scores take ----
-        float factor[2], fine[F32 ? 2 : 1];                  // ... and what f32 leaves of it
-        int pmax[2], wmin = INT_MAX;                         // last visible position of rows g and g + 8; the warp's rows all see the positions up to wmin
-        named_bar_sync(1, S::WARPS * 32);                    // (the fragments of the unit before are read)
+    const int g = lane >> 2, t = lane & 3;
+    if (warp == S::WARPS + 1) {
+        // ---- queries: fragments ----
+        int buf = 0;
+        uint32_t parity = 1;
+        for (long long step = begin; step < end;) {
+            wait(&q_empty[buf], parity);
+            uint32_t* q = qs + buf * (S::QBYTES / 4);
+#pragma unroll 1
+            for (int i = 0; i < 2 * MG; ++i) {               // rows g and g + 8 of each 16
+                const int r = i & 1, mg = i >> 1, row = u.grp * M + mg * 16 + g + r * 8, tok = row / group, h = u.head * group + row % group;
+                const bool in = tok < u.q.n;
+                const T* src = reinterpret_cast<const T*>(a.q) + (long long)(u.q.s0 + (in ? tok : 0)) * a.ldq + (long long)h * a.ldqh;
+                float v[D / 4], top = 0.f;                   // this lane's columns of the row
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = u.grp * M + mg * 16 + g + r * 8, tok = row / group, h = u.head * group + row % group;
-            const bool in = tok < u.q.n;
-            pmax[r] = in ? u.q.first + tok : -1;
-            if (in) wmin = min(wmin, pmax[r]);
-            const T* src = reinterpret_cast<const T*>(a.q) + (long long)(u.q.s0 + (in ? tok : 0)) * a.ldq + (long long)h * a.ldqh;
-            float v[D / 4], top = 0.f;                       // this lane's columns of the row
+                for (int p = 0; p < D / 64; ++p) {
 #pragma unroll
-            for (int p = 0; p < D / 64; ++p) {
+                    for (int j = 0; j < 16; ++j) v[p * 16 + j] = 0.f;
+                    if (in) load16<T>(src + p * 64 + t * 16, a.vec, v + p * 16);
+                }
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[p * 16 + j] = 0.f;
-                if (in) load16<T>(src + p * 64 + t * 16, a.vec, v + p * 16);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) top = v[p * 16 + j] != v[p * 16 + j] ? INFINITY : fmaxf(top, fabsf(v[p * 16 + j]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // 2^e that takes the row's largest magnitude to [2^14, 2^15); rows of less than 2^-100 count as zeros, rows with an infinity or a NaN give NaN
-            const uint32_t ex = __float_as_uint(fmaxf(top, 0x1p-100f)) >> 23;
-            const float up = __uint_as_float((uint32_t)(268 - ex) << 23), down = __uint_as_float((ex - 14) << 23);
-            factor[r] = top < INFINITY ? a.scale2 * down : NAN;
-            if (F32) fine[F32 ? r : 0] = a.scale2_rest * down;
-            if (tg == 0 && cw == 0) {
+                for (int j = 0; j < D / 4; ++j) top = v[j] != v[j] ? INFINITY : fmaxf(top, fabsf(v[j]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                // 2^e that takes the row's largest magnitude to [2^14, 2^15); rows of less than 2^-100 count as zeros, rows with an infinity or a NaN give NaN
+                const uint32_t ex = __float_as_uint(fmaxf(top, 0x1p-100f)) >> 23;
+                const float up = __uint_as_float((uint32_t)(268 - ex) << 23);
+                if (t == 0) down_s[buf][mg * 16 + g + r * 8] = top < INFINITY ? __uint_as_float((ex - 14) << 23) : NAN;
 #pragma unroll
                 for (int s = 0; s < KS; ++s)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {            // registers r and r + 2 of the fragment
-                        const float x = top < INFINITY ? v[4 * s + 2 * i] * up : 0.f, y = top < INFINITY ? v[4 * s + 2 * i + 1] * up : 0.f;
+                    for (int c = 0; c < 2; ++c) {            // registers r and r + 2 of the fragment
+                        const float x = top < INFINITY ? v[4 * s + 2 * c] * up : 0.f, y = top < INFINITY ? v[4 * s + 2 * c + 1] * up : 0.f;
                         const uint32_t f = pack_f16(x, y);
-                        uint32_t* d = qs + ((mg * KS + s) * 32 + lane) * 4 + r + 2 * i;
+                        uint32_t* d = q + ((mg * KS + s) * 32 + lane) * 4 + r + 2 * c;
                         d[0] = f;
                         if (F32) { const float2 hf = unpack_f16(f); d[MG * KS * 128] = pack_f16(x - hf.x, y - hf.y); }
                     }
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[buf]);
+            if (++buf == S::QB) { buf = 0; parity ^= 1; }
+            step = u.stop(end);
+            if (step < end && !u.next(a.d)) break;
         }
-        named_bar_sync(1, S::WARPS * 32);
-        const uint4* qf = reinterpret_cast<const uint4*>(qs) + mg * KS * 32 + lane;
+        return;
+    }
+
+    // ---- products ----
+    const int mg = warp % MG, cw = warp / MG % CW, tg = warp / (MG * CW);
+    int stage = 0, buf = 0;
+    uint32_t parity = 0, q_parity = 0;
+    for (long long step = begin; step < end;) {
+        const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
+        // ---- the unit's rows: what their scores are multiplied by, what they see ----
+        float factor[2], fine[F32 ? 2 : 1];                  // ... and what f32 leaves of it
+        int pmax[2], wmin = INT_MAX;                         // last visible position of rows g and g + 8; the warp's rows all see the positions up to wmin
+        wait(&q_full[buf], q_parity);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = u.grp * M + mg * 16 + g + r * 8, tok = row / group;
+            const bool in = tok < u.q.n;
+            pmax[r] = in ? u.q.first + tok : -1;
+            if (in) wmin = min(wmin, pmax[r]);
+            const float down = down_s[buf][mg * 16 + g + r * 8];
+            factor[r] = a.scale2 * down;
+            if (F32) fine[F32 ? r : 0] = a.scale2_rest * down;
+        }
+        const uint4* qf = reinterpret_cast<const uint4*>(qs + buf * (S::QBYTES / 4)) + mg * KS * 32 + lane;
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) wmin = min(wmin, __shfl_xor_sync(0xffffffffu, wmin, o));
         float o_acc[NT][4];
@@ -273,13 +297,13 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 const bool edge = pos0[1] + 15 > wmin || sc[0].w == 0.f || sc[1].w == 0.f;      // not all of the warp's rows see all of it
                 if (edge && __all_sync(0xffffffffu, (sc[0].w == 0.f || (pos0[0] > pmax[0] && pos0[0] > pmax[1])) && (sc[1].w == 0.f || (pos0[1] > pmax[0] && pos0[1] > pmax[1])))) continue;
                 // ---- scores ----
-                float s_acc[2][2][4], lo_acc[F32 ? 2 : 1][2][4];
+                float s_acc[2][2][4];
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) { s_acc[k][nt][e] = 0.f; if (F32) lo_acc[F32 ? k : 0][nt][e] = 0.f; }
+                        for (int e = 0; e < 4; ++e) s_acc[k][nt][e] = 0.f;
 #pragma unroll
                 for (int p = 0; p < D / 64; ++p) {           // pieces t, t + 4 of each plane
                     uint32_t w[2][2][4];
@@ -299,18 +323,11 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                             for (int nt = 0; nt < 2; ++nt) {
                                 uint32_t b0, b1;
                                 halves_of(w[k][nt][i], b0, b1);
-                                if (F32) mma_f16(lo_acc[F32 ? k : 0][nt], z, b0, b1);      // (a chain of its own: the tensor core cuts its sums off where f32 rounds)
+                                if (F32) mma_f16(s_acc[k][nt], z, b0, b1);
                                 mma_f16(s_acc[k][nt], x, b0, b1);
                             }
                     }
                 }
-                if (F32)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s_acc[k][nt][e] += lo_acc[F32 ? k : 0][nt][e];
                 // ---- weights ----
                 float f[2][2], mx[2] = {-INFINITY, -INFINITY};
                 uint32_t hidden = 0;
@@ -422,7 +439,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
                                 float* acc = o_acc[w * 4 + c2 * 2 + c];
-                                if constexpr (F32) {         // (long sums are f32 additions)
+                                if constexpr (F32) {         // (long sums are f32 additions: the tensor core cuts its sums off where f32 rounds)
                                     float part[4] = {0.f, 0.f, 0.f, 0.f};
                                     mma_f16(part, pl[F32 ? k : 0], b[c][0], b[c][1]);
                                     mma_f16(part, pa[k], b[c][0], b[c][1]);
@@ -440,6 +457,9 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
             for (int i = 0; i < S::AT_ONCE; ++i) if (i == 0 || two) { if (++stage == STAGES) { stage = 0; parity ^= 1; } }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_empty[buf]);
+        if (++buf == S::QB) { buf = 0; q_parity ^= 1; }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             l_row[r] += __shfl_xor_sync(0xffffffffu, l_row[r], 1);
@@ -461,44 +481,38 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         }
             }
         }
-        // ---- the warps that share rows and columns add up, half of them into the other half each time, a quarter of the columns at a time ----
+        // ---- the warps that share rows and columns add up, half of them into the other half each time ----
 #pragma unroll
         for (int h = TG / 2; h >= 1; h /= 2) {
-            float c0[2] = {1.f, 1.f}, c1[2] = {1.f, 1.f};
+            named_bar_sync(1, S::WARPS * 32);
+            float* d = join + (size_t)((tg % h) * (MG * CW) + cw * MG + mg) * 32 * (NT * 4 + 4) + lane;
+            if (tg >= h && tg < 2 * h) {
 #pragma unroll
-            for (int j4 = 0; j4 < 4; ++j4) {
-                named_bar_sync(1, S::WARPS * 32);
-                float* d = join + (size_t)((tg % h) * (MG * CW) + cw * MG + mg) * 32 * (S::JT * 4 + 4) + lane;
-                if (tg >= h && tg < 2 * h) {
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int j = 0; j < S::JT; ++j)
+                    for (int e = 0; e < 4; ++e) d[(j * 4 + e) * 32] = o_acc[j][e];
+                d[(NT * 4) * 32] = m_row[0]; d[(NT * 4 + 1) * 32] = m_row[1]; d[(NT * 4 + 2) * 32] = l_row[0]; d[(NT * 4 + 3) * 32] = l_row[1];
+            }
+            named_bar_sync(1, S::WARPS * 32);
+            if (tg < h) {
+                float c0[2], c1[2];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) d[(j * 4 + e) * 32] = o_acc[j4 * S::JT + j][e];
-                    if (j4 == 0) { d[(S::JT * 4) * 32] = m_row[0]; d[(S::JT * 4 + 1) * 32] = m_row[1]; d[(S::JT * 4 + 2) * 32] = l_row[0]; d[(S::JT * 4 + 3) * 32] = l_row[1]; }
+                for (int r = 0; r < 2; ++r) {
+                    const float mo = d[(NT * 4 + r) * 32], mn = fmaxf(m_row[r], mo);
+                    c0[r] = m_row[r] == -INFINITY ? 0.f : m_row[r] == mn ? 1.f : ex2(m_row[r] - mn);
+                    c1[r] = mo == -INFINITY ? 0.f : mo == mn ? 1.f : ex2(mo - mn);
+                    m_row[r] = mn;
+                    l_row[r] = l_row[r] * c0[r] + d[(NT * 4 + 2 + r) * 32] * c1[r];
                 }
-                named_bar_sync(1, S::WARPS * 32);
-                if (tg < h) {
-                    if (j4 == 0)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float mo = d[(S::JT * 4 + r) * 32], mn = fmaxf(m_row[r], mo);
-                            c0[r] = m_row[r] == -INFINITY ? 0.f : ex2(m_row[r] - mn);
-                            c1[r] = mo == -INFINITY ? 0.f : ex2(mo - mn);
-                            if (m_row[r] == mn) c0[r] = mn == -INFINITY ? 0.f : 1.f;
-                            if (mo == mn) c1[r] = mn == -INFINITY ? 0.f : 1.f;
-                            m_row[r] = mn;
-                            l_row[r] = l_row[r] * c0[r] + d[(S::JT * 4 + 2 + r) * 32] * c1[r];
-                        }
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int j = 0; j < S::JT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) { float& o = o_acc[j4 * S::JT + j][e]; o = o * c0[e >> 1] + d[(j * 4 + e) * 32] * c1[e >> 1]; }
-                }
+                    for (int e = 0; e < 4; ++e) o_acc[j][e] = o_acc[j][e] * c0[e >> 1] + d[(j * 4 + e) * 32] * c1[e >> 1];
             }
         }
-        if (tid == 0 && t0 == 0 && t1 < u.tiles) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
+        if (tid == 0 && u.begins(step, end)) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
         if (tg == 0) {
-            const bool whole = t0 == 0 && t1 == u.tiles;
+            const bool whole = u.whole(step, end);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int row = mg * 16 + g + r * 8, tok = (u.grp * M + row) / group, h = u.head * group + (u.grp * M + row) % group;
@@ -520,7 +534,7 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 if (!whole && t == 0 && cw == 0) { part[D] = m_row[r]; part[D + 1] = l_row[r]; }
             }
         }
-        step = u.first + t1;
+        step = u.stop(end);
         if (step < end && !u.next(a.d)) break;
     }
     if (tid == 0) wait.drain();
@@ -580,8 +594,11 @@ join_kernel(Args a) {
 
 // Rows of a kv head from which on a sequence goes through kv8_flash.cu: 16-bit ones of 64 and 128 columns.
 constexpr int FLASH_FROM = 65;
+// Where some sequence may bring more rows than this, and none goes to kv8_flash.cu, those of up to so many run by themselves, 16 rows a group: a decoded token beside a prompt's
+// portion would have one warp of four at work (23 sequences, portions of up to 333 tokens among decoded ones, f32: 265 us in one, NNN in two)
+constexpr int MIXED_FROM = 32;
 bool flash_takes(int type, int dim, int group, int max_rows) { return type != KV8_F32 && dim <= 128 && (long long)group * max_rows >= FLASH_FROM; }
-// Rows of a group of queries: 16 where no sequence brings more, else 32 or 64.  (Beside kv8_flash.cu 16: most of what is left are decoded tokens.)
+// Rows of a group of queries, from the most that a sequence brings: 16 or 32 where that is enough, else 64 (or 32).  (Beside kv8_flash.cu 16: most of what is left are decoded tokens.)
 int rows_of(int group, int dim, int max_rows, bool flash) {
     const long long r = (long long)group * max_rows;
     return r <= 16 || flash ? 16 : r <= 32 || dim == 256 ? 32 : 64;
@@ -599,7 +616,7 @@ int launch(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const 
     if (const int e = ensure_dyn_smem(small_kernel<D, T, MG>, (size_t)S::SMEM, seen)) return e;
     const int ctas = tc_device_sms() * S::CTAS;
     if (const int e = launch_k(small_kernel<D, T, MG>, dim3(ctas), dim3(S::THREADS), S::SMEM, st, pdl, mk, mv, a)) return e;
-    return launch_k(join_kernel<D, T, S::M>, dim3(ctas - 1, S::M / 4), dim3(128), 0, st, true, a);
+    return launch_k(join_kernel<D, T, S::M>, dim3(ctas - 1, S::M == 64 ? 64 : 4), dim3(128), 0, st, true, a);
 }
 template <int D, typename T>
 int launch_rows(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int rows, bool pdl) {
@@ -643,8 +660,17 @@ int kv8_attention_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Pool& 
     const bool vec = (reinterpret_cast<uintptr_t>(k.q.p) | reinterpret_cast<uintptr_t>(k.out)) % 16 == 0 && (k.q.ld | k.q.ldh | k.ldo | k.ldoh) % per == 0;
     const double scale2 = (double)k.scale * 1.4426950408889634074;
     const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)scale2, (float)(scale2 - (double)(float)scale2), Kv8Deal{s, pool, group, 0, flash ? FLASH_FROM - 1 : 1LL << 62}, reinterpret_cast<Kv8Join*>(k.work), reinterpret_cast<float*>(reinterpret_cast<char*>(k.work) + kv8_joins(2 * tc_device_sms())), k.err, vec};
-    if (k.q.type == KV8_F32) return launch_dim<float>(st, mk, mv, a, rows, pdl);
-    if (const int e = k.q.type == KV8_BF16 ? launch_dim<bf16>(st, mk, mv, a, rows, pdl) : launch_dim<__half>(st, mk, mv, a, rows, pdl)) return e;
+    auto go = [&](const Args& x, int m, bool dependent) {
+        return k.q.type == KV8_F32 ? launch_dim<float>(st, mk, mv, x, m, dependent) : k.q.type == KV8_BF16 ? launch_dim<bf16>(st, mk, mv, x, m, dependent) : launch_dim<__half>(st, mk, mv, x, m, dependent);
+    };
+    if (!flash && s.seqs > 1 && (long long)group * k.max_rows > MIXED_FROM) {
+        Args few = a, many = a;
+        few.d.hi = MIXED_FROM;
+        many.d.lo = MIXED_FROM + 1;
+        if (const int e = go(few, 16, pdl)) return e;
+        return go(many, rows, true);
+    }
+    if (const int e = go(a, rows, pdl)) return e;
     if (!flash) return 0;
     Args f = a;
     f.d.lo = FLASH_FROM;

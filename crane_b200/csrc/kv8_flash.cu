@@ -18,7 +18,7 @@ namespace {
 
 constexpr int M = KV8_FLASH_ROWS, BN = 128, THREADS = 512;
 constexpr float P_SHIFT = 6.f;                 // weights run up to 2^14: the reference trails a row's maximum by up to 8
-using Units = Kv8Units<M, BN>;
+using Units = Kv8Units<M, BN, 0>;       // (no steps of a unit's own: every part has a tile)
 
 struct Args {
     const void* q; long long ldq, ldqh;
@@ -115,7 +115,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         int st = 0, seq = 0;
         uint32_t ph = 1;
         for (long long step = begin; step < end;) {
-            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first), n = (t1 - t0) * boxes;
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end)), n = (t1 - t0) * boxes;
             for (int base = 0; base < n; base += 32) {
                 int row = a.d.p.pages * a.d.p.kv_heads * P;                  // behind the pool: zeros come
                 float4 sc = make_float4(0.f, 0.f, 1.f, 0.f);
@@ -149,7 +149,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     }
                 }
             }
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
     } else if (warp == 1) {
@@ -180,7 +180,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         auto release = [&](int slot) { if (elect_one()) umma_commit(&empty[slot]); __syncwarp(); };
         auto step_on = [&]() { if (++st == NF) { st = 0; ph ^= 1; } };
         for (long long step = begin; step < end; ++part) {
-            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
             wait(&full[st], ph);
             for (int w = 0; w < 2; ++w) {
                 wait(&q_full[w], part & 1);
@@ -208,7 +208,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 p_ph ^= 1;
                 if (!last) { release(st); step_on(); }
             }
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
     } else if (warp >= 12) {
@@ -217,7 +217,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         int rs = 0, fs = 0, seq = 0, part = 0;
         uint32_t r_ph = 0, f_ph = 1;
         for (long long step = begin; step < end; ++part) {
-            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
             const int seen = u.q.first + (int)((long long)u.grp * M / group);      // last position that all rows see
             for (int t = t0; t < t1; ++t, ++seq) {
                 const bool edge = t * BN + BN - 1 > seen;
@@ -257,7 +257,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     if (++fs == NF) { fs = 0; f_ph ^= 1; }
                 }
             }
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
     } else if (warp >= 4) {
@@ -268,7 +268,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         int seq = 0, part = 0;
         uint32_t s_ph = 0;
         for (long long step = begin; step < end; ++part) {
-            const int t0 = (int)(step - u.first), t1 = (int)min((long long)u.tiles, end - u.first);
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
             // ---- the queries of this warp's rows, D / 8 lanes a row: f16, each row's largest moved to [2^14, 2^15) by a power of two ----
             constexpr int LR = D / 8, RW = 32 / LR;          // lanes a row, rows at a time
 #pragma unroll 4
@@ -426,7 +426,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         for (int j = 0; j < 32; ++j) if ((v[i * 32 + j] & 0x7f) == 0x7f) odd[i] |= 1u << j;
                 }
             }
-            const bool whole = t0 == 0 && t1 == u.tiles;
+            const bool whole = u.whole(step, end);
             const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
             T* dst = reinterpret_cast<T*>(a.out) + (long long)(u.q.s0 + (in ? tok : 0)) * a.ldo + (long long)h * a.ldoh;
             float* part_dst = a.work + ((size_t)kv8_slot(blockIdx.x, begin, step) * M + r) * (D + 2);
@@ -459,9 +459,9 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 }
             }
             if (!whole) { part_dst[D] = m; part_dst[D + 1] = l; }
-            if (tid == 128 && t0 == 0 && t1 < u.tiles) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
+            if (tid == 128 && u.begins(step, end)) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
             tc_fence_before();
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
     }

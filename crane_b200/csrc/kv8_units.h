@@ -61,10 +61,10 @@ CB_HD Kv8Piece kv8_piece(const Kv8Seqs& s, const Kv8Seq& q, int page, int b, int
 
 // ---- attention: how the steps are dealt out ----------------------------------------------------------------------------------------
 // A unit is a sequence, a kv head and a group of M rows of its queries (row = token * group + head of the group); its steps are the tiles of TILE positions that the group's last
-// row sees, one at least.  All steps, unit after unit, are dealt out evenly to the CTAs, whatever the lengths: a unit may lie with several CTAs, which then leave their parts of
+// row sees, one at least, behind OWN more that stand for what a unit costs by itself.  All steps, unit after unit, are dealt out evenly to the CTAs, whatever the lengths: a unit may lie with several CTAs, which then leave their parts of
 // the sums to be joined.  A kernel takes the sequences that bring from `lo` to `hi` rows.
 struct Kv8Deal { Kv8Seqs s; Kv8Pool p; int group; long long lo, hi; };
-template <int M, int TILE>
+template <int M, int TILE, int OWN>
 struct Kv8Units {
     int b, head, grp;                          // the unit
     Kv8Seq q;
@@ -82,11 +82,16 @@ struct Kv8Units {
     }
     CB_HD long long head_steps(const Kv8Deal& d) const {
         long long n = 0;
-        for (int g = 0; g < groups; ++g) n += tiles_of(d, g);
+        for (int g = 0; g < groups; ++g) n += tiles_of(d, g) + OWN;
         return n;
     }
+    CB_HD int size() const { return tiles + OWN; }
+    CB_HD long long stop(long long end) const { return least(first + size(), end); }       // where the part of a CTA whose steps run up to `end` ends
+    CB_HD int tile_at(long long step) const { return most(0, (int)(step - first) - OWN); }       // tiles ahead of a step
+    CB_HD bool whole(long long step, long long end) const { return step == first && stop(end) == first + size(); }
+    CB_HD bool begins(long long step, long long end) const { return step == first && stop(end) < first + size(); }      // ... and goes on with the next CTA
     CB_HD bool next(const Kv8Deal& d) {        // false: behind the last
-        first += tiles;
+        first += size();
         if (++grp >= groups) {
             grp = 0;
             if (++head >= d.p.kv_heads) {
@@ -111,7 +116,7 @@ struct Kv8Units {
         }
         head = (int)quotient(step - at, most(each, 1LL));
         first = at + head * each;
-        for (grp = 0; tiles = tiles_of(d, grp), first + tiles <= step && grp + 1 < groups; ++grp) first += tiles;
+        for (grp = 0; tiles = tiles_of(d, grp), first + size() <= step && grp + 1 < groups; ++grp) first += size();
     }
 };
 CB_HD long long kv8_range(long long total, int ctas, int c) { const long long base = quotient(total, ctas); return base * c + least((long long)c, total - base * ctas); }       // a CTA's first step
@@ -126,7 +131,7 @@ CB_HD int kv8_slot(int cta, long long begin, long long part) { return 2 * cta + 
 struct Kv8Join { int s0, head, grp, rows, last, slot, pad[2]; };
 template <typename U>
 CB_HD Kv8Join kv8_join(const Kv8Deal& d, const U& u, int m, long long total, int ctas, int c, long long begin) {
-    return Kv8Join{u.q.s0, u.head, u.grp, (int)least((long long)m, (long long)u.q.n * d.group - (long long)u.grp * m), kv8_owner(total, ctas, u.first + u.tiles - 1), kv8_slot(c, begin, u.first), {0, 0}};
+    return Kv8Join{u.q.s0, u.head, u.grp, (int)least((long long)m, (long long)u.q.n * d.group - (long long)u.grp * m), kv8_owner(total, ctas, u.first + u.size() - 1), kv8_slot(c, begin, u.first), {0, 0}};
 }
 
 }  // namespace cb

@@ -67,9 +67,9 @@ static void pieces(const Case& c, bool wild) {
     }
 }
 
-template <int M, int TILE>
+template <int M, int TILE, int OWN>
 static void units(const Case& c, int group, int ctas, long long lo, long long hi) {
-    using U = Kv8Units<M, TILE>;
+    using U = Kv8Units<M, TILE, OWN>;
     const Kv8Deal d = {c.s, c.p, group, lo, hi};
     long long total = 0;
     for (int b = 0; b < c.s.seqs; ++b) {
@@ -92,18 +92,19 @@ static void units(const Case& c, int group, int ctas, long long lo, long long hi
         U u;
         u.seek(d, 0, 0, begin);
         for (long long step = begin; step < end;) {
-            CHECK(u.first <= step && step < u.first + u.tiles && u.head >= 0 && u.head < c.p.kv_heads && u.grp >= 0 && u.grp < u.groups && u.b < c.s.seqs);
+            CHECK(u.first <= step && step < u.first + u.size() && u.head >= 0 && u.head < c.p.kv_heads && u.grp >= 0 && u.grp < u.groups && u.b < c.s.seqs);
             CHECK(u.tiles >= 1 && (long long)(u.tiles - 1) * TILE < (long long)c.s.width * c.p.page);
             const long long row = least((long long)u.q.n * group, (u.grp + 1LL) * M) - 1;            // the group's last row and what it sees
             const long long seen = least((long long)u.q.first + row / group + 1, (long long)c.s.width * c.p.page);
             CHECK((long long)u.tiles * TILE >= seen && ((long long)(u.tiles - 1) * TILE < seen || u.tiles == 1));
-            const int t0 = (int)(step - u.first), t1 = (int)least((long long)u.tiles, end - u.first);
-            const bool whole = t0 == 0 && t1 == u.tiles;
+            const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
+            const bool whole = u.whole(step, end);
+            CHECK(t0 <= t1 && t1 <= u.tiles && u.size() == u.tiles + OWN && (!whole || (t0 == 0 && t1 == u.tiles)));
             const int slot = whole ? -1 : kv8_slot(k, begin, step);
             if (!whole) CHECK(slot < 2 * ctas && slots.insert(slot).second);
             parts[{u.b, u.head, u.grp}].push_back({slot, {t0, t1}});
             tiles[{u.b, u.head, u.grp}] = u.tiles;
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end) CHECK(u.next(d));
         }
     }
@@ -117,8 +118,7 @@ static void units(const Case& c, int group, int ctas, long long lo, long long hi
         u.seek(d, 0, 0, begin);
         int here = 0;
         for (long long step = begin; step < end;) {
-            const int t0 = (int)(step - u.first), t1 = (int)least((long long)u.tiles, end - u.first);
-            if (t0 == 0 && t1 < u.tiles) {
+            if (u.begins(step, end)) {
                 const Kv8Join j = kv8_join(d, u, M, total, ctas, k, begin);
                 CHECK(!here++ && j.rows >= 1 && j.rows <= M && j.last > k && j.last < ctas);
                 const auto& p = parts.at({u.b, u.head, u.grp});
@@ -126,7 +126,7 @@ static void units(const Case& c, int group, int ctas, long long lo, long long hi
                 for (int i = k; i <= j.last; ++i) CHECK(p[i - k].first == (i == k ? j.slot : kv8_slot(i, 0, 0)));
                 CHECK(joined.insert({u.b, u.head, u.grp}).second);
             }
-            step = u.first + t1;
+            step = u.stop(end);
             if (step < end) CHECK(u.next(d));
         }
     }
@@ -150,11 +150,11 @@ int main() {
         pieces(wild, true);
         for (int ctas : {1, 3, 148, 296}) {
             const int group = 1 + i % 7;
-            units<16, 64>(tame, group, ctas, 0, 1LL << 62);
-            units<16, 64>(tame, group, ctas, 0, 64);
-            units<64, 64>(wild, group, ctas, 0, 1LL << 62);
-            units<256, 128>(tame, group, ctas, 65, 1LL << 62);
-            units<256, 128>(wild, group, ctas, 65, 1LL << 62);
+            units<16, 64, 2>(tame, group, ctas, 0, 1LL << 62);
+            units<16, 64, 2>(tame, group, ctas, 0, 64);
+            units<64, 64, 2>(wild, group, ctas, 0, 1LL << 62);
+            units<256, 128, 0>(tame, group, ctas, 65, 1LL << 62);
+            units<256, 128, 0>(wild, group, ctas, 65, 1LL << 62);
         }
     }
     std::puts("ok");
