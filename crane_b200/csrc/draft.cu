@@ -184,7 +184,8 @@ race_kernel(Draft d, int parts) {
     pdl_wait();
     pdl_launch_dependents();
     __shared__ int first_s;
-    __shared__ Part rows_s[2];
+    constexpr int KEPT = 32;                            // rows of a sequence whose sums stay at hand
+    __shared__ Part rows_s[2], p_s[KEPT], q_s[KEPT];
     __shared__ double key_s[RACERS / 32];
     __shared__ int at_s[RACERS / 32];
     __shared__ double best_s;
@@ -200,11 +201,12 @@ race_kernel(Draft d, int parts) {
     const T* y0 = reinterpret_cast<const T*>(d.q) + (d.q ? (long long)s0 * d.ldq : 0);
     if (threadIdx.x == 0) first_s = n;
     __syncthreads();
-    for (int j = warp; j < n; j += RACERS / 32) {
+    for (int j = warp; j <= n; j += RACERS / 32) {
         const Part p = whole(parts_p + (long long)(s0 + b + j) * parts, parts, inv_t);
         Part q = {};
-        if (d.q && !greedy) q = whole(parts_p + (long long)(d.total + d.seqs + s0 + j) * parts, parts, inv_t);
-        if (lane == 0) {
+        if (d.q && !greedy && j < n) q = whole(parts_p + (long long)(d.total + d.seqs + s0 + j) * parts, parts, inv_t);
+        if (lane == 0 && j < KEPT) { p_s[j] = p; q_s[j] = q; }
+        if (lane == 0 && j < n) {
             const int tok = __ldg(d.tokens + s0 + j);
             bool ok = (unsigned)tok < (unsigned)d.vocab;
             if (ok && greedy) ok = p.top > -INFINITY && tok == p.at;
@@ -217,15 +219,17 @@ race_kernel(Draft d, int parts) {
     }
     __syncthreads();
     const int j = first_s;
-    if (warp == 0) {
-        const Part p = whole(parts_p + (long long)(s0 + b + j) * parts, parts, inv_t);
-        if (lane == 0) rows_s[0] = p;
-    } else if (warp == 1 && d.q && !greedy && j < n) {
-        const Part q = whole(parts_p + (long long)(d.total + d.seqs + s0 + j) * parts, parts, inv_t);
-        if (lane == 0) rows_s[1] = q;
+    if (j >= KEPT) {                                    // (the block alike)
+        if (warp == 0) {
+            const Part p = whole(parts_p + (long long)(s0 + b + j) * parts, parts, inv_t);
+            if (lane == 0) rows_s[0] = p;
+        } else if (warp == 1 && d.q && !greedy && j < n) {
+            const Part q = whole(parts_p + (long long)(d.total + d.seqs + s0 + j) * parts, parts, inv_t);
+            if (lane == 0) rows_s[1] = q;
+        }
+        __syncthreads();
     }
-    __syncthreads();
-    const Part p = rows_s[0], q = j < n && d.q && !greedy ? rows_s[1] : Part{0.f, 0, 0.0};
+    const Part p = j < KEPT ? p_s[j] : rows_s[0], q = j < n && d.q && !greedy ? (j < KEPT ? q_s[j] : rows_s[1]) : Part{0.f, 0, 0.0};
     if (greedy || p.sum <= 0.0) {                       // (the whole cluster alike)
         if (rank == 0 && threadIdx.x == 0) { d.accepted[b] = j; d.next[b] = p.top > -INFINITY ? p.at : -1; }
         return;
@@ -241,7 +245,8 @@ race_kernel(Draft d, int parts) {
     for (int pass = 0; pass < 2; ++pass) {              // the second only where p exceeds q nowhere: the race over p itself
         // f32 brackets every key (its p and q are 1e-5 of themselves off at most, a tenth of what is allowed for).  Places whose upper end stays below the best lower end of the
         // whole row cannot win; the few others' keys are computed in 64 bits.
-        float low = 0.f, high = 0.f;                    // best lower and upper ends among this thread's places
+        float low = 0.f, high = 0.f, second = 0.f;      // best lower end, two best upper ends among this thread's places
+        int high_at = 0;
         auto bracket = [&](int i, float xv, float yv, float uv, float& lo_key, float& hi_key) {
             const float pi = xv == -INFINITY || (pass == 0 && i == sure) ? 0.f : ex2(below(xv, p.top) * c) * pz, qi = yv == -INFINITY ? 0.f : ex2(below(yv, q.top) * c) * qz;
             const float slack = 1e-4f * (pi + qi), inv = __fdividef(1.f, -logf(fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f)));
@@ -276,7 +281,8 @@ race_kernel(Draft d, int parts) {
             float a, z;
             bracket(i, xv, yv, uv, a, z);
             low = fmaxf(low, a);
-            high = fmaxf(high, z);
+            if (z > high) { second = high; high = z; high_at = i; }
+            else second = fmaxf(second, z);
         });
         float bar = warp_max(low);
         if (lane == 0) bars_s[warp] = bar;
@@ -294,16 +300,23 @@ race_kernel(Draft d, int parts) {
         }
         double best = 0.0;
         int at = INT_MAX;
-        if (high > 0.f && high >= bar)
-            all([&](int i, float xv, float yv, float uv) {
-                float a, z;
-                bracket(i, xv, yv, uv, a, z);
-                if (!(z > 0.f && z >= bar)) return;
-                const double w = share(xv, p, inv_t) - (yv == -INFINITY ? 0.0 : share(yv, q, inv_t));
-                if (!(w > 0.0)) return;
-                const double key = w / -log((double)fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f));
-                if (key > best || (key == best && i < at)) { best = key; at = i; }
-            });
+        auto exactly = [&](int i, float xv, float yv, float uv) {
+            const double w = share(xv, p, inv_t) - (yv == -INFINITY ? 0.0 : share(yv, q, inv_t));
+            if (!(w > 0.0)) return;
+            const double key = w / -log((double)fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f));
+            if (key > best || (key == best && i < at)) { best = key; at = i; }
+        };
+        if (high > 0.f && high >= bar) {
+            if (second < bar || second <= 0.f) {
+                exactly(high_at, clean(to_f<T>(x[high_at])), y && pass == 0 ? clean(to_f<T>(y[high_at])) : -INFINITY, __ldg(u + high_at));
+            } else {
+                all([&](int i, float xv, float yv, float uv) {
+                    float a, z;
+                    bracket(i, xv, yv, uv, a, z);
+                    if (z > 0.f && z >= bar) exactly(i, xv, yv, uv);
+                });
+            }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             const double k2 = __shfl_xor_sync(0xffffffffu, best, o);

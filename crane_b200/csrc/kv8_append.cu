@@ -10,40 +10,37 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace cb {
 namespace {
 
-constexpr int AP_THREADS = 128;
+constexpr int CHUNKS = 8;                      // of eight columns that a thread has: a page and head stay in registers from their maximum to their codes
 
-__device__ __forceinline__ float ld1(const void* p, int type, long long i) {
-    if (type == KV8_F32) return __ldg(reinterpret_cast<const float*>(p) + i);
-    const unsigned short u = __ldg(reinterpret_cast<const unsigned short*>(p) + i);
-    return type == KV8_BF16 ? __uint_as_float((uint32_t)u << 16) : __half2float(__ushort_as_half(u));
-}
-// Eight columns; VEC: aligned to 16 bytes
-template <bool VEC>
-__device__ __forceinline__ void ld8(const void* p, int type, long long i, float* y) {
-    if constexpr (VEC) {
-        if (type == KV8_F32) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + i) + 1);
-            y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w; y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
-            return;
-        }
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const unsigned short*>(p) + i));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// Eight columns as they lie (VEC: on 16-byte boundaries), and as numbers
+template <typename T> struct Eight {
+    uint32_t w[2 * sizeof(T)];
+    template <bool VEC> __device__ __forceinline__ void load(const T* p) {
+        if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (type == KV8_BF16) { y[2 * j] = bf16lo(w[j]); y[2 * j + 1] = bf16hi(w[j]); }
-            else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j])); y[2 * j] = f.x; y[2 * j + 1] = f.y; }
-        }
-    } else {
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) { const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i); w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w; }
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = ld1(p, type, i + j);
+            for (int i = 0; i < 8; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+        } else {
+            const unsigned short* s = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = __ldg(s + 2 * i) | (uint32_t)__ldg(s + 2 * i + 1) << 16;
+        }
     }
-}
+    __device__ __forceinline__ float2 pair(int i) const {                    // columns 2 i and 2 i + 1
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[(2 * i) % (2 * sizeof(T))]), __uint_as_float(w[(2 * i + 1) % (2 * sizeof(T))]));
+        else if constexpr (std::is_same<T, bf16>::value) return make_float2(bf16lo(w[i]), bf16hi(w[i]));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    }
+};
 __device__ __forceinline__ uint32_t codes2(float a, float b) {
     uint16_t r;
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(b), "f"(a));
@@ -66,12 +63,12 @@ __device__ __forceinline__ int search(int n, int at, K key) {
 }
 
 // blockIdx.x: a piece (kv8_units.h)
-template <bool VEC, bool BY_ROW>
-__global__ void __launch_bounds__(AP_THREADS)
+template <typename T, int THREADS, bool VEC, bool BY_ROW>
+__global__ void __launch_bounds__(THREADS)
 append_kernel(Kv8Rows kr, Kv8Rows vr, Kv8Pool pool, Kv8Seqs s) {
     pdl_wait();
     pdl_launch_dependents();
-    __shared__ float wmax[AP_THREADS / 32];
+    __shared__ float wmax[THREADS / 32];
     const int P = pool.page, D = pool.dim, at = blockIdx.x, head = blockIdx.y, half = blockIdx.z, tid = threadIdx.x;
     const int b = search(s.seqs, at, [&](int i) { return kv8_piece_key(s, P, i, BY_ROW); });
     const Kv8Seq q = kv8_seq(s, b);
@@ -82,22 +79,30 @@ append_kernel(Kv8Rows kr, Kv8Rows vr, Kv8Pool pool, Kv8Seqs s) {
     if (page < 0) return;
     const Kv8Rows& x = half ? vr : kr;
     const long long base = (long long)(q.s0 + pos - q.first) * x.ld + (long long)head * x.ldh;
-    const int cpr = D / 8, total = count * cpr, kept = pos - block * P;
+    const int cpr = D / 8, total = count * cpr, kept = pos - block * P;      // (at most THREADS * CHUNKS)
     float top = 0.f;
-    for (int c = tid; c < total; c += AP_THREADS) {
-        float y[8];
-        const int r = c / cpr;
-        ld8<VEC>(x.p, x.type, base + r * x.ld + (c - r * cpr) * 8, y);
+    Eight<T> y[CHUNKS];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (!infinite(y[j])) top = fmaxf(top, fabsf(y[j]));
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int c = tid + i * THREADS, row = c / cpr;
+        if (c < total) y[i].template load<VEC>(reinterpret_cast<const T*>(x.p) + base + row * x.ld + (c - row * cpr) * 8);
     }
-    top = warp_max(top);
-    if ((tid & 31) == 0) wmax[tid >> 5] = top;
     float* sp = pool.scales + ((size_t)page * pool.kv_heads + head) * 2 + half;
     const float own = kept ? *sp : 0.f;
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i)
+        if (tid + i * THREADS < total)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 v = y[i].pair(j);
+                if (!infinite(v.x)) top = fmaxf(top, fabsf(v.x));
+                if (!infinite(v.y)) top = fmaxf(top, fabsf(v.y));
+            }
+    top = warp_max(top);
+    if ((tid & 31) == 0) wmax[tid >> 5] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < AP_THREADS / 32; ++w) top = fmaxf(top, wmax[w]);
+    for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, wmax[w]);
     top = fmaxf(top, 0x1p-100f);
     const uint32_t bits = __float_as_uint(top);                      // top = m 2^(E - 127), m in [1, 2); 448 = 1.75 x 2^8
     const uint32_t e = (bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u);
@@ -106,7 +111,7 @@ append_kernel(Kv8Rows kr, Kv8Rows vr, Kv8Pool pool, Kv8Seqs s) {
     unsigned char* dst = (half ? pool.v : pool.k) + ((size_t)page * pool.kv_heads + head) * P * D;
     if (kept && scale != own) {                                      // (uniform in the CTA)
         const float ratio = own * inv;
-        for (int c = tid; c < kept * D / 8; c += AP_THREADS) {
+        for (int c = tid; c < kept * D / 8; c += THREADS) {
             uint2* p = reinterpret_cast<uint2*>(dst) + c;
             uint2 u = *p;
             uint32_t* w = &u.x;
@@ -126,21 +131,18 @@ append_kernel(Kv8Rows kr, Kv8Rows vr, Kv8Pool pool, Kv8Seqs s) {
         }
     }
     dst += (size_t)kept * D;
-    for (int c = tid; c < total; c += AP_THREADS) {
-        float y[8];
-        const int r = c / cpr;
-        ld8<VEC>(x.p, x.type, base + r * x.ld + (c - r * cpr) * 8, y);
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+        const int c = tid + i * THREADS;
+        if (c >= total) break;
         uint2 u;
         uint32_t* w = &u.x;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            uint32_t v = 0;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float a = y[4 * i + 2 * j], c2 = y[4 * i + 2 * j + 1];
-                v |= codes2(infinite(a) ? NAN : a * inv, infinite(c2) ? NAN : c2 * inv) << (16 * j);
-            }
-            w[i] = v;
+        for (int k = 0; k < 4; ++k) {
+            const float2 v = y[i].pair(k);
+            const uint32_t two = codes2(infinite(v.x) ? NAN : v.x * inv, infinite(v.y) ? NAN : v.y * inv);
+            if (k & 1) w[k >> 1] |= two << 16;
+            else w[k >> 1] = two;
         }
         reinterpret_cast<uint2*>(dst)[c] = u;
     }
@@ -159,8 +161,18 @@ int kv8_append_launch(cudaStream_t st, const Kv8Rows& k, const Kv8Rows& v, const
     const long long slots = (long long)s.rows / pool.page + 2LL * s.seqs;
     const bool vec = vec_ok(k) && vec_ok(v), by_row = s.rows <= slots;
     const dim3 grid((unsigned)(by_row ? s.rows : slots), pool.kv_heads, 2);
-    auto f = vec ? (by_row ? append_kernel<true, true> : append_kernel<true, false>) : (by_row ? append_kernel<false, true> : append_kernel<false, false>);
-    return launch_k(f, grid, dim3(AP_THREADS), 0, st, pdl, k, v, pool, s);
+    const int threads = pool.page * pool.dim / (8 * CHUNKS);
+    auto go = [&](auto type, auto count) {
+        using T = decltype(type);
+        constexpr int N = decltype(count)::value;
+        auto f = vec ? (by_row ? append_kernel<T, N, true, true> : append_kernel<T, N, true, false>) : (by_row ? append_kernel<T, N, false, true> : append_kernel<T, N, false, false>);
+        return launch_k(f, grid, dim3(N), 0, st, pdl, k, v, pool, s);
+    };
+    auto sized = [&](auto type) {
+        if (threads <= 128) return go(type, std::integral_constant<int, 128>());
+        return threads == 256 ? go(type, std::integral_constant<int, 256>()) : go(type, std::integral_constant<int, 512>());
+    };
+    return k.type == KV8_F32 ? sized(float()) : k.type == KV8_BF16 ? sized(bf16()) : sized(__half());
 }
 
 }  // namespace cb

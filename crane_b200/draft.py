@@ -15,6 +15,10 @@ from .fp8 import _F32, _failed, _matrix, _raw_stream, _refuse, _rows_in
 from .kv8 import _entry, _ints
 
 
+_I32 = torch.int32
+_sizes = {}                # bytes of workspaces by what they depend on
+
+
 def _floats(what: str, t, dev: int, n: int):
     if not isinstance(t, torch.Tensor) or t.dtype is not _F32 or t.shape != (n,) or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
         _refuse(f"{what}: {n} contiguous f32 values on cuda:{dev} are wanted")
@@ -36,22 +40,42 @@ def verify(logits, tokens, starts, uniforms, noise, *, draft_logits=None, temper
     seqs = rows - total
     if seqs < 0:
         _refuse(f"logits: {rows} rows for {total} drafts and a row more for each sequence")
-    tp, sp = _ints("tokens", tokens, dev, (total,)), _ints("starts", starts, dev, (seqs + 1,))
-    up = _floats("uniforms", uniforms, dev, total)
-    ldn = _matrix("noise", noise, (_F32,), logits.device, (seqs, vocab))
-    ldq = 0 if draft_logits is None else _matrix("draft_logits", draft_logits, (logits.dtype,), logits.device, (total, vocab))
-    temps = None if temperatures is None else _floats("temperatures", temperatures, dev, seqs)
     if out is None:
-        out = torch.empty((2, seqs), dtype=torch.int32, device=logits.device).unbind(0)
+        out = torch.empty((2, seqs), dtype=_I32, device=logits.device).unbind(0)
     accepted, following = out
-    ap, fp = _ints("out[0]", accepted, dev, (seqs,)), _ints("out[1]", following, dev, (seqs,))
-    need = C.c_size_t()
-    rc = _entry("draft_verify_bytes")(dev, vocab, seqs, total, draft_logits is not None, C.byref(need))
-    if rc:
-        _failed(rc)
-    work = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
-    rc = _entry("draft_verify")(dev, logits.data_ptr(), ld, None if draft_logits is None else draft_logits.data_ptr(), ldq, dtype, vocab, tp, sp, seqs, total, temps, up,
-                                noise.data_ptr(), ldn, ap, fp, work.data_ptr(), need.value, _raw_stream(dev))
+    q, temps = draft_logits, temperatures
+    try:
+        ldn, step = noise.stride()
+        ldq, qstep = (0, 1) if q is None else q.stride()
+        good = (step == qstep == 1 and tokens.dtype is _I32 and starts.dtype is _I32 and accepted.dtype is _I32 and following.dtype is _I32 and uniforms.dtype is _F32 and noise.dtype is _F32
+                and starts.shape == (seqs + 1,) and uniforms.shape == (total,) and noise.shape == (seqs, vocab) and accepted.shape == (seqs,) and following.shape == (seqs,)
+                and dev == tokens.get_device() == starts.get_device() == uniforms.get_device() == noise.get_device() == accepted.get_device() == following.get_device()
+                and (q is None or (q.dtype is logits.dtype and q.shape == (total, vocab) and q.get_device() == dev and ldq >= vocab)) and ldn >= vocab
+                and (temps is None or (temps.dtype is _F32 and temps.shape == (seqs,) and temps.get_device() == dev and temps.is_contiguous()))
+                and tokens.is_contiguous() and starts.is_contiguous() and uniforms.is_contiguous() and accepted.is_contiguous() and following.is_contiguous())
+    except (AttributeError, ValueError):
+        good = False
+    if not good:                                        # one by one, to name what is wrong or find a rarer layout good
+        _ints("tokens", tokens, dev, (total,)), _ints("starts", starts, dev, (seqs + 1,)), _ints("out[0]", accepted, dev, (seqs,)), _ints("out[1]", following, dev, (seqs,))
+        _floats("uniforms", uniforms, dev, total)
+        ldn = _matrix("noise", noise, (_F32,), logits.device, (seqs, vocab))
+        ldq = 0 if q is None else _matrix("draft_logits", q, (logits.dtype,), logits.device, (total, vocab))
+        if temps is not None:
+            _floats("temperatures", temps, dev, seqs)
+    key = (dev, vocab, seqs, total, q is not None)
+    need = _sizes.get(key)
+    if need is None:
+        n = C.c_size_t()
+        rc = _entry("draft_verify_bytes")(*key, C.byref(n))
+        if rc:
+            _failed(rc)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        need = _sizes[key] = n.value
+    work = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    rc = _entry("draft_verify")(dev, logits.data_ptr(), ld, None if q is None else q.data_ptr(), ldq, dtype, vocab, tokens.data_ptr(), starts.data_ptr(), seqs, total,
+                                None if temps is None else temps.data_ptr(), uniforms.data_ptr(), noise.data_ptr(), ldn, accepted.data_ptr(), following.data_ptr(), work.data_ptr(), need,
+                                _raw_stream(dev))
     if rc:
         _failed(rc)
     return accepted, following

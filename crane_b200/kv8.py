@@ -19,6 +19,7 @@ from .fp8 import _DTYPES, _failed, _raw_stream, _refuse, CODES
 
 _F32, _I32 = torch.float32, torch.int32
 _fn = {}
+_sizes = {}                # bytes of workspaces by what they depend on
 
 
 def _entry(name: str):
@@ -38,10 +39,10 @@ def _cache(cache):
     """(pointers, sizes, device index) of a cache."""
     try:
         k, v, scales = cache
-        dev = k.get_device()
-        n, h, p, d = k.shape
-        if (k.dtype is CODES and v.dtype is CODES and scales.dtype is _F32 and v.shape == k.shape and scales.shape == (n, h, 2) and dev >= 0 and dev == v.get_device()
-                and dev == scales.get_device() and k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
+        shape, dev = k.shape, k.get_device()
+        n, h, p, d = shape
+        if (k.dtype is CODES and v.dtype is CODES and scales.dtype is _F32 and v.shape == shape and scales.shape == (n, h, 2) and dev >= 0 and dev == v.get_device() == scales.get_device()
+                and k.is_contiguous() and v.is_contiguous() and scales.is_contiguous()):
             return (k.data_ptr(), v.data_ptr(), scales.data_ptr(), n, h, p, d), dev
     except (AttributeError, TypeError, ValueError):
         pass
@@ -56,30 +57,42 @@ def _ints(what: str, t, dev: int, shape):
     return t.data_ptr()
 
 
+# As in fp8.py: one look tells that all is in order; what it does not find goes through the checks one by one, which name what is wrong or find the rarer layouts good.
 def _seqs(table, lens, starts, dev: int):
+    try:
+        seqs, width = table.shape
+        ldt, step = table.stride()
+        if (step == 1 and table.dtype is _I32 and lens.dtype is _I32 and starts.dtype is _I32 and lens.shape == (seqs,) and starts.shape == (seqs + 1,) and lens.is_contiguous()
+                and starts.is_contiguous() and dev == table.get_device() == lens.get_device() == starts.get_device()):
+            return table.data_ptr(), max(ldt, width), width, lens.data_ptr(), starts.data_ptr(), seqs
+    except (AttributeError, ValueError):
+        pass
     t = _ints("table", table, dev, (None, None))
     seqs, width = table.shape
-    return (t, table.stride(0) if seqs > 1 else width, width, _ints("lens", lens, dev, (seqs,)), _ints("starts", starts, dev, (seqs + 1,)), seqs)
+    return t, table.stride(0) if seqs > 1 else width, width, _ints("lens", lens, dev, (seqs,)), _ints("starts", starts, dev, (seqs + 1,)), seqs
 
 
 def _rows(what: str, x, dev: int, rows, heads, dim: int, dtype=None):
-    """(address, row distance, head distance) of [rows, heads, dim] with contiguous columns."""
-    if (not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES or (dtype is not None and x.dtype is not dtype) or x.get_device() != dev or x.shape[2] != dim
-            or (rows is not None and x.shape[0] != rows) or (heads is not None and x.shape[1] != heads)):
-        _refuse(f"{what}: [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}] of {dtype or 'f32, bf16 or f16'} on cuda:{dev} is wanted")
-    ld, ldh, step = x.stride()
-    if step != 1:
+    """(address, row distance, head distance, type) of [rows, heads, dim] with contiguous columns."""
+    try:
+        (r, h, d), (ld, ldh, step), t = x.shape, x.stride(), x.dtype
+        code = _DTYPES.get(t)
+        if step == 1 and d == dim and code is not None and (dtype is None or t is dtype) and x.get_device() == dev and (rows is None or r == rows) and (heads is None or h == heads):
+            return x.data_ptr(), ld, ldh if h > 1 else dim, code
+    except (AttributeError, ValueError):
+        pass
+    if isinstance(x, torch.Tensor) and x.dim() == 3 and x.stride(2) != 1 and x.shape[2] == dim:
         _refuse(f"{what}: its columns are not contiguous")
-    return x.data_ptr(), ld, ldh if x.shape[1] > 1 else dim
+    _refuse(f"{what}: [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}] of {dtype or 'f32, bf16 or f16'} on cuda:{dev} is wanted")
 
 
 def append(k, v, cache, table, lens, starts):
     """Rows k and v [rows, kv_heads, dim] (f32, bf16 or f16; any row and head distance) into the pages of their sequences."""
     c, dev = _cache(cache)
-    kp, ldk, ldkh = _rows("k", k, dev, None, c[4], c[6])
-    vp, ldv, ldvh = _rows("v", v, dev, k.shape[0], c[4], c[6], k.dtype)
-    t, ldt, width, l, s, seqs = _seqs(table, lens, starts, dev)
-    rc = _entry("kv8_append")(dev, kp, ldk, ldkh, vp, ldv, ldvh, _DTYPES[k.dtype], *c, t, ldt, width, l, s, seqs, k.shape[0], _raw_stream(dev))
+    kp, ldk, ldkh, code = _rows("k", k, dev, None, c[4], c[6])
+    rows = k.shape[0]
+    vp, ldv, ldvh, _ = _rows("v", v, dev, rows, c[4], c[6], k.dtype)
+    rc = _entry("kv8_append")(dev, kp, ldk, ldkh, vp, ldv, ldvh, code, *c, *_seqs(table, lens, starts, dev), rows, _raw_stream(dev))
     if rc:
         _failed(rc)
     return cache
@@ -89,22 +102,25 @@ def attention(q, cache, table, lens, starts, *, scale: float = None, max_rows: i
     """q [rows, heads, dim] (f32, bf16 or f16) over the cache -> out of q's shape and type.  `scale`: None is dim ** -0.5.  `max_rows`: the most rows that any sequence brings, 0 if
     not known: decode rounds run faster when it is.  Rows of no sequence are left as they are (in a result that is made here: zeros)."""
     c, dev = _cache(cache)
-    qp, ldq, ldqh = _rows("q", q, dev, None, None, c[6])
-    rows, heads, dim = q.shape
-    if heads == 0 or heads % max(c[4], 1):
-        _refuse(f"q: {heads} heads over {c[4]} of the cache")
-    t, ldt, width, l, s, seqs = _seqs(table, lens, starts, dev)
+    kv_heads, dim = c[4], c[6]
+    qp, ldq, ldqh, code = _rows("q", q, dev, None, None, dim)
+    rows, heads, _ = q.shape
+    s = _seqs(table, lens, starts, dev)
     if out is None:
         out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
-    op, ldo, ldoh = _rows("out", out, dev, rows, heads, dim, q.dtype)
-    stream = _raw_stream(dev)
-    need = C.c_size_t()
-    rc = _entry("kv8_attention_bytes")(dev, _DTYPES[q.dtype], heads, c[4], dim, seqs, rows, max_rows, C.byref(need))
-    if rc:
-        _failed(rc)
-    work = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-    rc = _entry("kv8_attention")(dev, qp, ldq, ldqh, op, ldo, ldoh, _DTYPES[q.dtype], heads, dim ** -0.5 if scale is None else scale, *c, t, ldt, width, l, s, seqs, rows, max_rows,
-                                 work.data_ptr(), need.value, stream)
+    op, ldo, ldoh, _ = _rows("out", out, dev, rows, heads, dim, q.dtype)
+    key = (dev, code, heads, kv_heads, dim, s[5], rows, max_rows)
+    need = _sizes.get(key)
+    if need is None:
+        n = C.c_size_t()
+        rc = _entry("kv8_attention_bytes")(*key, C.byref(n))
+        if rc:
+            _failed(rc)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        need = _sizes[key] = n.value
+    work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    rc = _entry("kv8_attention")(dev, qp, ldq, ldqh, op, ldo, ldoh, code, heads, dim ** -0.5 if scale is None else scale, *c, *s, rows, max_rows, work.data_ptr(), need, _raw_stream(dev))
     if rc:
         _failed(rc)
     return out
