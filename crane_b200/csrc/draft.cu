@@ -27,7 +27,7 @@ template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_f<bf16>(bf16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
-__device__ __forceinline__ float clean(float x) { return x == x ? x : -INFINITY; }
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }      // (NaN: -inf)
 __device__ __forceinline__ float below(float x, float top) { return x == top ? 0.f : x - top; }      // infinities by themselves
 // log2 e / T as f32, kept off zero and infinity so that 0 and -inf stay what they are under it
 __device__ __forceinline__ float rate(float temp) { return fminf(fmaxf((float)(LOG2E / (double)temp), 0x1p-126f), 0x1p127f); }
@@ -243,15 +243,21 @@ race_kernel(Draft d, int parts) {
     constexpr int N = 16 / (int)sizeof(T);
     const bool wide = ((reinterpret_cast<uintptr_t>(x + lo) | (y ? reinterpret_cast<uintptr_t>(y + lo) : 0) | reinterpret_cast<uintptr_t>(u + lo)) & 15) == 0;
     for (int pass = 0; pass < 2; ++pass) {              // the second only where p exceeds q nowhere: the race over p itself
-        // f32 brackets every key (its p and q are 1e-5 of themselves off at most, a tenth of what is allowed for).  Places whose upper end stays below the best lower end of the
-        // whole row cannot win; the few others' keys are computed in 64 bits.
+        // f32 brackets every key (its p, q and clock are 6e-5 of themselves off at most, a third of what is allowed for).  Places whose upper end stays below the best lower end
+        // of the whole row cannot win; the few others' keys are computed in 64 bits.
         float low = 0.f, high = 0.f, second = 0.f;      // best lower end, two best upper ends among this thread's places
         int high_at = 0;
+        // p = 2^(x c + bp) in one step where the rounding of its terms stays below 2^-14; not for infinite or far maxima
+        const float tp = p.top * c, tq = q.top * c, bp = __log2f(pz) - tp, bq = y ? __log2f(qz) - tq : 0.f;
+        const bool near = fabsf(tp) < 500.f && (!y || fabsf(tq) < 500.f);
         auto bracket = [&](int i, float xv, float yv, float uv, float& lo_key, float& hi_key) {
-            const float pi = xv == -INFINITY || (pass == 0 && i == sure) ? 0.f : ex2(below(xv, p.top) * c) * pz, qi = yv == -INFINITY ? 0.f : ex2(below(yv, q.top) * c) * qz;
-            const float slack = 1e-4f * (pi + qi), inv = __fdividef(1.f, -logf(fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f)));
-            lo_key = (pi - qi - slack) * inv * 0.9999f;
-            hi_key = (pi - qi + slack) * inv * 1.0001f;
+            float pi = near ? ex2(fmaf(xv, c, bp)) : xv == -INFINITY ? 0.f : ex2(below(xv, p.top) * c) * pz;
+            const float qi = !y || pass ? 0.f : near ? ex2(fmaf(yv, c, bq)) : yv == -INFINITY ? 0.f : ex2(below(yv, q.top) * c) * qz;
+            if (i == sure && pass == 0) pi = 0.f;
+            const float slack = 2e-4f * (pi + qi), z = fminf(fmaxf(uv, 0x1p-126f), 0x1.fffffep-1f), w = 1.f - z;
+            const float clock = w < 0.02f ? w * fmaf(w, fmaf(w, 0.33333334f, 0.5f), 1.f) : -0.69314718f * __log2f(z), inv = __fdividef(1.f, clock);
+            lo_key = (pi - qi - slack) * inv;
+            hi_key = (pi - qi + slack) * inv;
         };
         auto all = [&](auto&& f) {                      // f(i, x, y, u) over this thread's places
             if (wide) {
@@ -287,17 +293,14 @@ race_kernel(Draft d, int parts) {
         float bar = warp_max(low);
         if (lane == 0) bars_s[warp] = bar;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < RACERS / 32; ++w) bar = fmaxf(bar, bars_s[w]);
-            bar_s = bar;
+        if (warp == 0) {
+            bar = warp_max(lane < RACERS / 32 ? bars_s[lane] : 0.f);
+            if (lane == 0) bar_s = bar;
         }
         cluster_sync_all();
-        bar = 0.f;
-        for (int r = 0; r < CLUSTER; ++r) {
-            float v;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer_smem(&bar_s, r)) : "memory");
-            bar = fmaxf(bar, v);
-        }
+        bar = 0.f;                                      // (a lane for each CTA)
+        if (lane < CLUSTER) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(bar) : "r"(peer_smem(&bar_s, lane)) : "memory");
+        bar = warp_max(bar);
         double best = 0.0;
         int at = INT_MAX;
         auto exactly = [&](int i, float xv, float yv, float uv) {
@@ -317,30 +320,31 @@ race_kernel(Draft d, int parts) {
                 });
             }
         }
+        auto reduce = [&]() {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const double k2 = __shfl_xor_sync(0xffffffffu, best, o);
-            const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
-            if (k2 > best || (k2 == best && a2 < at)) { best = k2; at = a2; }
-        }
+            for (int o = 16; o > 0; o >>= 1) {
+                const double k2 = __shfl_xor_sync(0xffffffffu, best, o);
+                const int a2 = __shfl_xor_sync(0xffffffffu, at, o);
+                if (k2 > best || (k2 == best && a2 < at)) { best = k2; at = a2; }
+            }
+        };
+        if (__any_sync(0xffffffffu, best > 0.0)) reduce();
         if (lane == 0) { key_s[warp] = best; at_s[warp] = at; }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < RACERS / 32; ++w)
-                if (key_s[w] > best || (key_s[w] == best && at_s[w] < at)) { best = key_s[w]; at = at_s[w]; }
-            best_s = best;
-            best_at_s = at;
+        if (warp == 0) {
+            best = lane < RACERS / 32 ? key_s[lane] : 0.0;
+            at = lane < RACERS / 32 ? at_s[lane] : INT_MAX;
+            reduce();
+            if (lane == 0) { best_s = best; best_at_s = at; }
         }
         cluster_sync_all();
         best = 0.0;
         at = INT_MAX;
-        for (int r = 0; r < CLUSTER; ++r) {
-            double k2;
-            int a2;
-            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(k2) : "r"(peer_smem(&best_s, r)) : "memory");
-            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(a2) : "r"(peer_smem(&best_at_s, r)) : "memory");
-            if (k2 > best || (k2 == best && a2 < at)) { best = k2; at = a2; }
+        if (lane < CLUSTER) {
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(best) : "r"(peer_smem(&best_s, lane)) : "memory");
+            asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(at) : "r"(peer_smem(&best_at_s, lane)) : "memory");
         }
+        reduce();
         cluster_sync_all();                             // (read: it may be written again, or its owner leave)
         if (best > 0.0 || pass == 1) {
             if (rank == 0 && threadIdx.x == 0) { d.accepted[b] = j; d.next[b] = best > 0.0 ? at : -1; }      // (a row's largest logit always has a key)
