@@ -42,29 +42,73 @@ template <typename T, int N> struct Piece {
         }
     }
 };
-template <typename T, int N, bool VEC>
+// Any boundary: the aligned 16 bytes that hold one of them, moved into place.  RO: nobody writes them while the kernel runs.
+template <typename T, int N, bool VEC, bool RO = true>
 __device__ __forceinline__ Piece<T, N> load(const T* p, int have) {
     Piece<T, N> r;
-#pragma unroll
-    for (int i = 0; i < r.W; ++i) r.w[i] = 0;
+    constexpr int W = Piece<T, N>::W;
+    auto get = [](const uint4* q) { if constexpr (RO) return __ldg(q); else return *q; };
     if constexpr (VEC) {
-        if (have >= N) {
 #pragma unroll
-            for (int i = 0; i < r.W; i += r.W < 4 ? 2 : 4) {
-                if constexpr (Piece<T, N>::W < 4) { const uint2 v = __ldg(reinterpret_cast<const uint2*>(p)); r.w[0] = v.x; r.w[1] = v.y; }
-                else { const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4); r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w; }
+        for (int i = 0; i < W; ++i) r.w[i] = 0;
+        if (have >= N) {
+            if constexpr (W < 4) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                r.w[0] = v.x; r.w[1] = v.y;
+            } else {
+#pragma unroll
+                for (int i = 0; i < W; i += 4) { const uint4 v = get(reinterpret_cast<const uint4*>(p) + i / 4); r.w[i % W] = v.x; r.w[(i + 1) % W] = v.y; r.w[(i + 2) % W] = v.z; r.w[(i + 3) % W] = v.w; }
             }
         }
     } else {
+        constexpr int B = (W + 3) / 4 + 1;                           // aligned pieces that may hold something of it
+        uint32_t w[4 * B + 1];
+        const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15), n = min(have, N) * (int)sizeof(T);
+        const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)15);
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < have) {
-                if constexpr (sizeof(T) == 4) r.w[i] = __float_as_uint(__ldg(reinterpret_cast<const float*>(p) + i));
-                else r.w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p) + i) << (16 * (i & 1));
-            }
+        for (int i = 0; i < B; ++i) {
+            const uint4 v = n > 0 && 16 * i < off + n ? get(q + i) : make_uint4(0, 0, 0, 0);
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
+        w[4 * B] = 0;
+#pragma unroll
+        for (int s = 2; s >= 1; s >>= 1)
+            if (off >> 2 & s)
+#pragma unroll
+                for (int i = 0; i + s <= 4 * B; ++i) w[i] = w[i + s];
+#pragma unroll
+        for (int i = 0; i < W; ++i) r.w[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], (off & 2) * 8);
+        if (n < N * (int)sizeof(T))
+#pragma unroll
+            for (int i = 0; i < W; ++i) r.w[i] &= n >= 4 * i + 4 ? 0xffffffffu : n <= 4 * i ? 0u : 0xffffu;
     }
     return r;
+}
+// Eight neighbours, `have` of them there
+template <typename T, bool VEC> __device__ __forceinline__ void store8(T* p, int have, const T* y) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(y);
+    constexpr int W = 2 * (int)sizeof(T);
+    if constexpr (VEC) {
+        if (have >= 8)
+#pragma unroll
+            for (int q = 0; q < W / 4; ++q) reinterpret_cast<uint4*>(p)[q] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
+    } else if (have >= 8) {                                          // 32 bits at a time, a single one at either end of an odd row
+        if (reinterpret_cast<uintptr_t>(p) & 2) {
+            p[0] = y[0];
+#pragma unroll
+            for (int q = 0; q < 3; ++q) *reinterpret_cast<uint32_t*>(p + 1 + 2 * q) = __funnelshift_r(w[q], w[q + 1], 16);
+            p[7] = y[7];
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) reinterpret_cast<uint32_t*>(p)[q] = w[q];
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
+    }
 }
 
 template <typename W> __device__ __forceinline__ void mma16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -93,12 +137,14 @@ struct Shape {
     static constexpr int EB = MT > 1 ? 1 : T32 && RT > 4 ? 1 : 2;    // blocks of 32 columns a warp has under way
     static constexpr int KS = T32 ? RT : RT / 2;                     // MMAs along the rank
     static constexpr int T_BYTES = ROWS * LDT * 4, FRAG = MT * KS * 32 * 16;
-    // Many rows: the columns of a step, add and B, come in through a ring of stages
+    // The columns of a step, add and B, come in through a ring of stages
     static constexpr int NC = CW * 32, ADD = ROWS * NC * (int)sizeof(X), STAGE = ADD + NC * RP * (int)sizeof(W);
-    static constexpr int CTAS = MT == 1 ? 2 : 2 * FRAG + 3 * STAGE <= 112 * 1024 ? 2 : 1;            // resident on an SM
-    static constexpr int FITS = ((CTAS == 2 ? 112 : 222) * 1024 - 2 * FRAG) / STAGE, STAGES = MT == 1 || FITS < 2 ? 0 : FITS > 4 ? 4 : FITS;
-    static constexpr int ROOM = STAGES * STAGE > 2 * T_BYTES ? STAGES * STAGE : 2 * T_BYTES;         // shares of T (this CTA's, read by the cluster) and T; later the stages
-    static constexpr int SMEM = 2 * FRAG + ROOM;                     // ahead of those the two parts of T
+    // Shares of T (this CTA's, read by the cluster) and T; where there are few rows the first stages are asked for ahead of them, otherwise they come into the same room
+    static constexpr int T_ROOM = 2 * T_BYTES, AHEAD = MT == 1;
+    static constexpr int CTAS = MT == 1 || 2 * FRAG + AHEAD * T_ROOM + 3 * STAGE <= 112 * 1024 ? 2 : 1;         // resident on an SM
+    static constexpr int FITS = ((CTAS == 2 ? 112 : 222) * 1024 - 2 * FRAG - AHEAD * T_ROOM) / STAGE, STAGES = MT == 1 || FITS < 2 ? 0 : FITS > 4 ? 4 : FITS;
+    static constexpr int ROOM = AHEAD ? T_ROOM + STAGES * STAGE : STAGES * STAGE > T_ROOM ? STAGES * STAGE : T_ROOM;
+    static constexpr int SMEM = 2 * FRAG + ROOM, RING = 2 * FRAG + AHEAD * T_ROOM;                   // ahead of those the two parts of T
 };
 
 // o += T B^T over 16 of the rank: EM row tiles from `er` on, 32 columns
@@ -139,7 +185,7 @@ __device__ __forceinline__ void multiply(float (&o)[EM][4][4], const Piece<W, 4>
 
 template <typename X, typename W, int MT, int RT, bool VEC>
 __global__ void __launch_bounds__(THREADS, Shape<X, W, MT, RT>::CTAS)
-lora_kernel(Lora l, bool gather) {
+lora_kernel(Lora l, bool gather, int slots) {
     using S = Shape<X, W, MT, RT>;
     constexpr bool T32 = S::T32;
     constexpr int ROWS = S::ROWS, LDT = S::LDT, KS = S::KS, MW = S::MW, KW = S::KW, MPW = S::MPW, EM = S::EM, EW = S::EW, CW = S::CW, EB = S::EB;
@@ -156,7 +202,7 @@ lora_kernel(Lora l, bool gather) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     uint32_t cl;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cl));
-    const int cr = (int)cluster_rank(), nc = (int)cl, tile = blockIdx.x / nc;
+    const int cr = (int)cluster_rank(), nc = (int)cl, tile = blockIdx.x / nc / slots, slot = blockIdx.x / nc % slots;
 
     // ---- the tile's rows ----
     if (gather) {
@@ -196,13 +242,58 @@ lora_kernel(Lora l, bool gather) {
     X* out = reinterpret_cast<X*>(l.out);
     const int nb = (l.n + 31) / 32, nb0 = (int)((long long)nb * cr / nc), nb1 = (int)((long long)nb * (cr + 1) / nc);
     unsigned long long left = n_rows == 64 ? ~0ull : (1ull << n_rows) - 1;
-    while (left) {
+    for (int turn = 0; left;) {
         // ---- the next adapter among the rows that are left ----
         const int w = which_s[__ffsll(left) - 1];
         unsigned long long mine = __ballot_sync(0xffffffffu, lane < ROWS && which_s[lane % ROWS] == w);
         if constexpr (ROWS > 32) mine |= (unsigned long long)__ballot_sync(0xffffffffu, which_s[(lane + 32) % ROWS] == w) << 32;
         mine &= left;
         left &= ~mine;
+        if (turn++ < slot || (slot + 1 < slots && turn - 1 > slot)) continue;      // another cluster's adapter
+        const W* B = reinterpret_cast<const W*>(l.b) + (size_t)max(w, 0) * l.n * l.rank;
+        // ---- the ring: a thread fetches the same piece of every AR-th row of add and of every BR-th row of B, whatever the step ----
+        constexpr bool STAGED = VEC && S::STAGES > 0;
+        constexpr int ST = S::STAGES, NC = S::NC, CX = NC * (int)sizeof(X) / 16, CB = S::RP * (int)sizeof(W) / 16, EX = 16 / (int)sizeof(X), EWT = 16 / (int)sizeof(W);
+        constexpr int AR = THREADS / CX, AK = ROWS / AR, BR = THREADS / CB, BK = NC / BR;
+        // (16-byte pieces of a row change places by row, so that what a warp reads of several rows lies in banks of its own)
+        auto add_at = [](int row, int c) { return (row * CX + (c ^ (sizeof(X) == 4 ? row & 1 : (row & 1) << 2))) * 16; };
+        auto b_at = [](int row, int c) { return (row * CB + (c ^ ((sizeof(W) == 4 ? (row & 1) << 2 : ((row & 1) | (row >> 2 & 2)) << 1) & (CB - 1)))) * 16; };
+        const int c0 = nb0 * 32, c1 = min(nb1 * 32, l.n), steps = (c1 - c0 + NC - 1) / NC;
+        const X* a_src = nullptr;                                    // rows of many are neighbours: one address
+        const W* b_src = nullptr;
+        uint32_t a_in = 0;
+        bool b_in = false;
+        auto setup = [&]() {
+#pragma unroll
+            for (int k = 0; k < AK; ++k) a_in |= (uint32_t)(add && (mine >> (tid / CX + k * AR) & 1)) << k;
+            if (MT > 1 && add) a_src = add + (long long)(tile * ROWS + tid / CX) * l.ldadd + c0 + tid % CX * EX;
+            b_in = tid % CB * EWT < l.rank;
+            b_src = B + (b_in ? (size_t)(c0 + tid / CB) * l.rank + tid % CB * EWT : 0);
+        };
+        auto copy = [](uint32_t dst, const void* src, bool in) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); };
+        auto fetch = [&](int step) {
+            const uint32_t st = smem_u32(sm) + S::RING + step % (ST > 0 ? ST : 1) * S::STAGE;
+            const int off = step * NC;
+            if (add) {
+                const bool here = c0 + off + tid % CX * EX < c1;
+                const uint32_t dst = st + add_at(tid / CX, tid % CX);
+#pragma unroll
+                for (int k = 0; k < AK; ++k) {
+                    const bool in = here && (a_in >> k & 1);
+                    const X* src = MT > 1 ? a_src + (long long)(k * AR) * l.ldadd + off : add + (in ? (long long)rows_s[tid / CX + k * AR] * l.ldadd + c0 + off + tid % CX * EX : 0);
+                    copy(dst + k * (THREADS * 16), in ? src : add, in);
+                }
+            }
+            if (w >= 0) {
+                const W* src = b_src + (size_t)off * l.rank;
+                const uint32_t dst = st + S::ADD + b_at(tid / CB, tid % CB);
+                const int left_n = b_in ? c1 - c0 - off - tid / CB : 0;
+#pragma unroll
+                for (int k = 0; k < BK; ++k) copy(dst + k * (THREADS * 16), k * BR < left_n ? src + (size_t)(k * BR) * l.rank : B, k * BR < left_n);
+            }
+        };
+        auto first = [&]() { for (int i = 0; i < ST - 1; ++i) { if (i < steps) fetch(i); asm volatile("cp.async.commit_group;" ::: "memory"); } };
+        if (STAGED && S::AHEAD && (w >= 0 || add != out)) { setup(); first(); }
         if (w >= 0) {
             // ---- this CTA's share of T ----
             const W* A = reinterpret_cast<const W*>(l.a) + (size_t)w * l.rank * l.k;
@@ -335,62 +426,23 @@ lora_kernel(Lora l, bool gather) {
             __syncthreads();
         }
         // ---- out = add + T B^T: EB blocks of 32 columns a warp at a time ----
-        const W* B = reinterpret_cast<const W*>(l.b) + (size_t)max(w, 0) * l.n * l.rank;
         const int er = warp % EW * EM;                               // this warp's first row tile
-        if constexpr (VEC && S::STAGES > 0) {
-            constexpr int ST = S::STAGES, NC = S::NC, CX = NC * (int)sizeof(X) / 16, CB = S::RP * (int)sizeof(W) / 16, EX = 16 / (int)sizeof(X), EWT = 16 / (int)sizeof(W);
-            // (16-byte pieces of a row change places by row, so that what a warp reads of several rows lies in banks of its own)
-            auto add_at = [](int row, int c) { return (row * CX + (c ^ (sizeof(X) == 4 ? row & 1 : (row & 1) << 2))) * 16; };
-            auto b_at = [](int row, int c) { return (row * CB + (c ^ ((sizeof(W) == 4 ? (row & 1) << 2 : ((row & 1) | (row >> 2 & 2)) << 1) & (CB - 1)))) * 16; };
-            unsigned char* ring = sm + 2 * S::FRAG;
-            const int c0 = nb0 * 32, c1 = min(nb1 * 32, l.n), steps = (c1 - c0 + NC - 1) / NC;
-            // A thread fetches the same piece of every AR-th row of add and of every BR-th row of B, whatever the step: addresses only advance
-            constexpr int AR = THREADS / CX, AK = ROWS / AR, BR = THREADS / CB, BK = NC / BR;
-            const int ac = tid % CX, bc = tid % CB, a_dst = add_at(tid / CX, ac), b_dst = S::ADD + b_at(tid / CB, bc);
-            const X* a_src[AK];
-            uint32_t a_in = 0;
-#pragma unroll
-            for (int k = 0; k < AK; ++k) {
-                const int row = tid / CX + k * AR;
-                const bool in = add && (mine >> row & 1);
-                a_in |= (uint32_t)in << k;
-                a_src[k] = add + (in ? (long long)rows_s[row] * l.ldadd + c0 + ac * EX : 0);
-            }
-            const bool b_in = bc * EWT < l.rank;
-            const W* b_src = B + (b_in ? (size_t)(c0 + tid / CB) * l.rank + bc * EWT : 0);
-            auto copy = [](uint32_t dst, const void* src, bool in) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); };
-            const uint32_t ring32 = smem_u32(ring);
-            auto fetch = [&](int step) {
-                const uint32_t st = ring32 + step % ST * S::STAGE;
-                const int off = step * NC;
-                if (add) {
-                    const bool here = c0 + off + ac * EX < c1;
-#pragma unroll
-                    for (int k = 0; k < AK; ++k) { const bool in = here && (a_in >> k & 1); copy(st + a_dst + k * (THREADS * 16), a_src[k] + (in ? off : 0), in); }
-                }
-                if (w >= 0) {
-                    const W* src = b_src + (size_t)off * l.rank;
-#pragma unroll
-                    for (int k = 0; k < BK; ++k) { const bool in = b_in && c0 + off + tid / CB + k * BR < c1; copy(st + b_dst + k * (THREADS * 16), in ? src + (size_t)(k * BR) * l.rank : B, in); }
-                }
-            };
-            const int cw = warp / EW * 32;
-            const bool idle = !(mine >> (er * 16) & ((1ull << (16 * EM)) - 1));      // none of this warp's rows
-            X* dst[EM][2];
-            uint32_t row_in = 0;
-            float downs[EM][2];
-#pragma unroll
-            for (int i = 0; i < EM; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = (er + i) * 16 + h * 8 + g;
-                    const bool in = mine >> row & 1;
-                    row_in |= (uint32_t)in << (2 * i + h);
-                    dst[i][h] = out + (in ? (long long)rows_s[row] * l.ldo : 0) + c0 + cw + t * 8;
-                    downs[i][h] = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[row] : 1.f;
-                }
+        if constexpr (STAGED) {
             if (w >= 0 || add != out) {
-                for (int i = 0; i < ST - 1; ++i) { if (i < steps) fetch(i); asm volatile("cp.async.commit_group;" ::: "memory"); }
+                if (!S::AHEAD) { setup(); first(); }
+                const bool idle = !(mine >> (er * 16) & ((1ull << (16 * EM)) - 1));      // none of this warp's rows
+                const int cw = warp / EW * 32;
+                uint32_t row_in = 0;
+                X* dst[EM][2];
+#pragma unroll
+                for (int i = 0; i < EM; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int row = (er + i) * 16 + h * 8 + g;
+                        const bool in = mine >> row & 1;
+                        row_in |= (uint32_t)in << (2 * i + h);
+                        dst[i][h] = out + (in ? (long long)rows_s[row] * l.ldo : 0) + c0 + cw + t * 8;
+                    }
 #pragma unroll 1
                 for (int step = 0; step < steps; ++step) {
                     asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
@@ -398,7 +450,7 @@ lora_kernel(Lora l, bool gather) {
                     if (step + ST - 1 < steps) fetch(step + ST - 1);
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (idle) continue;
-                    const unsigned char* st = ring + step % ST * S::STAGE;
+                    const unsigned char* st = sm + S::RING + step % ST * S::STAGE;
                     float o[EM][4][4];
 #pragma unroll
                     for (int i = 0; i < EM; ++i)
@@ -435,9 +487,10 @@ lora_kernel(Lora l, bool gather) {
                                     const uint4 v = add ? *reinterpret_cast<const uint4*>(st + add_at((er + i) * 16 + h * 8 + g, (cw + t * 8) / EX + q / 4)) : make_uint4(0, 0, 0, 0);
                                     av.w[q] = v.x; av.w[q + 1] = v.y; av.w[q + 2] = v.z; av.w[q + 3] = v.w;
                                 }
+                                const float down = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[(er + i) * 16 + h * 8 + g] : 1.f;
                                 __align__(16) X y[8];
 #pragma unroll
-                                for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[i][q >> 1][2 * h + (q & 1)], downs[i][h], av.at(q)));
+                                for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[i][q >> 1][2 * h + (q & 1)], down, av.at(q)));
 #pragma unroll
                                 for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(dst[i][h] + step * NC)[q] = reinterpret_cast<const uint4*>(y)[q];
                             }
@@ -457,25 +510,7 @@ lora_kernel(Lora l, bool gather) {
                         for (int h = 0; h < 2; ++h) {
                             const int r = (er + i) * 16 + h * 8 + g;
                             const bool in = add && (mine >> r & 1);
-#pragma unroll
-                            for (int q = 0; q < Piece<X, 8>::W; ++q) av[b][i][h].w[q] = 0;
-                            const X* p = add + (in ? (long long)rows_s[r] * l.ldadd : 0) + col;      // (may be out: not through the read-only path)
-                            if constexpr (VEC) {
-                                if (in && have >= 8) {
-#pragma unroll
-                                    for (int q = 0; q < Piece<X, 8>::W; q += 4) {
-                                        const uint4 v = reinterpret_cast<const uint4*>(p)[q / 4];
-                                        av[b][i][h].w[q] = v.x; av[b][i][h].w[q + 1] = v.y; av[b][i][h].w[q + 2] = v.z; av[b][i][h].w[q + 3] = v.w;
-                                    }
-                                }
-                            } else {
-#pragma unroll
-                                for (int q = 0; q < 8; ++q)
-                                    if (in && q < have) {
-                                        if constexpr (sizeof(X) == 4) av[b][i][h].w[q] = reinterpret_cast<const uint32_t*>(p)[q];
-                                        else av[b][i][h].w[q / 2] |= (uint32_t)reinterpret_cast<const unsigned short*>(p)[q] << (16 * (q & 1));
-                                    }
-                            }
+                            av[b][i][h] = load<X, 8, VEC, false>(add + (in ? (long long)rows_s[r] * l.ldadd : 0) + col, in ? have : 0);      // (may be out)
 #pragma unroll
                             for (int j = 0; j < 4; ++j) o[b][i][j][2 * h] = o[b][i][j][2 * h + 1] = 0.f;
                         }
@@ -507,17 +542,10 @@ lora_kernel(Lora l, bool gather) {
                             if (!(mine >> r & 1) || have <= 0) continue;
                             X* p = out + (long long)rows_s[r] * l.ldo + col;
                             const float down = TYPE<W> == 2 && !T32 && w >= 0 ? down_s[r] : 1.f;
-                            X y[8];
+                            __align__(16) X y[8];
 #pragma unroll
                             for (int q = 0; q < 8; ++q) y[q] = from_f<X>(fmaf(o[b][i][q >> 1][2 * h + (q & 1)], down, av[b][i][h].at(q)));
-                            if constexpr (VEC) {
-                                if (have >= 8)
-#pragma unroll
-                                    for (int q = 0; q < Piece<X, 8>::W / 4; ++q) reinterpret_cast<uint4*>(p)[q] = reinterpret_cast<const uint4*>(y)[q];
-                            } else {
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) if (q < have) p[q] = y[q];
-                            }
+                            store8<X, VEC>(p, have, y);
                         }
                 }
             }
@@ -532,15 +560,17 @@ int launch(cudaStream_t st, const Lora& l, bool gather, int cluster, bool pdl) {
     auto kernel = lora_kernel<X, W, MT, RT, VEC>;
     if (const int e = ensure_dyn_smem(kernel, (size_t)S::SMEM, seen)) return e;
     const int tiles = gather ? l.m : (l.m + S::ROWS - 1) / S::ROWS;
+    // A tile of neighbours may hold several adapters: the first few have a cluster each, the last one the rest
+    const int slots = gather ? 1 : tiles >= 75 ? 2 : tiles <= 9 ? 16 : 150 / tiles;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)tiles * cluster); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = st;
+    cfg.gridDim = dim3((unsigned)tiles * cluster * slots); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
-    return (int)cudaLaunchKernelEx(&cfg, kernel, l, gather);
+    return (int)cudaLaunchKernelEx(&cfg, kernel, l, gather, slots);
 }
 template <typename X, typename W, int MT, bool VEC>
 int launch_rank(cudaStream_t st, const Lora& l, bool gather, int cluster, bool pdl) {
