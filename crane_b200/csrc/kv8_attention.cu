@@ -594,15 +594,10 @@ join_kernel(Args a) {
 
 // Rows of a kv head from which on a sequence goes through kv8_flash.cu: 16-bit ones of 64 and 128 columns.
 constexpr int FLASH_FROM = 65;
-// Where some sequence may bring more rows than this, and none goes to kv8_flash.cu, those of up to so many run by themselves, 16 rows a group: a decoded token beside a prompt's
-// portion would have one warp of four at work (23 sequences, portions of up to 333 tokens among decoded ones, f32: 265 us in one, NNN in two)
-constexpr int MIXED_FROM = 32;
 bool flash_takes(int type, int dim, int group, int max_rows) { return type != KV8_F32 && dim <= 128 && (long long)group * max_rows >= FLASH_FROM; }
-// Rows of a group of queries, from the most that a sequence brings: 16 or 32 where that is enough, else 64 (or 32).  (Beside kv8_flash.cu 16: most of what is left are decoded tokens.)
-int rows_of(int group, int dim, int max_rows, bool flash) {
-    const long long r = (long long)group * max_rows;
-    return r <= 16 || flash ? 16 : r <= 32 || dim == 256 ? 32 : 64;
-}
+// Rows of a group of queries: 16, or 32 where some sequence may bring many and none goes to kv8_flash.cu.  Us, 16 / 32 / 64 rows: portions of 500 tokens, 16 heads over 8, f32 231 / 177 /
+// 190; up to 9 drafts, 32 heads over 8, bf16 45 / 52 / 87; 23 sequences, portions of up to 333 tokens among decoded ones, f32 245 / 234 / 267.
+int rows_of(int group, int max_rows, bool flash) { return flash || (long long)group * max_rows <= 64 ? 16 : 32; }
 template <typename T>
 int join_flash(cudaStream_t st, const Args& a) {
     auto k = a.d.p.dim == 64 ? join_kernel<64, T, KV8_FLASH_ROWS> : join_kernel<128, T, KV8_FLASH_ROWS>;
@@ -616,14 +611,11 @@ int launch(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const 
     if (const int e = ensure_dyn_smem(small_kernel<D, T, MG>, (size_t)S::SMEM, seen)) return e;
     const int ctas = tc_device_sms() * S::CTAS;
     if (const int e = launch_k(small_kernel<D, T, MG>, dim3(ctas), dim3(S::THREADS), S::SMEM, st, pdl, mk, mv, a)) return e;
-    return launch_k(join_kernel<D, T, S::M>, dim3(ctas - 1, S::M == 64 ? 64 : 4), dim3(128), 0, st, true, a);
+    return launch_k(join_kernel<D, T, S::M>, dim3(ctas - 1, S::M / 4), dim3(128), 0, st, true, a);
 }
 template <int D, typename T>
 int launch_rows(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int rows, bool pdl) {
-    if (rows == 16) return launch<D, T, 1>(st, mk, mv, a, pdl);
-    if (rows == 32) return launch<D, T, 2>(st, mk, mv, a, pdl);
-    if constexpr (D < 256) return launch<D, T, 4>(st, mk, mv, a, pdl);
-    return -1000;
+    return rows == 16 ? launch<D, T, 1>(st, mk, mv, a, pdl) : launch<D, T, 2>(st, mk, mv, a, pdl);
 }
 template <typename T>
 int launch_dim(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, int rows, bool pdl) {
@@ -640,7 +632,7 @@ int launch_dim(cudaStream_t st, const CUtensorMap& mk, const CUtensorMap& mv, co
 size_t kv8_attention_bytes(int type, int heads, int kv_heads, int dim, int rows, int seqs, int max_rows) {
     if (!rows || !seqs) return 0;
     const bool flash = flash_takes(type, dim, heads / kv_heads, max_rows);
-    const size_t small = (size_t)tc_device_sms() * 2 * 2 * rows_of(heads / kv_heads, dim, max_rows, flash), large = flash ? (size_t)tc_device_sms() * 2 * KV8_FLASH_ROWS : 0;
+    const size_t small = (size_t)tc_device_sms() * 2 * 2 * rows_of(heads / kv_heads, max_rows, flash), large = flash ? (size_t)tc_device_sms() * 2 * KV8_FLASH_ROWS : 0;
     return kv8_joins(2 * tc_device_sms()) + (small > large ? small : large) * (dim + 2) * 4;
 }
 
@@ -648,7 +640,7 @@ int kv8_attention_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Pool& 
     if (s.rows == 0 || s.seqs == 0) return 0;
     const int group = k.heads / pool.kv_heads;
     const bool flash = flash_takes(k.q.type, pool.dim, group, k.max_rows);
-    const int rows = rows_of(group, pool.dim, k.max_rows, flash), box = pool.dim < 128 ? pool.dim : 128;
+    const int rows = rows_of(group, k.max_rows, flash), box = pool.dim < 128 ? pool.dim : 128;
     const uint64_t n = (uint64_t)pool.pages * pool.kv_heads * pool.page;
     CUtensorMap mk, mv;
     const CUtensorMapSwizzle sw = box == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
@@ -660,17 +652,8 @@ int kv8_attention_launch(cudaStream_t st, const Kv8Attention& k, const Kv8Pool& 
     const bool vec = (reinterpret_cast<uintptr_t>(k.q.p) | reinterpret_cast<uintptr_t>(k.out)) % 16 == 0 && (k.q.ld | k.q.ldh | k.ldo | k.ldoh) % per == 0;
     const double scale2 = (double)k.scale * 1.4426950408889634074;
     const Args a = {k.q.p, k.q.ld, k.q.ldh, k.out, k.ldo, k.ldoh, (float)scale2, (float)(scale2 - (double)(float)scale2), Kv8Deal{s, pool, group, 0, flash ? FLASH_FROM - 1 : 1LL << 62}, reinterpret_cast<Kv8Join*>(k.work), reinterpret_cast<float*>(reinterpret_cast<char*>(k.work) + kv8_joins(2 * tc_device_sms())), k.err, vec};
-    auto go = [&](const Args& x, int m, bool dependent) {
-        return k.q.type == KV8_F32 ? launch_dim<float>(st, mk, mv, x, m, dependent) : k.q.type == KV8_BF16 ? launch_dim<bf16>(st, mk, mv, x, m, dependent) : launch_dim<__half>(st, mk, mv, x, m, dependent);
-    };
-    if (!flash && s.seqs > 1 && (long long)group * k.max_rows > MIXED_FROM) {
-        Args few = a, many = a;
-        few.d.hi = MIXED_FROM;
-        many.d.lo = MIXED_FROM + 1;
-        if (const int e = go(few, 16, pdl)) return e;
-        return go(many, rows, true);
-    }
-    if (const int e = go(a, rows, pdl)) return e;
+    const int e = k.q.type == KV8_F32 ? launch_dim<float>(st, mk, mv, a, rows, pdl) : k.q.type == KV8_BF16 ? launch_dim<bf16>(st, mk, mv, a, rows, pdl) : launch_dim<__half>(st, mk, mv, a, rows, pdl);
+    if (e) return e;
     if (!flash) return 0;
     Args f = a;
     f.d.lo = FLASH_FROM;
