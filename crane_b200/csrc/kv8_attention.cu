@@ -550,6 +550,43 @@ join_kernel(Args a) {
     pdl_launch_dependents();
     const Kv8Join u = a.joins[blockIdx.x];
     const int c = blockIdx.x, parts = u.last - c + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto store = [&](int row, int j, float y) {
+        const int rr = u.grp * M + row, tok = rr / a.d.group, h = u.head * a.d.group + rr % a.d.group;
+        reinterpret_cast<T*>(a.out)[(long long)(u.s0 + tok) * a.ldo + (long long)h * a.ldoh + j] = from_f<T>(y);
+    };
+    constexpr int B = 8;                                             // parts on their way at once
+    if (parts <= B) {                                                // a row a warp
+        for (int row = blockIdx.y * 4 + warp; row < u.rows; row += 4 * gridDim.y) {
+            float m[B], s[B], y[B][V], top = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                m[i] = -INFINITY;
+                if (i >= parts) continue;
+                const float* src = a.work + ((size_t)(i ? kv8_slot(c + i, 0, 0) : u.slot) * M + row) * (D + 2);
+                m[i] = src[D];
+                s[i] = src[D + 1];
+#pragma unroll
+                for (int j = 0; j < V; ++j) y[i][j] = src[lane + j * 32];
+            }
+#pragma unroll
+            for (int i = 0; i < B; ++i) top = fmaxf(top, m[i]);
+            float o[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) o[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                if (i >= parts) continue;
+                const float f = m[i] == -INFINITY ? 0.f : m[i] == top ? 1.f : ex2(m[i] - top);
+                l = fmaf(s[i], f, l);
+#pragma unroll
+                for (int j = 0; j < V; ++j) o[j] = fmaf(y[i][j], f, o[j]);
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+            for (int j = 0; j < V; ++j) store(row, lane + j * 32, o[j] * inv);
+        }
+        return;
+    }
     for (int row = blockIdx.y; row < u.rows; row += gridDim.y) {
         const float* first = a.work + ((size_t)u.slot * M + row) * (D + 2);
         auto part = [&](int k) { return k == 0 ? first : a.work + ((size_t)kv8_slot(c + k, 0, 0) * M + row) * (D + 2); };
@@ -559,7 +596,6 @@ join_kernel(Args a) {
         float o[V], l = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = 0.f;
-        constexpr int B = 8;                                         // parts on their way at once
         for (int k0 = warp; k0 < parts; k0 += 4 * B) {
             float m[B], s[B], y[B][V];
 #pragma unroll
@@ -584,10 +620,8 @@ join_kernel(Args a) {
         if (lane == 0) l_s[warp] = l;
         __syncthreads();
         l = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
-        const int rr = u.grp * M + row, tok = rr / a.d.group, h = u.head * a.d.group + rr % a.d.group;
-        T* dst = reinterpret_cast<T*>(a.out) + (long long)(u.s0 + tok) * a.ldo + (long long)h * a.ldoh;
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        for (int j = threadIdx.x; j < D; j += 128) dst[j] = from_f<T>(((o_s[0][j] + o_s[1][j]) + (o_s[2][j] + o_s[3][j])) * inv);
+        for (int j = threadIdx.x; j < D; j += 128) store(row, j, ((o_s[0][j] + o_s[1][j]) + (o_s[2][j] + o_s[3][j])) * inv);
         __syncthreads();
     }
 }

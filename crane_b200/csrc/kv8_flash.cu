@@ -19,7 +19,7 @@ namespace {
 
 constexpr int M = KV8_FLASH_ROWS, BN = 128, THREADS = 768;
 constexpr float P_SHIFT = 6.f;                 // weights run up to 2^14: the reference trails a row's maximum by up to 8
-using Units = Kv8Units<M, BN, 0>;       // (no steps of a unit's own: every part has a tile)
+using Units = Kv8Units<M, BN, 4>;
 
 struct Args {
     const void* q; long long ldq, ldqh;
@@ -207,8 +207,9 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             if (!DIRECT) step_on();
             else if (++kst == NK) { kst = 0; k_ph ^= 1; }
         };
-        for (long long step = begin; step < end; ++part) {
+        for (long long step = begin; step < end;) {
             const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
+            if (t0 < t1) {
             wait_keys();
             for (int w = 0; w < 2; ++w) {
                 wait(&q_full[w], part & 1);
@@ -235,6 +236,8 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 p_ph ^= 1;
                 if (!last) release_keys();
             }
+            ++part;
+            }
             step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
@@ -243,7 +246,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         const int ct = tid - 128;
         int rs = 0, fs = 0, seq = 0, part = 0;
         uint32_t r_ph = 0, f_ph = 1;
-        for (long long step = begin; step < end; ++part) {
+        for (long long step = begin; step < end;) {
             const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
             const int seen = u.q.first + (int)((long long)u.grp * M / group);      // last position that all rows see
             for (int t = t0; t < t1; ++t, ++seq) {
@@ -281,6 +284,7 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     if (++fs == NF) { fs = 0; f_ph ^= 1; }
                 }
             }
+            part += t0 < t1;
             step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }
@@ -291,8 +295,17 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         const uint32_t sa = tmem + lanes + C::C_S + w * BN + hf * 64, oa = tmem + lanes + w * D + hf * (D / 2);
         int seq = 0, part = 0;
         uint32_t s_ph = 0;
-        for (long long step = begin; step < end; ++part) {
+        for (long long step = begin; step < end;) {
             const int t0 = u.tile_at(step), t1 = u.tile_at(u.stop(end));
+            if (tid == 256 && u.begins(step, end)) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
+            if (t0 == t1) {                                                  // the unit's own steps alone: an empty part
+                float* dst = a.work + ((size_t)kv8_slot(blockIdx.x, begin, step) * M + r) * (D + 2);
+                for (int c = hf * (D / 2); c < (hf + 1) * (D / 2); c += 2) *reinterpret_cast<float2*>(dst + c) = make_float2(0.f, 0.f);
+                if (hf == 0) { dst[D] = -INFINITY; dst[D + 1] = 0.f; }
+                step = u.stop(end);
+                if (step < end && !u.next(a.d)) break;
+                continue;
+            }
             // ---- the queries, sixteen rows a warp, D / 8 lanes a row: each row's largest moved to [2^14, 2^15) by a power of two, f16 (or two e4m3 parts) ----
             constexpr int LR = D / 8, RW = 32 / LR;          // lanes a row, rows at a time
 #pragma unroll 2
@@ -506,8 +519,8 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                 }
             }
             if (!whole && hf == 0) { part_dst[D] = m; part_dst[D + 1] = l; }
-            if (tid == 256 && u.begins(step, end)) a.joins[blockIdx.x] = kv8_join(a.d, u, M, total, gridDim.x, blockIdx.x, begin);
             tc_fence_before();
+            ++part;
             step = u.stop(end);
             if (step < end && !u.next(a.d)) break;
         }

@@ -150,11 +150,11 @@ int main() {
         pieces(wild, true);
         for (int ctas : {1, 3, 148, 296}) {
             const int group = 1 + i % 7;
-            units<16, 64, 2>(tame, group, ctas, 0, 1LL << 62);
-            units<16, 64, 2>(tame, group, ctas, 0, 64);
-            units<64, 64, 2>(wild, group, ctas, 0, 1LL << 62);
-            units<256, 128, 0>(tame, group, ctas, 65, 1LL << 62);
-            units<256, 128, 0>(wild, group, ctas, 65, 1LL << 62);
+            units<16, 64, 4>(tame, group, ctas, 0, 1LL << 62);
+            units<16, 64, 4>(tame, group, ctas, 0, 64);
+            units<32, 32, 4>(wild, group, ctas, 0, 1LL << 62);
+            units<256, 128, 4>(tame, group, ctas, 65, 1LL << 62);
+            units<256, 128, 4>(wild, group, ctas, 65, 1LL << 62);
         }
     }
     std::puts("ok");
