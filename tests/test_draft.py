@@ -26,7 +26,7 @@ P = 1 << 20            # an address that is never used: every call below is refu
 
 
 @pytest.mark.parametrize("change, said", [
-    ({"dtype": 3}, "type 3"), ({"vocab": 0}, "vocab = 0"), ({"vocab": 1 << 31}, "vocab"), ({"seqs": 1 << 31}, "seqs"), ({"drafts": 1 << 31}, "drafts"), ({"logits": None}, "logits is NULL"),
+    ({"dtype": 3}, "type 3"), ({"vocab": 0}, "vocab = 0"), ({"vocab": 1 << 31}, "vocab"), ({"seqs": 1 << 31}, "seqs"), ({"drafts": 1 << 31}, "drafts"), ({"drafts": 1 << 27}, "2^27"), ({"logits": None}, "logits is NULL"),
     ({"ld": 9}, "9 apart"), ({"draft_logits": P + 1}, "draft_logits is not aligned"), ({"ldd": 9}, "draft_logits"), ({"tokens": None}, "tokens"), ({"starts": None}, "starts"),
     ({"starts": P + 2}, "starts"), ({"temperatures": P + 2}, "temperatures"), ({"uniforms": None}, "uniforms"), ({"noise": None}, "noise"), ({"ldn": 3}, "noise"),
     ({"accepted": None}, "accepted"), ({"next": P + 2}, "next")])

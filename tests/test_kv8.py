@@ -50,7 +50,7 @@ def test_numbers_of_device_memory_stay_in_range(tmp_path):
 CACHE = {"k_codes": P, "v_codes": P, "scales": P, "pages": 8, "kv_heads": 2, "page": 64, "dim": 128, "table": P, "ldt": 4, "width": 4, "lens": P, "starts": P, "seqs": 2, "rows": 3}
 BAD_CACHE = [({"k_codes": None}, "NULL"), ({"scales": None}, "NULL"), ({"v_codes": P + 8}, "16-byte"), ({"scales": P + 4}, "8-byte"), ({"pages": 0}, "pages"), ({"pages": 1 << 40}, "pages"),
              ({"pages": 1 << 25}, "pages"), ({"kv_heads": 0}, "kv_heads"), ({"page": 48}, "page = 48"), ({"dim": 96}, "dim = 96"), ({"table": None}, "table"), ({"table": P + 2}, "table"),
-             ({"ldt": 3}, "apart"), ({"width": 0}, "width"), ({"lens": None}, "lens"), ({"starts": None}, "starts"), ({"rows": 1 << 33}, "rows"), ({"seqs": 1 << 33}, "seqs")]
+             ({"ldt": 3}, "apart"), ({"width": 0}, "width"), ({"lens": None}, "lens"), ({"starts": None}, "starts"), ({"rows": 1 << 33}, "rows"), ({"seqs": 1 << 33}, "seqs"), ({"seqs": 1 << 25}, "seqs")]
 
 
 @pytest.mark.parametrize("change, said", BAD_CACHE + [({"dtype": 3}, "type 3"), ({"k": None}, "k is NULL"), ({"v": P + 1}, "not aligned"), ({"ldk": 100}, "100 apart"), ({"ldvh": 5}, "heads of 128")])

@@ -30,9 +30,9 @@ P = 1 << 20            # an address that is never used: every call below is refu
     ({"dtype": 3}, "type 3"), ({"w_dtype": 9}, "type 9"), ({"dtype": 1}, "their own type"), ({"rank": 0}, "rank = 0"), ({"rank": 129}, "rank = 129"), ({"k": 0}, "k = 0"),
     ({"adapters": 0}, "adapters"), ({"m": 1 << 40}, "m ="), ({"n": 1 << 33}, "n ="), ({"x": None}, "x is NULL"), ({"a": None}, "a is NULL"), ({"b": P + 2}, "b is not aligned"),
     ({"which": None}, "which"), ({"which": P + 1}, "which"), ({"scales": P + 2}, "scales"), ({"out": None}, "out"), ({"ldx": 7}, "7 apart"), ({"ldo": 5}, "5 apart"),
-    ({"ldadd": 5}, "add"), ({"add": P, "out": P, "ldadd": 300}, "add is out")])
+    ({"ldadd": 5}, "add"), ({"add": 4 * P, "out": 4 * P, "ldadd": 300}, "add is out"), ({"out": P}, "x is out")])
 def test_calls_are_refused_by_their_numbers(change, said):
-    a = {"device": 0, "x": P, "ldx": 64, "dtype": 0, "a": P, "b": P, "w_dtype": 0, "adapters": 3, "rank": 8, "which": P, "scales": None, "add": 2 * P, "ldadd": 200, "out": P, "ldo": 200,
+    a = {"device": 0, "x": P, "ldx": 64, "dtype": 0, "a": P, "b": P, "w_dtype": 0, "adapters": 3, "rank": 8, "which": P, "scales": None, "add": 2 * P, "ldadd": 200, "out": 3 * P, "ldo": 200,
          "m": 4, "n": 200, "k": 64, "stream": None}
     a.update(change)
     assert lib().crane_b200_lora_linear(*a.values()) in (crane_b200.INVALID_ARG, crane_b200.UNSUPPORTED)
