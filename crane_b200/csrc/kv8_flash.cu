@@ -1,10 +1,16 @@
 // Attention over an 8-bit paged cache (kv8.cuh) for sequences that bring many rows: 16-bit queries, tcgen05.  The mathematics is kv8_attention.cu's.
 //
-// Bound by the MMAs and, as much, by the exponentials: 256 query rows x 128 positions x D = 128 are 2 048 cycles of MMAs and as many of the SM's 16 exponentials a cycle.
-// A CTA has 256 query rows (two tiles of 128, each with its own softmax warps, scores and output in TMEM): while one tile's softmax runs, the other's MMAs do.  Codes come in by TMA
-// as they lie; four warps turn them into f16 operands once for both tiles (e4m3 is exact in f16; 32 K codes a step are 256 cvts a thread, under the MMAs), keys K-major, values
-// MN-major.  The alternative, codes as operands with queries and weights in two e4m3 parts each, needs no conversion but loses weights below 2^-19 of a row's
-// largest, and a first token that takes nearly everything is common.  Weights replace their scores in TMEM and are the A operand from there.
+// 256 query rows x 128 positions x D = 128 are 2 048 cycles of MMAs and as many of the SM's 16 exponentials a cycle.  A CTA has 256 query rows (two tiles of 128, each with its own
+// softmax warps, scores and output in TMEM): while one tile's softmax runs, the other's MMAs do.  Codes come in by TMA as they lie.  Four warps turn values into f16 operands, MN-major,
+// once for both tiles (e4m3 is exact in f16).  Keys of bf16 queries with 128 columns are operands as they come: such a query is two e4m3 parts, 2^-17 of its row's largest element,
+// and the two products take as long as one of f16.  Otherwise keys become f16 as well, K-major.  Weights stay f16: two e4m3 parts would lose those below 2^-19 of the largest, and a
+// first token that takes nearly everything is common.  They replace their scores in TMEM and are the A operand from there.
+//
+// What a step takes, two portions of 4096 rows behind 8192 positions, 32 heads over 8: 4 200 cycles, of which the MMAs fill 2 400: scores to weights 2 400 (720 to the maximum, 1 650 through
+// the exponentials), 330 until the MMA warp hears of it, 1 190 of output and next scores, 310 back; the two tiles' chains run half a turn apart.  1 021 us, 832 TFLOP/s of 1 675 measured.
+// By what it gave: one thread a row 1 546 -> two (80 registers) 1 215; with keys turned into f16 four warps could not keep three operand slots filled (1 544 with two threads a row);
+// every unit four steps of its own in the deal and parts joined a row a warp 1 021.  One pass over the scores with last step's reference, weights held back until it proves good,
+// spills: 1 413.
 // Work is dealt out by the 128-position step (kv8_units.h): persistent CTAs, whatever the lengths.
 #include <cuda_fp16.h>
 

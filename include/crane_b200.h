@@ -371,7 +371,7 @@ CRANE_B200_API int crane_b200_kv8_append(int device, const void* k, size_t ldk, 
                                          float* scales, size_t pages, size_t kv_heads, size_t page, size_t dim, const int32_t* table, size_t ldt, size_t width, const int32_t* lens,
                                          const int32_t* starts, size_t seqs, size_t rows, void* stream);
 /* out[i, h] = sum over the positions p <= that of row i of softmax(scale * q[i, h] . k_p) v_p, kv head h / (heads / kv_heads); q and out [rows, heads, dim] of one type.  Sums in f32,
- * weights in f16 (f32 rows: two f16 parts), rounded once to out's type.  Rows that see nothing give zeros; rows behind starts[seqs] are left as they are.  Scales are
+ * weights in f16 (f32 rows: two f16 parts), rounded once to out's type; bf16 queries of a sequence that brings more than 64 rows of a kv head keep 2^-17 of a row's largest element.  Rows that see nothing give zeros; rows behind starts[seqs] are left as they are.  Scales are
  * positive.  max_rows: the most rows that a sequence brings (0: not known); more than that only take longer.  crane_b200_fp8_status tells of a bounded wait that ran out. */
 CRANE_B200_API int crane_b200_kv8_attention_bytes(int device, int dtype, size_t heads, size_t kv_heads, size_t dim, size_t seqs, size_t rows, size_t max_rows, size_t* bytes);
 CRANE_B200_API int crane_b200_kv8_attention(int device, const void* q, size_t ldq, size_t ldqh, void* out, size_t ldo, size_t ldoh, int dtype, size_t heads, float scale,

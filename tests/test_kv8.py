@@ -6,6 +6,8 @@ Codes and scales are held bit for bit: a scale is a power of two, so every quoti
 Tolerance of attention, per output and fixed ahead of the first run; G = sum of w |v| (weights of the exact softmax), T positions, D columns:
   scores   products of f16 parts are exact, their f32 sums off by at most (D + 8) 2^-23 of A = max sum |q k| scale log2 e; f32 queries are two f16 parts, 2^-22 more; the exponent is rounded
            once more, 2^-23 of the distance to the maximum, and the factor scale log2 e of 16-bit rows, 2^-24: all within (D + 16) 2^-23 (A + 2), in units of log2
+           bf16 queries of 128 columns in sequences of more than 64 rows of a kv head are two e4m3 parts: the largest element is taken to [2^7, 2^8), a part's steps are 2^-9 there at
+           least, so each element is off by 2^-10 2^-7 of the largest at most: 2^-17 max |q| sum |k| scale log2 e more
   weights  ln 2 times that, in the numerator and in the denominator, and 2^-22 of the exponential in each; the numerator's are rounded to f16, 2^-11 (f32: two parts, 2^-22);
            weights below 2^-28 of the largest to 2^-39 of it, T in all
   sums     T / 16 additions of 16 products each, off by 2^-22 of the running sum, and as many joins as there are warps and CTAs: (T / 16 + 64) 2^-22
@@ -238,7 +240,10 @@ def attend_ref(q, cache, table, lens, starts, scale):
             out[starts[b]:starts[b + 1], h] = o
             size = w @ torch.nan_to_num(v).abs()
             a = torch.where(seen, (x.abs() @ torch.nan_to_num(k).abs().t()) * abs(scale) * 1.4427, 0.0).amax(1, keepdim=True) if t else x[:, :1] * 0
-            off = 2 * (0.6932 * (d + 16) * 2.0 ** -23 * (a + 2) + 2.0 ** -22) + (2.0 ** -22 if exact32 else 2.0 ** -11) + (t / 16 + 64) * 2.0 ** -22
+            parts = 0.0
+            if q.dtype == torch.bfloat16 and d == 128 and n * group > 64 and t:
+                parts = 2.0 ** -17 * x.abs().amax(1, keepdim=True) * torch.nan_to_num(k).abs().sum(1).amax() * abs(scale) * 1.4427
+            off = 2 * (0.6932 * ((d + 16) * 2.0 ** -23 * (a + 2) + parts) + 2.0 ** -22) + (2.0 ** -22 if exact32 else 2.0 ** -11) + (t / 16 + 64) * 2.0 ** -22
             tiny = t * 2.0 ** -39 * torch.nan_to_num(v).abs().amax() if t else 0.0
             tol[starts[b]:starts[b + 1], h] = off * size + tiny
     return out, tol
@@ -362,6 +367,18 @@ def test_queries_of_extreme_values():
         check(got[keep], (ref[0][keep], ref[1][keep]))
         fine = torch.isfinite(q[2]).all(1, keepdim=True)                # (f16 has infinities among these)
         assert torch.equal(torch.isfinite(got[2]), fine.expand_as(got[2]))      # (scores of 1e30: one position takes all, which one is a matter of the last bit)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_queries_with_a_column_far_larger_than_the_rest(dt):
+    """... that the keys have little of: the small elements decide."""
+    for loud in (30.0, 1000.0):
+        q, c, table, lens, starts = problem(gen_of("loud", dt, loud), dt, 8, 2, 128, 64, [200, 90], [150, 2], loud=False)
+        q[:, :, 17] *= loud
+        c[0][:, :, :, 17] = (c[0][:, :, :, 17].float() / loud).to(F8)
+        p = (q, c, table, lens, starts)
+        check(run_attention(p, scale=0.3), attend_ref(*p, 0.3))
 
 
 @pytest.mark.gpu
