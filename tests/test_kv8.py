@@ -79,6 +79,11 @@ def test_sizes_of_workspaces_are_refused():
     assert lib().crane_b200_kv8_attention_bytes(0, 1, 4, 2, 128, 1, 1, 0, None) == crane_b200.INVALID_ARG
 
 
+def test_numbers_of_heads_that_pass_32_bits_are_refused():
+    n = C.c_size_t()
+    assert lib().crane_b200_kv8_attention_bytes(0, 1, 65535 * 65534, 65534, 128, 1, 1, 0, C.byref(n)) == crane_b200.INVALID_ARG and "heads over 65534" in why()
+
+
 def test_tensors_are_refused():
     from crane_b200 import kv8
     c = kv8.pages(4, 2, 64, 16, device="cpu")
@@ -454,3 +459,32 @@ def test_a_sequence_grows():
         run_append(cache, qkv[:, 4:6], qkv[:, 6:], table, lens, starts)
         p = (qkv[:, :4], cache, table, lens, starts)
         check(run_attention(p), attend_ref(*p, 128 ** -0.5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [0.0, -0.4, 2.5])
+def test_scales_of_any_sign(scale, dim):
+    """Zero weighs all positions alike; a negative one turns the order round."""
+    for dt in TYPES:
+        for new in ([1, 2, 1], [100, 5, 70]):
+            p = problem(gen_of("sign", dt, scale, dim, new), dt, 8, 2, dim, 64, [150, 90, 200], new, loud=False)
+            check(run_attention(p, scale=scale), attend_ref(*p, scale))
+
+
+@pytest.mark.gpu
+def test_a_cache_whose_codes_pass_32_bits():
+    """The highest pages of 4.6 GB of codes against the same pages of a small cache, rows and results, the results over the queries too."""
+    from crane_b200 import kv8
+    big, few = kv8.pages(70000, 8, 128, 64), kv8.pages(6, 8, 128, 64)
+    assert big[0].numel() > 1 << 32
+    pages = [69999, 3, 68000, 66001, 69998, 5]
+    lens, starts = ints([150, 140]), ints([0, 150, 290])
+    x = torch.randn((290, 32, 128), generator=gen_of("wide"), device="cuda").bfloat16()
+    for cache, table in ((big, pages), (few, list(range(6)))):
+        kv8.append(x[:, 16:24], x[:, 24:], cache, ints(table).reshape(2, 3), lens, starts)
+    for a, b in zip(big, few):
+        assert torch.equal(a.view(torch.uint8)[pages], b.view(torch.uint8))
+    for q, s in ((x[:, :16].clone(), starts), (x[:2, :16].clone(), ints([0, 1, 2]))):
+        want = kv8.attention(q, few, ints(list(range(6))).reshape(2, 3), lens, s)
+        assert torch.equal(kv8.attention(q, big, ints(pages).reshape(2, 3), lens, s, out=q), want)
