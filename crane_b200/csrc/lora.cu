@@ -6,7 +6,7 @@
 // two of its own), so that the rank's sum loses nothing that a 16-bit result could show.  f32 weights or rows: tf32 parts, hi hi + lo hi + hi lo, 2^-22 of each product.
 //
 // Bound by bytes in principle: for single rows those of A and B, for prompts those of add and out.  Which k a place of a fragment stands for is free as long as both operands agree, so a
-// lane takes 16 neighbouring bytes of a row straight from global memory, and the columns of a result are dealt so that a lane leaves eight neighbours.  Up to 256 rows any 16 that share
+// lane takes 16 neighbouring bytes of a row straight from global memory, and the columns of a result are dealt so that a lane leaves eight neighbours.  Up to 384 rows any 16 that share
 // an adapter are a tile; beyond, 64 neighbours, one adapter after the other, the first few of them by clusters of their own, and add and B come in through a ring of stages.
 // 8192 rows x 4096 -> 24 576, rank 64, bf16: 401 us (883 MB: 137): fixed work of a CTA (its sums, the cluster's, T's parts) 84, X A^T 50; add, B, products and stores, some 70 each,
 // one behind the other (leaving any one out saves its 70): eight warps in step.  Without the ring 570.  One row 5.6, 33 rows of 20 adapters, f32, 25.6 (36 MB: 5.6).
@@ -140,14 +140,12 @@ struct Shape {
     static constexpr int EB = MT > 1 ? 1 : T32 && RT > 4 ? 1 : 2;    // blocks of 32 columns a warp has under way
     static constexpr int KS = T32 ? RT : RT / 2;                     // MMAs along the rank
     static constexpr int T_BYTES = ROWS * LDT * 4, FRAG = MT * KS * 32 * 16;
-    // The columns of a step, add and B, come in through a ring of stages
+    // Many rows: the columns of a step, add and B, come in through a ring of stages
     static constexpr int NC = CW * 32, ADD = ROWS * NC * (int)sizeof(X), STAGE = ADD + NC * RP * (int)sizeof(W);
-    // Shares of T (this CTA's, read by the cluster) and T; where there are few rows the first stages are asked for ahead of them, otherwise they come into the same room
-    static constexpr int T_ROOM = 2 * T_BYTES, AHEAD = MT == 1;
-    static constexpr int CTAS = MT == 1 || 2 * FRAG + AHEAD * T_ROOM + 3 * STAGE <= 112 * 1024 ? 2 : 1;         // resident on an SM
-    static constexpr int FITS = ((CTAS == 2 ? 112 : 222) * 1024 - 2 * FRAG - AHEAD * T_ROOM) / STAGE, STAGES = MT == 1 || FITS < 2 ? 0 : FITS > 4 ? 4 : FITS;
-    static constexpr int ROOM = AHEAD ? T_ROOM + STAGES * STAGE : STAGES * STAGE > T_ROOM ? STAGES * STAGE : T_ROOM;
-    static constexpr int SMEM = 2 * FRAG + ROOM, RING = 2 * FRAG + AHEAD * T_ROOM;                   // ahead of those the two parts of T
+    static constexpr int T_ROOM = 2 * T_BYTES;                       // shares of T (this CTA's, read by the cluster) and T; the stages come into the same room
+    static constexpr int CTAS = MT == 1 || 2 * FRAG + 3 * STAGE <= 112 * 1024 ? 2 : 1;               // resident on an SM
+    static constexpr int FITS = ((CTAS == 2 ? 112 : 222) * 1024 - 2 * FRAG) / STAGE, STAGES = MT == 1 || FITS < 2 ? 0 : FITS > 4 ? 4 : FITS;
+    static constexpr int ROOM = STAGES * STAGE > T_ROOM ? STAGES * STAGE : T_ROOM, SMEM = 2 * FRAG + ROOM;      // ahead of those the two parts of T
 };
 
 // o += T B^T over 16 of the rank: EM row tiles from `er` on, 32 columns
@@ -262,20 +260,20 @@ lora_kernel(Lora l, bool gather, int slots) {
         auto add_at = [](int row, int c) { return (row * CX + (c ^ (sizeof(X) == 4 ? row & 1 : (row & 1) << 2))) * 16; };
         auto b_at = [](int row, int c) { return (row * CB + (c ^ ((sizeof(W) == 4 ? (row & 1) << 2 : ((row & 1) | (row >> 2 & 2)) << 1) & (CB - 1)))) * 16; };
         const int c0 = nb0 * 32, c1 = min(nb1 * 32, l.n), steps = (c1 - c0 + NC - 1) / NC;
-        const X* a_src = nullptr;                                    // rows of many are neighbours: one address
+        const X* a_src = nullptr;                                    // the tile's rows are neighbours: one address
         const W* b_src = nullptr;
         uint32_t a_in = 0;
         bool b_in = false;
         auto setup = [&]() {
 #pragma unroll
             for (int k = 0; k < AK; ++k) a_in |= (uint32_t)(add && (mine >> (tid / CX + k * AR) & 1)) << k;
-            if (MT > 1 && add) a_src = add + (long long)(tile * ROWS + tid / CX) * l.ldadd + c0 + tid % CX * EX;
+            if (add) a_src = add + (long long)(tile * ROWS + tid / CX) * l.ldadd + c0 + tid % CX * EX;
             b_in = tid % CB * EWT < l.rank;
             b_src = B + (b_in ? (size_t)(c0 + tid / CB) * l.rank + tid % CB * EWT : 0);
         };
         auto copy = [](uint32_t dst, const void* src, bool in) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory"); };
         auto fetch = [&](int step) {
-            const uint32_t st = smem_u32(sm) + S::RING + step % (ST > 0 ? ST : 1) * S::STAGE;
+            const uint32_t st = smem_u32(sm) + 2 * S::FRAG + step % (ST > 0 ? ST : 1) * S::STAGE;
             const int off = step * NC;
             if (add) {
                 const bool here = c0 + off + tid % CX * EX < c1;
@@ -283,8 +281,7 @@ lora_kernel(Lora l, bool gather, int slots) {
 #pragma unroll
                 for (int k = 0; k < AK; ++k) {
                     const bool in = here && (a_in >> k & 1);
-                    const X* src = MT > 1 ? a_src + (long long)(k * AR) * l.ldadd + off : add + (in ? (long long)rows_s[tid / CX + k * AR] * l.ldadd + c0 + off + tid % CX * EX : 0);
-                    copy(dst + k * (THREADS * 16), in ? src : add, in);
+                    copy(dst + k * (THREADS * 16), in ? a_src + (long long)(k * AR) * l.ldadd + off : add, in);
                 }
             }
             if (w >= 0) {
@@ -296,7 +293,6 @@ lora_kernel(Lora l, bool gather, int slots) {
             }
         };
         auto first = [&]() { for (int i = 0; i < ST - 1; ++i) { if (i < steps) fetch(i); asm volatile("cp.async.commit_group;" ::: "memory"); } };
-        if (STAGED && S::AHEAD && (w >= 0 || add != out)) { setup(); first(); }
         if (w >= 0) {
             // ---- this CTA's share of T ----
             const W* A = reinterpret_cast<const W*>(l.a) + (size_t)w * l.rank * l.k;
@@ -432,7 +428,8 @@ lora_kernel(Lora l, bool gather, int slots) {
         const int er = warp % EW * EM;                               // this warp's first row tile
         if constexpr (STAGED) {
             if (w >= 0 || add != out) {
-                if (!S::AHEAD) { setup(); first(); }
+                setup();
+                first();
                 const bool idle = !(mine >> (er * 16) & ((1ull << (16 * EM)) - 1));      // none of this warp's rows
                 const int cw = warp / EW * 32;
                 uint32_t row_in = 0;
@@ -453,7 +450,7 @@ lora_kernel(Lora l, bool gather, int slots) {
                     if (step + ST - 1 < steps) fetch(step + ST - 1);
                     asm volatile("cp.async.commit_group;" ::: "memory");
                     if (idle) continue;
-                    const unsigned char* st = sm + S::RING + step % ST * S::STAGE;
+                    const unsigned char* st = sm + 2 * S::FRAG + step % ST * S::STAGE;
                     float o[EM][4][4];
 #pragma unroll
                     for (int i = 0; i < EM; ++i)
@@ -584,7 +581,10 @@ int launch_rank(cudaStream_t st, const Lora& l, bool gather, int cluster, bool p
 }
 template <typename X, typename W>
 int launch_types(cudaStream_t st, const Lora& l, bool vec, bool pdl) {
-    const bool gather = l.m <= 256;
+    // Rows that share an adapter side by side, or as they lie.  Us, rank 16, bf16, 4096 -> 12 288, rows of 1 / 8 / 60 adapters: 200 rows 19 / 20 / 25 against 23 / 24 / 73, 400 rows
+    // 26 / 27 / 37 against 26 / 28 / 52, 800 rows 50 / 53 / 53 against 36 / 36 / 58; rank 64, 2048 -> 2048, of 1 / 6 / 40: 300 rows 20 / 20 / 21 against 19 / 21 / 31, 500 rows 31 / 31 / 32
+    // against 22 / 26 / 45.
+    const bool gather = l.m <= 384;
     const int tiles = gather ? (l.m + 7) / 8 : (l.m + 63) / 64, sms = tc_device_sms();
     int cluster = 1;
     while (cluster < 8 && (!gather || tiles * cluster * 2 <= 2 * sms)) cluster *= 2;

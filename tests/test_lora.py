@@ -99,6 +99,7 @@ SIZES = [  # rows, n, k, rank, adapters, order
     (1, 8, 8, 8, 1, "one"), (1, 1, 1, 1, 1, "one"), (1, 4096, 2048, 16, 3, "one"), (5, 33, 77, 3, 4, "any"), (33, 1000, 520, 16, 9, "any"), (64, 264, 1024, 64, 2, "any"),
     (65, 96, 64, 17, 5, "any"), (256, 512, 256, 128, 3, "any"), (257, 512, 256, 128, 3, "any"), (257, 136, 328, 8, 40, "any"), (300, 1001, 1037, 40, 4, "runs"), (513, 2048, 1536, 32, 5, "runs"),
     (20, 72, 64, 8, 2, "none"), (400, 72, 64, 8, 2, "none"), (1000, 24, 40, 100, 1, "one"), (2500, 640, 128, 64, 6, "runs"),
+    (384, 512, 256, 128, 3, "any"), (385, 512, 256, 128, 3, "any"), (390, 136, 328, 8, 40, "any"), (450, 1001, 1037, 40, 4, "runs"),
 ]
 
 
