@@ -9,7 +9,7 @@
 // lane takes 16 neighbouring bytes of a row straight from global memory, and the columns of a result are dealt so that a lane leaves eight neighbours.  Up to 384 rows any 16 that share
 // an adapter are a tile; beyond, 64 neighbours, one adapter after the other, the first few of them by clusters of their own, and add and B come in through a ring of stages.
 // 8192 rows x 4096 -> 24 576, rank 64, bf16: 401 us (883 MB: 137): fixed work of a CTA (its sums, the cluster's, T's parts) 84, X A^T 50; add, B, products and stores, some 70 each,
-// one behind the other (leaving any one out saves its 70): eight warps in step.  Without the ring 570.  One row 5.6, 33 rows of 20 adapters, f32, 25.6 (36 MB: 5.6).
+// one behind the other (leaving any one out saves its 70): eight warps in step, which is why lora_tiles.cu has these.  Without the ring 570.  One row 5.6, 33 rows of 20 adapters, f32, 25.6 (36 MB: 5.6).
 #include <cuda_fp16.h>
 
 #include "lora.cuh"
@@ -606,6 +606,10 @@ int lora_linear_launch(cudaStream_t st, const Lora& l, bool pdl) {
         if (l.w_type == LORA_BF16) return launch_types<float, bf16>(st, l, vec, pdl);
         if (l.w_type == LORA_F16) return launch_types<float, __half>(st, l, vec, pdl);
     } else if (l.type == l.w_type) {
+        // Us, bf16, here / in tiles of 128 rows, rows of 1, 6 and 40 adapters.  2048 -> 2048, rank 64: 1200 rows 29, 30, 49 / 34, 39, 55; 2500 rows 46, 49, 57 / 38, 40, 68; 9400 rows 132, 136,
+        // 140 / 55, 56, 66.  4096 -> 12 288: 2500 rows, rank 64, 119, 122, 132 / 79, 79, 152, rank 32, 95, 96, 110 / 69, 68, 136, rank 16, 61, 63, 70 / 64, 63, 126; 9400 rows, rank 32,
+        // 247, 247, 272 / 195, 211, 224.
+        if (vec && l.m >= 2048 && l.rank > 16 && l.rank <= 64) return lora_tiles_launch(st, l, pdl);
         if (l.type == LORA_BF16) return launch_types<bf16, bf16>(st, l, vec, pdl);
         if (l.type == LORA_F16) return launch_types<__half, __half>(st, l, vec, pdl);
     }

@@ -15,8 +15,11 @@ struct Lora {
     const void* add; long long ldadd;                               // nullptr: zeros; may be out
     void* out; long long ldo;
     int m, n, k, rank, adapters;
+    int* err;                                                       // tc_err_word, or the like: of a wait that ran out
 };
 constexpr int LORA_MAX_RANK = 128;
+// Many rows of 16 bits, ranks from 17 to 64, everything on 16-byte boundaries (lora_tiles.cu)
+int lora_tiles_launch(cudaStream_t st, const Lora& l, bool pdl);
 int lora_linear_launch(cudaStream_t st, const Lora& l, bool pdl);
 
 }  // namespace cb

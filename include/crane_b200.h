@@ -380,7 +380,8 @@ CRANE_B200_API int crane_b200_kv8_attention(int device, const void* q, size_t ld
                                             void* work, size_t work_bytes, void* stream);
 /* out[i, :] = add[i, :] + scales[w] * B_w (A_w x[i, :]), w = which[i]; rows whose w is outside [0, adapters) have none: out = add.  x [m, k], add (NULL: zeros; may be out) and out
  * [m, n] of one type, a [adapters, rank, k] and b [adapters, n, rank] contiguous, of that type too or, beside f32 rows, of any; scales [adapters] (NULL: ones).  rank 1 to 128.
- * Sums in f32, rounded once.  Any order of `which` is right; beyond 384 rows neighbours of one adapter are fastest. */
+ * Sums in f32, rounded once.  Any order of `which` is right; beyond 384 rows neighbours of one adapter are fastest.
+ * crane_b200_fp8_status tells of a bounded wait that ran out. */
 CRANE_B200_API int crane_b200_lora_linear(int device, const void* x, size_t ldx, int dtype, const void* a, const void* b, int w_dtype, size_t adapters, size_t rank,
                                           const int32_t* which, const float* scales, const void* add, size_t ldadd, void* out, size_t ldo, size_t m, size_t n, size_t k, void* stream);
 /* Drafted tokens against the target's probabilities.  Sequence b has the drafts starts[b] .. starts[b + 1] - 1 of `tokens` [drafts] (starts ascends from 0, [seqs + 1]) and the logits

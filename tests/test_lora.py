@@ -75,7 +75,10 @@ def check(got, ref):
     y, off = ref
     half = torch.finfo(got.dtype).eps / 2
     lim = off + 2.0 ** -24 * y.abs() + half * (y.abs() + off) + (2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -149)
-    err = (got.double() - y).abs()
+    top = torch.finfo(got.dtype).max
+    edge = top + top * half / (2 - 2 * half)                            # half a step above the largest value: from there on the nearest is infinity (f16: 65 504 and 65 520)
+    over = torch.isinf(got) & (torch.sign(got.double()) == torch.sign(y)) & (y.abs() + off >= edge)
+    err = torch.where(over, 0.0, (got.double() - y).abs())
     assert bool((err <= lim).all()), (int((err > lim).sum()), float((err / lim).max()))
 
 
@@ -147,6 +150,55 @@ def test_infinities_and_nan_stay_in_their_rows(m):
         y = lora.linear(x, a, b, which, scales=scales, add=add)
         assert torch.equal(y[0], add[0]) and torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any() and torch.isnan(y[m - 1]).all()
         check(y[3:m - 1], tuple(t[3:m - 1] for t in reference(x, a, b, which, scales, add)))
+
+
+TILES = [(2048, 72, 40, 24, 3, "any"), (2100, 1000, 520, 64, 40, "runs"), (3001, 520, 2048, 40, 5, "runs"), (2048, 8, 8, 32, 1, "one"), (4100, 136, 1096, 56, 30, "any"),
+         (2177, 4096, 1024, 32, 7, "runs"), (2100, 72, 64, 32, 2, "none"), (6000, 640, 256, 24, 300, "runs")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("size", TILES, ids=lambda s: "-".join(map(str, s)))
+def test_adapters_of_prompts(size, dt):
+    from crane_b200 import lora
+    x, a, b, which, scales, add = problem(gen_of("tiles", size, dt), dt, dt, *size)
+    ref = reference(x, a, b, which, scales, add)
+    y = lora.linear(x, a, b, which, scales=scales, add=add)
+    check(y, ref)
+    check(lora.linear(x, a, b, which), reference(x, a, b, which, None, None))
+    m, n, k = size[:3]                                                  # rows further apart, columns beside the result's stay, in place, other rows not finite
+    wide, room = torch.full((m, k + 16), math.nan, dtype=TYPES[dt], device="cuda"), torch.full((m, n + 24), 3.0, dtype=TYPES[dt], device="cuda")
+    wide[:, 8:8 + k], room[:, 16:16 + n] = x, add
+    out = room[:, 16:16 + n]
+    bad = [5, m // 2, m - 1]
+    wide[bad[0]], wide[bad[1], 9], wide[bad[2], 10] = math.nan, math.inf, -math.inf
+    lora.linear(wide[:, 8:8 + k], a, b, which, scales=scales, add=out, out=out)
+    rest = torch.ones(m, dtype=torch.bool, device="cuda")
+    rest[bad] = False
+    assert torch.equal(out[rest], y[rest]) and (room[:, :16] == 3).all() and (room[:, 16 + n:] == 3).all()
+    for i in bad:
+        assert torch.equal(out[i], add[i]) if not 0 <= int(which[i]) < a.shape[0] else not torch.isfinite(out[i]).any()
+
+
+@pytest.mark.gpu
+def test_prompts_repeat_in_graphs_and_on_streams():
+    from crane_b200 import lora
+    x, a, b, which, scales, add = problem(gen_of("tiles repeat"), "bf16", "bf16", 2300, 1032, 1024, 64, 5, "runs")
+    one = lora.linear(x, a, b, which, scales=scales, add=add)
+    outs = []
+    for st in [torch.cuda.Stream() for _ in range(3)] * 3:
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            outs.append(lora.linear(x, a, b, which, scales=scales, add=add))
+    torch.cuda.synchronize()
+    assert all(torch.equal(one, o) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = lora.linear(x, a, b, which, scales=scales, add=add)
+    for i in range(3):
+        which.copy_(which.flip(0) if i else which[torch.randperm(2300, generator=gen_of("order"), device="cuda")])
+        graph.replay()
+        check(y, reference(x, a, b, which, scales, add))
 
 
 @pytest.mark.gpu
