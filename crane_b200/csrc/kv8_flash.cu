@@ -114,13 +114,13 @@ flash_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     pdl_wait();
     const long long total = kv8_count<Units>(a.d, sums);
     const long long begin = kv8_range(total, gridDim.x, blockIdx.x), end = kv8_range(total, gridDim.x, blockIdx.x + 1);
-    pdl_launch_dependents();
     if (tid == 256) a.joins[blockIdx.x].rows = 0;
     if (begin >= end) return;
     if (warp == 2) { tmem_alloc(&tmem_slot, 512); tmem_relinquish(); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();                                 // (behind the allocation: a kernel that allocates and then waits for this one must not come ahead of it)
     const uint32_t tmem = tmem_slot;
     const TcWait wait{&gave_up, a.err};
     Units u = kv8_find<Units>(a.d, sums, begin);

@@ -50,7 +50,7 @@ lora_tile_kernel(Lora l, int slots) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     if (tid == 0) { gave_up = 0; mbar_init(&bar, 1); fence_barrier_init(); }
     pdl_wait();
-    pdl_launch_dependents();
+    if (warp == 0) { tmem_alloc(&tmem_s, 64); tmem_relinquish(); }
     uint32_t cl;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(cl));
     const int cr = (int)cluster_rank(), nc = (int)cl, tile = blockIdx.x / nc / slots, slot = blockIdx.x / nc % slots;
@@ -59,7 +59,13 @@ lora_tile_kernel(Lora l, int slots) {
         const int r = tile * ROWS + tid, v = r < l.m ? __ldg(l.which + r) : -2;
         which_s[tid] = r >= l.m ? -2 : (unsigned)v < (unsigned)l.adapters ? v : -1;
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    // Behind the allocation: a kernel that allocates and then waits for this one must not come ahead of it.  Nor do two kernels wait for one another's columns while their CTAs wait for
+    // one another: those that take more than TMEM has beside two of these CTAs leave no room for them in shared memory.
+    pdl_launch_dependents();
+    const uint32_t tmem = tmem_s;
     if (tid < ROWS) {
         const int v = which_s[tid];
         bool lead = v != -2;
@@ -74,8 +80,7 @@ lora_tile_kernel(Lora l, int slots) {
     X* out = reinterpret_cast<X*>(l.out) + (long long)tile * ROWS * l.ldo;
     const int nb = (l.n + NC - 1) / NC, c0 = (int)((long long)nb * cr / nc) * NC, c1 = min((int)((long long)nb * (cr + 1) / nc) * NC, l.n), steps = c1 > c0 ? (c1 - c0 + NC - 1) / NC : 0;
     const int kc = (l.k + 63) / 64, k0 = (int)((long long)kc * cr / nc), chunks = (int)((long long)kc * (cr + 1) / nc) - k0, ksteps = (l.rank + 15) / 16;
-    uint32_t tmem = 0, phase = 0;
-    bool have_tmem = false;
+    uint32_t phase = 0;
     int turn = 0;
     for (int word = 0; word < 4; ++word)
     for (unsigned leads = lead_s[word]; leads; leads &= leads - 1) {
@@ -135,15 +140,6 @@ lora_tile_kernel(Lora l, int slots) {
                 if (r < RP) copy(st + PART + sw128_off(r, fp), in ? A + (size_t)r * l.k + at : A, in);
             }
         };
-        if (!have_tmem) {
-            // (two of these CTAs and none of those that take more than the rest of TMEM and wait for another CTA fit an SM: nobody holds what another one waits for)
-            if (warp == 0) { tmem_alloc(&tmem_s, 64); tmem_relinquish(); }
-            tc_fence_before();
-            __syncthreads();
-            tc_fence_after();
-            tmem = tmem_s;
-            have_tmem = true;
-        }
         const int row = (warp & 3) * 32 + lane, half = warp >> 2;     // TMEM's lanes of a warp are its rows, half of the columns
         const uint32_t mine_d = tmem + ((uint32_t)(warp & 3) << 21);
         // ---- this CTA's share of T ----
@@ -281,9 +277,7 @@ lora_tile_kernel(Lora l, int slots) {
         tc_fence_before();
         __syncthreads();                                             // (T's parts and the stages may be written again)
     }
-    if (have_tmem) {
-        if (warp == 0) { wait.drain(); tc_fence_after(); tmem_dealloc(tmem, 64); }
-    }
+    if (warp == 0) { wait.drain(); tc_fence_after(); tmem_dealloc(tmem, 64); }
 }
 
 template <typename X, int RP>
