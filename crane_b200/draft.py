@@ -31,7 +31,7 @@ def verify(logits, tokens, starts, uniforms, noise, *, draft_logits=None, temper
     Sequence b has the drafts tokens[starts[b]:starts[b + 1]] (int32, starts [sequences + 1] int32 from 0) and the rows starts[b] + b to starts[b + 1] + b of logits
     [drafts + sequences, vocabulary] (f32, bf16 or f16): one ahead of each draft, one behind the last.  p and q: softmax of a row / temperature, the target's and the draft model's
     (draft_logits [drafts, vocabulary] of the same type; None: the drafts were certain).  Draft j holds while uniforms[j] * q(draft) < p(draft); behind it follows the first argmax of
-    w / -log(noise[b]), w = max(p - q, 0) at the first that does not hold, or p behind the last.  temperatures [sequences] f32 (None: 1), 0: greedy.  noise
+    w / -log(noise[b]), w = max(p - q, 0) at the first that does not hold, or p behind the last.  temperatures [sequences] f32 (None: 1), 0 or less: greedy.  noise
     [sequences, vocabulary] f32 between 0 and 1.  -1 follows a row without a logit above -inf."""
     dev, rows, vocab, ld, dtype = _rows_in("logits", logits)
     if not isinstance(tokens, torch.Tensor) or tokens.dim() != 1:

@@ -216,6 +216,17 @@ def test_extreme_temperatures():
 
 
 @pytest.mark.gpu
+def test_infinite_and_negative_temperatures():
+    """Infinite: all tokens above -inf alike, so the noise alone decides; below zero: greedy."""
+    for dt in TYPES:
+        logits, _, starts, uniforms, noise, q, _ = problem(gen_of("all", dt), dt, [2, 2], 300, temps=[1.0, 1.0])
+        logits[:, 200:], q[:, 200:] = -math.inf, -math.inf
+        first = [int(logits[i].argmax()) for i in range(6)]
+        accepted, following = run((logits, [3, 250, first[3], first[4]], starts, uniforms * 0.5, noise, q, [math.inf, -1.0]))
+        assert accepted == [1, 2] and following[0] == int(noise[0, :200].argmax()) and following[1] == first[5]
+
+
+@pytest.mark.gpu
 def test_rows_on_any_boundary():
     for dt in TYPES:
         p = problem(gen_of("rows", dt), dt, [2, 1, 3], 1001)
