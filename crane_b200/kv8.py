@@ -4,7 +4,7 @@
     kv8.append(k, v, cache, table, lens, starts)                      # the new rows of all sequences into their pages
     out = kv8.attention(q, cache, table, lens, starts)                # each new row over what its sequence holds, itself included
 
-`table` [sequences, pages] int32 has the pages of each sequence (the rest: any number outside the cache), `lens` [sequences] int32 the positions it holds, new rows included, and
+`table` [sequences, pages] int32 has the pages of each sequence (the rest: any number outside the cache; a row of its own for each: expanded and overlapping tables are refused), `lens` [sequences] int32 the positions it holds, new rows included, and
 `starts` [sequences + 1] int32 where each sequence's new rows begin: a decoded token, drafted ones, or portions of prompts, side by side.  These three are read on the device only.
 Calls run on the tensors' device and its current stream, wait for nothing, keep nothing and may be captured into graphs.  Sequences may share pages that none of them writes.
 """
@@ -62,9 +62,9 @@ def _seqs(table, lens, starts, dev: int):
     try:
         seqs, width = table.shape
         ldt, step = table.stride()
-        if (step == 1 and table.dtype is _I32 and lens.dtype is _I32 and starts.dtype is _I32 and lens.shape == (seqs,) and starts.shape == (seqs + 1,) and lens.is_contiguous()
-                and starts.is_contiguous() and dev == table.get_device() == lens.get_device() == starts.get_device()):
-            return table.data_ptr(), max(ldt, width), width, lens.data_ptr(), starts.data_ptr(), seqs
+        if (step == 1 and ldt >= width and table.dtype is _I32 and lens.dtype is _I32 and starts.dtype is _I32 and lens.shape == (seqs,) and starts.shape == (seqs + 1,)
+                and lens.is_contiguous() and starts.is_contiguous() and dev == table.get_device() == lens.get_device() == starts.get_device()):
+            return table.data_ptr(), ldt, width, lens.data_ptr(), starts.data_ptr(), seqs
     except (AttributeError, ValueError):
         pass
     t = _ints("table", table, dev, (None, None))

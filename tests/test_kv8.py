@@ -95,6 +95,34 @@ def test_tensors_are_refused():
         kv8.attention(x, (x, x), i, i[0, :1], i[0, :2])
 
 
+def repeating_tables(device):
+    """Tables whose rows repeat or overlap: one row for all sequences, windows of one list."""
+    i = torch.arange(20, dtype=torch.int32, device=device)
+    return [i[:5].expand(4, -1), i.as_strided((4, 5), (2, 1)), i.as_strided((4, 5), (4, 1)), i[3:4].expand(4, 1)]
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_tables_whose_rows_repeat_or_overlap_are_refused(which):
+    """They are passed on as they lie: the distance of their rows is less than their width, and no distance that they do not have is made up, which would lead behind the storage."""
+    from crane_b200 import kv8
+    table, i = repeating_tables("cpu")[which], torch.zeros(5, dtype=torch.int32)
+    s = dict(zip(("table", "ldt", "width", "lens", "starts", "seqs"), kv8._seqs(table, i[:4], i, -1)))
+    assert s["ldt"] == table.stride(0) and s["width"] == table.shape[1] and s["seqs"] == 4
+    cache = {**CACHE, "ldt": s["ldt"], "width": s["width"], "seqs": s["seqs"]}
+    a = {"device": 0, "k": P, "ldk": 256, "ldkh": 128, "v": P, "ldv": 256, "ldvh": 128, "dtype": 1, **cache, "stream": None}
+    assert lib().crane_b200_kv8_append(*a.values()) == crane_b200.INVALID_ARG and "apart" in why()
+    a = {"device": 0, "q": P, "ldq": 512, "ldqh": 128, "out": P, "ldo": 512, "ldoh": 128, "dtype": 1, "heads": 4, "scale": 0.1, **cache, "max_rows": 0, "work": P, "bytes": 1 << 30, "stream": None}
+    assert lib().crane_b200_kv8_attention(*a.values()) == crane_b200.INVALID_ARG and "apart" in why()
+
+
+def test_a_single_row_of_pages_may_lie_at_any_distance():
+    from crane_b200 import kv8
+    i = torch.zeros(20, dtype=torch.int32)
+    for table in (i.as_strided((1, 5), (0, 1)), i.as_strided((1, 5), (2, 1)), i[:5].view(1, 5), i.view(4, 5)[2:3]):
+        t, ldt, width, *_, seqs = kv8._seqs(table, i[:1], i[:2], -1)
+        assert t == table.data_ptr() and ldt >= width == 5 and seqs == 1
+
+
 # ------------------------------------------------------------------------------------------------------------------ references
 def gen_of(*key):
     import zlib
@@ -488,3 +516,18 @@ def test_a_cache_whose_codes_pass_32_bits():
     for q, s in ((x[:, :16].clone(), starts), (x[:2, :16].clone(), ints([0, 1, 2]))):
         want = kv8.attention(q, few, ints(list(range(6))).reshape(2, 3), lens, s)
         assert torch.equal(kv8.attention(q, big, ints(pages).reshape(2, 3), lens, s, out=q), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(4))
+def test_calls_with_tables_whose_rows_repeat_or_overlap_are_refused(which):
+    from crane_b200 import kv8
+    cache, x = kv8.pages(20, 2, 64, 16), torch.ones((4, 2, 64), device="cuda")
+    table, lens, starts = repeating_tables("cuda")[which], ints([3] * 4), ints([0, 1, 2, 3, 4])
+    with pytest.raises(CraneB200Error, match="apart"):
+        kv8.append(x, x, cache, table, lens, starts)
+    with pytest.raises(CraneB200Error, match="apart"):
+        kv8.attention(x, cache, table, lens, starts)
+    assert all(int(c.view(torch.uint8).count_nonzero()) == 0 for c in cache[:2])
+    out = kv8.attention(x, cache, table.contiguous(), lens, starts)     # the same pages for each, in rows of their own
+    assert (out == 0).all()
