@@ -7,7 +7,7 @@
 // once, where it is small for the weights that count.
 //
 // Bound by bytes where there are few rows: a lane reads fragments of codes as they lie in shared memory (TMA, swizzled), two conversions for four codes, no transposition: 64 sequences of up
-// to 8192 positions, 32 heads over 8, 128 columns: 529 MB in 110 us, 4.8 TB/s (of 6.46 measured); issue slots 38 %, eight warps an SM that wait for one another's latencies.
+// to 8192 positions, 32 heads over 8, 128 columns: 529 MB in 113 us, 4.7 TB/s (of 6.46 measured); issue slots 38 %, eight warps an SM that wait for one another's latencies.
 // By what it gave there: 16 positions a warp at a time 182, 32 of two tiles 145, a warp that brings the queries a unit ahead 129, four steps of a unit's own in the deal 113.
 // Many rows (f32, or 256 columns) are bound by mma.sync: 44 % of its cycles, 16 or 32 rows beside conversions that every warp makes for itself.
 #include <cuda_fp16.h>
@@ -424,15 +424,18 @@ small_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                         if constexpr (St::BOX == 128) lds16(vb + piece<128>(r, col8(g)), x[i]);
                         else lds8(vb + piece<64>(r, g >> 1) + (g & 1) * 8, x[i]);
                     }
-                    if (edge) {                              // a NaN among values that not all rows see: 0 * NaN must not reach the others; those that see it look it up
+                    if (edge) {                              // a NaN among values that some row does not see: 0 * NaN must not reach that one; those that see it look it up
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 4; ++i) {
+                            const bool page = sc[k].w != 0.f;
+                            if (page && pos0[k] + pos8<D>(2 * t + (i & 1)) + (i >> 1) * 8 <= wmin) continue;      // (all see it: it stays)
 #pragma unroll
                             for (int w = 0; w < W; ++w) {
                                 const uint32_t n = (((x[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                                odd |= n;
+                                if (page) odd |= n;
                                 x[i][w] &= ~(n * 255u);
                             }
+                        }
                     }
 #pragma unroll
                     for (int w = 0; w < W; ++w)

@@ -531,3 +531,68 @@ def test_calls_with_tables_whose_rows_repeat_or_overlap_are_refused(which):
     assert all(int(c.view(torch.uint8).count_nonzero()) == 0 for c in cache[:2])
     out = kv8.attention(x, cache, table.contiguous(), lens, starts)     # the same pages for each, in rows of their own
     assert (out == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("dim, page", [(64, 16), (128, 64), (128, 16), (256, 32)])
+@pytest.mark.parametrize("new", [1, 4, 9, 90])
+def test_a_nan_among_the_values_reaches_every_row_that_sees_it(new, dim, page, dt):
+    """At the newest position, the ones ahead of it, the first, in the middle, beside missing pages; sequences of odd and even numbers of tiles.  Each has one, in a column and head of its own."""
+    lens, at = [], []
+    for t in (new, new + 1, 64, 65, 100, 130, 200, 500):
+        if t >= new:
+            for pos in {t - 1, t - 2, t - new - 1, t - new, t // 2, 31, 0}:
+                if 0 <= pos < t:
+                    lens.append(t)
+                    at.append(pos)
+    lens = lens + lens
+    q, c, table, lens, starts = problem(gen_of("seen", new, dim, page, dt), dt, 4, 2, dim, page, lens, [new] * len(lens))
+    for b, pos in enumerate(at + at):
+        c[1].view(torch.uint8)[table[b][pos // page], b & 1, pos % page, (37 * b) % dim] = 0x7f if b & 2 else 0xff
+        if b >= len(at):                                                # the pages on either side of it are not there
+            for i in (pos // page - 1, pos // page + 1):
+                if 0 <= i < len(table[b]):
+                    table[b][i] = -1
+    p = (q, c, table, lens, starts)
+    ref = attend_ref(*p, dim ** -0.5)
+    assert torch.isnan(ref[0]).any(2).any(1).sum() >= len(lens)
+    for hint in (0, new):
+        check(run_attention(p, max_rows=hint), ref)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("dim, page", [(64, 32), (128, 16), (256, 16)])
+def test_no_nan_of_a_long_history_is_lost(dim, page, dt):
+    """However the steps are dealt out: page i of every sequence has one in column i alone."""
+    new = [1, 3, 1, 70]
+    q, c, table, lens, starts = p = problem(gen_of("history", dim, page, dt), dt, 2, 1, dim, page, [5000, 1777, 900, 2500], new)
+    for row, n, t in zip(table, new, lens):
+        for i in range(min(dim, (t - n) // page)):
+            c[1].view(torch.uint8)[row[i], 0, (7 * i) % page, i] = 0x7f
+    ref = attend_ref(*p, dim ** -0.5)
+    check(run_attention(p), ref)
+    check(run_attention((q[:5], c, table[:3], lens[:3], starts[:4]), max_rows=3), (ref[0][:5], ref[1][:5]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_an_infinity_among_the_new_rows_is_seen(dt):
+    """Rows into the cache make a NaN of it; the rows that see the position get it, in its column."""
+    from crane_b200 import kv8
+    cache = kv8.pages(6, 1, 128, 64)
+    table, lens, starts = ints([[3, 1], [0, 5]]), ints([70, 65]), ints([0, 70, 135])
+    x = torch.randn((135, 1, 128), generator=gen_of("new inf", dt), device="cuda").to(TYPES[dt])
+    kv8.append(x, x, cache, table, lens, starts)
+    for n, col in ((71, 5), (72, 9)):
+        y = torch.ones((2, 1, 128), dtype=TYPES[dt], device="cuda")
+        v = y.clone()
+        v[0, 0, col], v[1, 0, col + 1] = math.inf, math.nan
+        lens.copy_(ints([n, n - 5]))
+        kv8.append(y, v, cache, table, lens, ints([0, 1, 2]))
+        out = kv8.attention(y, cache, table, lens, ints([0, 1, 2]))
+        want = torch.zeros((2, 128), dtype=torch.bool, device="cuda")
+        for first in range(5, col + 1, 4):
+            want[0, first], want[1, first + 1] = True, True
+        assert torch.equal(torch.isnan(out[:, 0]), want)
