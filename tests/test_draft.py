@@ -286,3 +286,107 @@ def test_tokens_come_out_as_the_target_draws_them():
     p = softmax(x, 1.0)
     count = torch.bincount(first.long(), minlength=v).double()
     assert bool(((count - n * p).abs() <= 5 * torch.sqrt(n * p * (1 - p)) + 1).all())
+
+
+# ------------------------------------------------------------------------------------------------------------------ borders: sums that matter are those of 64 bits
+# Sums of 64-bit terms are off by 2^-40 at most (terms 2^-51, up to 2^28 of them in any order); f32 uniforms near a border are chosen farther from it than that.
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("v", [1, 2, 127, 1001, 4099, 32003, 151937])
+def test_equal_rows_hold_whatever_u_below_one_and_wherever_they_lie(v, dt):
+    """Draft rows are the target's at every other boundary: u q < p for the largest u below 1; not for u = 1.  Behind a refused one p - q is zero everywhere: the race is over p."""
+    from crane_b200 import draft
+    g = gen_of("equal rows", v, dt)
+    n, seqs = 8, 4
+    x = (torch.randn((n * seqs + seqs, v), generator=g, device="cuda") * 3).to(TYPES[dt])
+    at = [i + i // n for i in range(n * seqs)]
+    wide = torch.zeros((n * seqs, v + 9), dtype=TYPES[dt], device="cuda")
+    starts = ints([i * n for i in range(seqs + 1)])
+    tokens = torch.randint(0, v, (n * seqs,), generator=g, device="cuda").to(torch.int32)
+    noise = torch.rand((seqs, v), generator=g, device="cuda").clamp(1e-7, 0.999)
+    temps = [1.0, 0.7, 0.3, 3.0]
+    for off in range(8):
+        q = wide[:, off:off + v]
+        q.copy_(x[at])
+        u = torch.full((n * seqs,), 1 - 2.0 ** -24, device="cuda")
+        a, f = draft.verify(x, tokens, starts, u, noise, draft_logits=q, temperatures=torch.tensor(temps, device="cuda"))
+        p = [softmax(x[b * (n + 1) + n], float(torch.tensor(temps[b]))) for b in range(seqs)]
+        alive = [int(j) for j in a]
+        for b in range(seqs):                                           # (a token so unlikely that its probability is 0 is not accepted)
+            none = [j for j in range(n) if float(softmax(x[b * (n + 1) + j], float(torch.tensor(temps[b])))[int(tokens[b * n + j])]) == 0]
+            assert alive[b] == (none[0] if none else n)
+            if not none:
+                assert int(f[b]) == int((p[b] / -torch.log(noise[b].double())).argmax())
+        u[3::n] = 1.0
+        a, f = draft.verify(x, tokens, starts, u, noise, draft_logits=q, temperatures=torch.tensor(temps, device="cuda"))
+        for b in range(seqs):
+            assert int(a[b]) <= 3
+            if int(a[b]) == 3:
+                assert int(f[b]) == int((softmax(x[b * (n + 1) + 3], float(torch.tensor(temps[b]))) / -torch.log(noise[b].double())).argmax())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_q", [True, False])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("v", [5, 1001, 32000, 151937])
+def test_uniforms_next_to_the_border(v, dt, with_q):
+    """u is the f32 number just below p / q, or at most two steps above it: 2^-24 of itself away from the border where the sums are of 2^-20."""
+    g = gen_of("border", v, dt)
+    for t in (1.0, 0.6, 2.0):
+        logits, tokens, starts, uniforms, noise, q, temps = problem(g, dt, [5] * 12, v, near=1.0, temps=[t] * 12)
+        t32 = float(torch.tensor(t))
+        seq = [i // 5 for i in range(60)]
+        for i in range(60):
+            p, y = softmax(logits[i + seq[i]], t32), softmax(q[i], t32) if with_q else None
+            ratio = (p / y) if with_q else p
+            ok = torch.nonzero((ratio < 0.9) & (ratio > 1e-30))[:, 0]
+            if not len(ok):
+                uniforms[i] = 0.0
+                continue
+            tokens[i] = int(ok[int(torch.randint(0, len(ok), (1,), generator=g, device="cuda"))])
+            border = float(ratio[tokens[i]])
+            u = torch.tensor(border, dtype=torch.float32)
+            below = u if float(u) < border * (1 - 2.0 ** -40) else torch.nextafter(u, torch.tensor(0.0))
+            if float(below) >= border * (1 - 2.0 ** -40):
+                below = torch.nextafter(below, torch.tensor(0.0))
+            above = u if float(u) > border * (1 + 2.0 ** -40) else torch.nextafter(u, torch.tensor(1.0))
+            uniforms[i] = above if i % 5 == 4 and seq[i] % 2 or i % 5 == seq[i] % 5 and seq[i] % 3 == 0 else below
+        accepted, following, _ = rule(logits, tokens, starts, uniforms, noise, q if with_q else None, [t32] * 12)
+        assert run((logits, tokens, starts, uniforms, noise, q, temps), with_q) == (accepted, following)
+        assert len(set(accepted)) > 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_races_between_keys_next_to_one_another(dt):
+    """p - q is a small part of p, a hundredth at one place, a thousandth at another, so that sums of 2^-20 would turn the order of their keys round: those are next to one another in 64 bits."""
+    from crane_b200 import draft
+    for v in (300, 5003, 151937):
+        g = gen_of("race", v, dt)
+        seqs = 16
+        logits = torch.randn((2 * seqs, v), generator=g, device="cuda")
+        q = (logits[0::2] + 0.01 * torch.randn((seqs, v), generator=g, device="cuda")).to(TYPES[dt])
+        logits = logits.to(TYPES[dt])
+        noise = torch.full((seqs, v), 1e-30, device="cuda")             # (a clock of 69 everywhere else)
+        want = []
+        for b in range(seqs):
+            size = softmax(logits[2 * b], 1.0)
+            w = (size - softmax(q[b], 1.0)).clamp_min(0)
+            i, j = int(w.argmax()), int((w * (w < 0.1 * w.max()) * (w < 0.002 * size)).argmax())
+            assert w[j] > 0 and float(w[j]) * 69 / 0.01 > 4 * float(w[i])
+            noise[b, j] = 0.99
+            key = float(w[j]) / -math.log(float(noise[b, j]))
+            u = torch.tensor(math.exp(-float(w[i]) / key), dtype=torch.float32)      # i's key beside j's: the f32 number of the wanted side that is nearest
+            for _ in range(4):
+                over = float(w[i]) / -math.log(float(u)) / key - 1
+                if over > 2.0 ** -36 if b % 2 else over < -2.0 ** -36:
+                    break
+                u = torch.nextafter(u, torch.tensor(1.0 if b % 2 else 0.0))
+            noise[b, i] = u
+            keys = w / -torch.log(noise[b].double().clamp(2.0 ** -126, 1 - 2.0 ** -24))
+            want.append(int(keys.argmax()))
+            top = torch.topk(keys, 2)
+            assert set(top.indices.tolist()) == {i, j} and float(top.values[1]) < float(top.values[0]) * (1 - 2.0 ** -36)
+        tokens = torch.tensor([int((softmax(q[b], 1.0) - softmax(logits[2 * b], 1.0)).argmax()) for b in range(seqs)], dtype=torch.int32, device="cuda")
+        a, f = draft.verify(logits, tokens, ints(list(range(seqs + 1))), torch.ones(seqs, device="cuda"), noise, draft_logits=q)
+        assert a.tolist() == [0] * seqs and f.tolist() == want
