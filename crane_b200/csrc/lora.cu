@@ -12,6 +12,8 @@
 // one behind the other (leaving any one out saves its 70): eight warps in step, which is why lora_tiles.cu has these.  Without the ring 570.  One row 5.6, 33 rows of 20 adapters, f32, 25.6 (36 MB: 5.6).
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "lora.cuh"
 #include "tc.cuh"
 
@@ -250,7 +252,7 @@ lora_kernel(Lora l, bool gather, int slots) {
         if constexpr (ROWS > 32) mine |= (unsigned long long)__ballot_sync(0xffffffffu, which_s[(lane + 32) % ROWS] == w) << 32;
         mine &= left;
         left &= ~mine;
-        if (turn++ < slot || (slot + 1 < slots && turn - 1 > slot)) continue;      // another cluster's adapter
+        if (turn++ % slots != slot) continue;                        // another cluster's adapter
         const W* B = reinterpret_cast<const W*>(l.b) + (size_t)max(w, 0) * l.n * l.rank;
         // ---- the ring: a thread fetches the same piece of every AR-th row of add and of every BR-th row of B, whatever the step ----
         constexpr bool STAGED = VEC && S::STAGES > 0;
@@ -560,8 +562,8 @@ int launch(cudaStream_t st, const Lora& l, bool gather, int cluster, bool pdl) {
     auto kernel = lora_kernel<X, W, MT, RT, VEC>;
     if (const int e = ensure_dyn_smem(kernel, (size_t)S::SMEM, seen)) return e;
     const int tiles = gather ? l.m : (l.m + S::ROWS - 1) / S::ROWS;
-    // A tile of neighbours may hold several adapters: the first few have a cluster each, the last one the rest
-    const int slots = gather ? 1 : tiles >= 75 ? 2 : tiles <= 9 ? 16 : 150 / tiles;
+    // A tile of neighbours may hold several adapters: they are dealt out in turn to as many clusters as give every SM a CTA, two at least
+    const int slots = gather ? 1 : std::min(l.adapters + 1, std::min(16, std::max(2, tc_device_sms() / tiles)));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tiles * cluster * slots); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = S::SMEM; cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -606,9 +608,11 @@ int lora_linear_launch(cudaStream_t st, const Lora& l, bool pdl) {
         if (l.w_type == LORA_BF16) return launch_types<float, bf16>(st, l, vec, pdl);
         if (l.w_type == LORA_F16) return launch_types<float, __half>(st, l, vec, pdl);
     } else if (l.type == l.w_type) {
-        // Us, bf16, here / in tiles of 128 rows, rows of 1, 6 and 40 adapters.  2048 -> 2048, rank 64: 1200 rows 29, 30, 49 / 34, 39, 55; 2500 rows 46, 49, 57 / 38, 40, 68; 9400 rows 132, 136,
-        // 140 / 55, 56, 66.  4096 -> 12 288: 2500 rows, rank 64, 119, 122, 132 / 79, 79, 152, rank 32, 95, 96, 110 / 69, 68, 136, rank 16, 61, 63, 70 / 64, 63, 126; 9400 rows, rank 32,
-        // 247, 247, 272 / 195, 211, 224.
+        // Us, bf16, here / in tiles of 128 rows, neighbours of 1, 6, 40 and 64 adapters, then 6 and 40 in any order.  2048 -> 2048, rank 64: 2048 rows 36, 43, 63, 76, 156, 712 / 37, 38, 70, 101,
+        // 113, 568; 9400 rows 131, 135, 163, 182, 645, 3162 / 54, 56, 69, 70, 205, 1122.  4096 -> 12 288, rank 64: 2048 rows 75, 113, 160, 174, 333, 1497 / 76, 77, 129, 199, 224, 1020; rank 32:
+        // 66, 91, 124, 137, 247, 973 / 66, 65, 108, 150, 183, 787; 9400 rows 244, 247, 286, 317, 967, 4301 / 178, 206, 200, 199, 607, 3233.  Neighbours of adapters that have less than half a
+        // tile of rows each lose a third at most; how many of the adapters rows go through only the device knows.  1200 rows, 2048 -> 2048, of 1, 6 and 40: 29, 30, 49 / 34, 39, 55.  Rank 16,
+        // 4096 -> 12 288, 2500 rows: 61, 63, 70 / 64, 63, 126.
         if (vec && l.m >= 2048 && l.rank > 16 && l.rank <= 64) return lora_tiles_launch(st, l, pdl);
         if (l.type == LORA_BF16) return launch_types<bf16, bf16>(st, l, vec, pdl);
         if (l.type == LORA_F16) return launch_types<__half, __half>(st, l, vec, pdl);

@@ -8,6 +8,8 @@
 // X A^T by mma.sync from global memory, by 8, 337; lora.cu 401.
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "lora.cuh"
 #include "tc.cuh"
 
@@ -85,7 +87,7 @@ lora_tile_kernel(Lora l, int slots) {
     for (int word = 0; word < 4; ++word)
     for (unsigned leads = lead_s[word]; leads; leads &= leads - 1) {
         // ---- the next adapter among the rows ----
-        if (turn++ < slot || (slot + 1 < slots && turn - 1 > slot)) continue;      // another cluster's
+        if (turn++ % slots != slot) continue;                        // another cluster's
         const int w = which_s[word * 32 + __ffs(leads) - 1];
         if (w < 0) {                                                 // none: add goes through
             if (l.add != l.out)
@@ -288,7 +290,7 @@ int launch(cudaStream_t st, const Lora& l, bool pdl) {
     const int tiles = (l.m + ROWS - 1) / ROWS;
     int cluster = 8;                                                 // (a power of two: what the sums' loads are counted by)
     while (cluster > 1 && tiles * cluster > 2 * tc_device_sms()) cluster /= 2;
-    const int slots = tiles >= 37 ? 2 : 74 / tiles;      // the first few adapters of a tile have a cluster each, the last one the rest
+    const int slots = std::min(l.adapters + 1, std::max(2, tc_device_sms() / 2 / tiles));      // a tile's adapters are dealt out in turn to so many clusters
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)tiles * cluster * slots); cfg.blockDim = dim3(THREADS); cfg.dynamicSmemBytes = SMEM; cfg.stream = st;
     cudaLaunchAttribute attr[2];

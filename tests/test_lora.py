@@ -181,6 +181,25 @@ def test_adapters_of_prompts(size, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt, wt", [("bf16", "bf16"), ("f16", "f16"), ("f32", "f32")])
+@pytest.mark.parametrize("size", [(390, 72, 64, 8, 300), (640, 136, 96, 32, 64), (2048, 136, 72, 24, 200), (2500, 264, 64, 64, 1), (3000, 72, 128, 40, 127), (5000, 72, 64, 64, 500)],
+                         ids=lambda s: "-".join(map(str, s)))
+def test_adapters_in_any_order_are_dealt_out_to_the_clusters_of_a_tile(size, dt, wt):
+    """Up to as many adapters as a tile has rows, more and fewer than it has clusters, rows without one among them: every row once, the same bits as by itself among its own."""
+    from crane_b200 import lora
+    m, n, k, rank, adapters = size
+    x, a, b, which, scales, add = problem(gen_of("dealt", size, dt), dt, wt, m, n, k, rank, adapters, "any")
+    y = add.clone()
+    lora.linear(x, a, b, which, scales=scales, add=y, out=y)
+    check(y, reference(x, a, b, which, scales, add))
+    assert torch.equal(lora.linear(x, a, b, which, scales=scales, add=add), y)
+    some = int(which[m // 2])
+    alone = torch.where(which == some, which, -1)                       # the others have none now
+    z = lora.linear(x, a, b, alone, scales=scales, add=add)
+    assert torch.equal(z[which == some], y[which == some]) and torch.equal(z[which != some], add[which != some])
+
+
+@pytest.mark.gpu
 def test_prompts_repeat_in_graphs_and_on_streams():
     from crane_b200 import lora
     x, a, b, which, scales, add = problem(gen_of("tiles repeat"), "bf16", "bf16", 2300, 1032, 1024, 64, 5, "runs")
