@@ -634,7 +634,10 @@ join_kernel(Args a) {
     }
 }
 
-// Rows of a kv head from which on a sequence goes through kv8_flash.cu: 16-bit ones of 64 and 128 columns.
+// Rows of a kv head from which on a sequence goes through kv8_flash.cu: 16-bit ones of 64 and 128 columns.  Us, here / there, 32 heads over 8 of 128, bf16, sequences that bring 96, 128, 256 and
+// 512 rows of a kv head.  Eight with nothing ahead of them: 24, 23, 30, 51 / 50, 50, 51, 55; behind 1000 positions: 37, 44, 68, 120 / 58, 61, 62, 81; behind 8000: 139, 177, 333, 645 / 119,
+// 119, 121, 192; 16 behind 8000: 255, 332, 640, 1262 / 186, 186, 191, 327; one: 39, 44, 59, 100 / 56, 58, 62, 75.  Its launches cost 20 us where there is little to do, rows here cost 70 where
+// there is much from the first group of 32 behind the 64th row on; the lengths, which tell, are on the device only.
 constexpr int FLASH_FROM = 65;
 bool flash_takes(int type, int dim, int group, int max_rows) { return type != KV8_F32 && dim <= 128 && (long long)group * max_rows >= FLASH_FROM; }
 // Rows of a group of queries: 16, or 32 where some sequence may bring many and none goes to kv8_flash.cu.  Us, 16 / 32 / 64 rows: portions of 500 tokens, 16 heads over 8, f32 231 / 177 /
