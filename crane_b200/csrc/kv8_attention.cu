@@ -7,7 +7,7 @@
 // once, where it is small for the weights that count.
 //
 // Bound by bytes where there are few rows: a lane reads fragments of codes as they lie in shared memory (TMA, swizzled), two conversions for four codes, no transposition: 64 sequences of up
-// to 8192 positions, 32 heads over 8, 128 columns: 529 MB in 113 us, 4.7 TB/s (of 6.46 measured); issue slots 38 %, eight warps an SM that wait for one another's latencies.
+// to 8192 positions, 32 heads over 8, 128 columns: 529 MB in 113 us, 4.7 TB/s (of 6.46 measured); issue slots 36 %, eight warps an SM that wait for one another's latencies.
 // By what it gave there: 16 positions a warp at a time 182, 32 of two tiles 145, a warp that brings the queries a unit ahead 129, four steps of a unit's own in the deal 113.
 // Many rows (f32, or 256 columns) are bound by mma.sync: 44 % of its cycles, 16 or 32 rows beside conversions that every warp makes for itself.
 #include <cuda_fp16.h>

@@ -18,7 +18,7 @@ def linear(x, a, b, which, *, scales=None, add=None, out=None):
     """out[i] = add[i] + scales[w] * (x[i] @ a[w].T) @ b[w].T, w = which[i].
 
     x [m, k] f32, bf16 or f16; a [adapters, rank, k] and b [adapters, n, rank], contiguous, of x's type or, beside f32 rows, any of the three; rank up to 128; which [m] int32;
-    scales [adapters] f32 (None: ones); add [m, n] (None: zeros; may be out) and out of x's type."""
+    scales [adapters] f32 (None: ones); add [m, n] (None: zeros; may be out) and out of x's type.  An infinity of x or of an adapter becomes an infinity or a NaN of the results that it reaches."""
     dev, m, k, ldx, dtype = _rows_in("x", x)
     for what, w in (("a", a), ("b", b)):
         if not isinstance(w, torch.Tensor) or w.dim() != 3 or w.dtype not in _DTYPES or w.get_device() != dev or not w.is_contiguous():

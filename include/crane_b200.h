@@ -361,9 +361,10 @@ CRANE_B200_API int crane_b200_fp8_status(int device, void* stream);
 CRANE_B200_API const char* crane_b200_device_last_error(void);
 /* A cache: codes of keys and values [pages, kv_heads, page, dim] e4m3, scales [pages, kv_heads, 2] f32 (a page and head's for keys, for values); value = code * scale.  page 16, 32,
  * 64 or 128; dim 64, 128 or 256.  Sequence b holds lens[b] positions, position i on page table[b * ldt + i / page]; its new rows are rows starts[b] .. starts[b + 1] - 1 (starts
- * ascends, [seqs + 1]) and have its last positions.  Positions behind `width` pages, on pages outside [0, pages) or below 0 hold nothing.
+ * ascends, [seqs + 1]) and have its last positions.  Positions behind `width` pages, on pages outside [0, pages) or below 0 hold nothing.  ldt is
+ * not below width: each sequence has a row of the table to itself.
  *
- * Rows k, v [rows, kv_heads, dim] (rows ldk, heads ldkh elements apart; values likewise) into their pages.  A page and head's scale is the smallest power of two 2^e with
+ * Rows k, v [rows, kv_heads, dim] (rows ldk, heads ldkh elements apart, dim at least; values likewise) into their pages.  A page and head's scale is the smallest power of two 2^e with
  * max |y| <= 448 * 2^e (max |y| counts as 2^-100 at least) over the rows written since its first position was; code = e4m3(y / 2^e), to nearest even.  A page that goes on takes
  * the larger of its own scale and its new rows', its codes ahead of them rescaled; codes behind the last row stay as they are.  NaN stays NaN, infinities become NaN.
  * Sequences may share pages that none of them writes in this call. */
@@ -372,7 +373,8 @@ CRANE_B200_API int crane_b200_kv8_append(int device, const void* k, size_t ldk, 
                                          const int32_t* starts, size_t seqs, size_t rows, void* stream);
 /* out[i, h] = sum over the positions p <= that of row i of softmax(scale * q[i, h] . k_p) v_p, kv head h / (heads / kv_heads); q and out [rows, heads, dim] of one type.  Sums in f32,
  * weights in f16 (f32 rows: two f16 parts), rounded once to out's type; bf16 queries of a sequence that brings more than 64 rows of a kv head keep 2^-17 of a row's largest element.  Rows that see nothing give zeros; rows behind starts[seqs] are left as they are.  Scales are
- * positive.  max_rows: the most rows that a sequence brings (0: not known); more than that only take longer.  crane_b200_fp8_status tells of a bounded wait that ran out. */
+ * positive.  max_rows: the most rows that a sequence brings (0: not known, `rows` stands for it); more than that only take longer.  Where heads / kv_heads * max_rows is above 64, 16-bit calls of 64
+ * and 128 columns launch the kernels for long portions beside those for few rows (four instead of two) and want work for them (39 MB at 128 columns).  out may be q.  crane_b200_fp8_status tells of a bounded wait that ran out. */
 CRANE_B200_API int crane_b200_kv8_attention_bytes(int device, int dtype, size_t heads, size_t kv_heads, size_t dim, size_t seqs, size_t rows, size_t max_rows, size_t* bytes);
 CRANE_B200_API int crane_b200_kv8_attention(int device, const void* q, size_t ldq, size_t ldqh, void* out, size_t ldo, size_t ldoh, int dtype, size_t heads, float scale,
                                             const uint8_t* k_codes, const uint8_t* v_codes, const float* scales, size_t pages, size_t kv_heads, size_t page, size_t dim,
@@ -380,15 +382,16 @@ CRANE_B200_API int crane_b200_kv8_attention(int device, const void* q, size_t ld
                                             void* work, size_t work_bytes, void* stream);
 /* out[i, :] = add[i, :] + scales[w] * B_w (A_w x[i, :]), w = which[i]; rows whose w is outside [0, adapters) have none: out = add.  x [m, k], add (NULL: zeros; may be out) and out
  * [m, n] of one type, a [adapters, rank, k] and b [adapters, n, rank] contiguous, of that type too or, beside f32 rows, of any; scales [adapters] (NULL: ones).  rank 1 to 128.
- * Sums in f32, rounded once.  Any order of `which` is right; beyond 384 rows neighbours of one adapter are fastest.
+ * Sums in f32, rounded once; an infinity of x or of an adapter becomes an infinity or a NaN of the results that it reaches.  Any order of `which` is right; beyond 384 rows neighbours of one
+ * adapter are fastest: a tile of 64 or 128 rows goes through each adapter that it holds.
  * crane_b200_fp8_status tells of a bounded wait that ran out. */
 CRANE_B200_API int crane_b200_lora_linear(int device, const void* x, size_t ldx, int dtype, const void* a, const void* b, int w_dtype, size_t adapters, size_t rank,
                                           const int32_t* which, const float* scales, const void* add, size_t ldadd, void* out, size_t ldo, size_t m, size_t n, size_t k, void* stream);
 /* Drafted tokens against the target's probabilities.  Sequence b has the drafts starts[b] .. starts[b + 1] - 1 of `tokens` [drafts] (starts ascends from 0, [seqs + 1]) and the logits
  * rows starts[b] + b .. starts[b + 1] + b of [drafts + seqs, vocab]: one ahead of each draft, one behind the last.  p and q: softmax of a row / temperature of the target's and the draft
  * model's logits ([drafts, vocab]; NULL: q is 1 at the draft).  accepted[b]: drafts ahead of the first with u q(d) >= p(d), u = uniforms[j]; next[b]: the token behind those, the first
- * argmax of w / -log(noise[b, :]) with w = max(p - q, 0) there (p where that is 0 everywhere), or p behind the last draft.  temperatures [seqs] (NULL: 1): 0 accepts the first
- * maximum only, which is next otherwise.  A NaN logit counts as -inf; infinite ones share a row's probability; a row of -inf accepts nothing and gives -1; a draft outside the
+ * argmax of w / -log(noise[b, :]) with w = max(p - q, 0) there (p where that is 0 everywhere), or p behind the last draft.  temperatures [seqs] (NULL: 1): 0, less or NaN
+ * accepts the first maximum only, which is next otherwise.  Both are decided as in 64 bits.  A NaN logit counts as -inf; infinite ones share a row's probability; a row of -inf accepts nothing and gives -1; a draft outside the
  * vocabulary is not accepted.  Noise lies between 0 and 1. */
 CRANE_B200_API int crane_b200_draft_verify_bytes(int device, size_t vocab, size_t seqs, size_t drafts, int with_draft_logits, size_t* bytes);
 CRANE_B200_API int crane_b200_draft_verify(int device, const void* logits, size_t ld, const void* draft_logits, size_t ldd, int dtype, size_t vocab, const int32_t* tokens,

@@ -596,3 +596,15 @@ def test_an_infinity_among_the_new_rows_is_seen(dt):
         for first in range(5, col + 1, 4):
             want[0, first], want[1, first + 1] = True, True
         assert torch.equal(torch.isnan(out[:, 0]), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_results_may_take_the_place_of_the_queries(dim, dt):
+    """Units that one CTA has and units that several share, few rows and many beside one another."""
+    for new in ([1, 1, 3, 1], [1, 300, 5, 40], [700, 1, 1, 90]):
+        q, c, table, lens, starts = problem(gen_of("in place", dim, dt, new), dt, 8, 2, dim, 64, [3000, 1400, 70, 900], new)
+        want = run_attention((q, c, table, lens, starts))
+        x = q.clone()
+        assert run_attention((x, c, table, lens, starts), out=x) is x and torch.equal(x, want)
