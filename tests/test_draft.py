@@ -390,3 +390,32 @@ def test_races_between_keys_next_to_one_another(dt):
         tokens = torch.tensor([int((softmax(q[b], 1.0) - softmax(logits[2 * b], 1.0)).argmax()) for b in range(seqs)], dtype=torch.int32, device="cuda")
         a, f = draft.verify(logits, tokens, ints(list(range(seqs + 1))), torch.ones(seqs, device="cuda"), noise, draft_logits=q)
         assert a.tolist() == [0] * seqs and f.tolist() == want
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+def test_many_drafts_next_to_the_border_in_a_replayed_graph(dt):
+    """More drafts than a block has warps or keeps sums of, every one too close to call by f32 sums; sequences of few beside them; the refused ones change between replays."""
+    from crane_b200 import draft
+    g = gen_of("many border", dt)
+    counts, v = [70, 3, 0, 40], 777
+    starts = [0, 70, 73, 73, 113]
+    x = (torch.randn((117, v), generator=g, device="cuda") * 2).to(TYPES[dt])
+    at = [i + b for b in range(4) for i in range(starts[b], starts[b + 1])]
+    wide = torch.zeros((113, v + 3), dtype=TYPES[dt], device="cuda")
+    q = wide[:, 1:v + 1].copy_(x[at])
+    tokens = [int(t) for t in torch.randint(0, v, (113,), generator=g, device="cuda")]
+    noise = torch.rand((4, v), generator=g, device="cuda").clamp(1e-7, 0.999)
+    u = torch.full((113,), 1 - 2.0 ** -24, device="cuda")
+    t, s = ints(tokens), ints(starts)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, f = draft.verify(x, t, s, u, noise, draft_logits=q)
+    for refused in ([], [50, 112], [0, 71, 73], [69, 72, 107]):
+        u.fill_(1 - 2.0 ** -24)
+        u[refused] = 1.0
+        graph.replay()
+        want = [min([i - starts[b] for i in refused if starts[b] <= i < starts[b + 1]], default=counts[b]) for b in range(4)]
+        assert a.tolist() == want
+        for b in range(4):                                              # p - q is zero everywhere: the race is over p
+            assert int(f[b]) == int((softmax(x[starts[b] + b + want[b]], 1.0) / -torch.log(noise[b].double())).argmax())
