@@ -608,3 +608,23 @@ def test_results_may_take_the_place_of_the_queries(dim, dt):
         want = run_attention((q, c, table, lens, starts))
         x = q.clone()
         assert run_attention((x, c, table, lens, starts), out=x) is x and torch.equal(x, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_nan_and_infinities_of_queries_and_keys_among_many_rows(dim, dt):
+    """A query's is its row's, even beside rows that see nothing; a key's reaches the rows that see it, in every column."""
+    q, c, table, lens, starts = problem(gen_of("many rows", dim, dt), dt, 4, 2, dim, 64, [600, 150, 3000, 40], [200, 150, 90, 70], loud=False)
+    clean = q.clone()
+    q[3, 0, 3], q[70, 1, 9], q[199, 2, 0], q[201, 3, dim - 1], q[399, 0, 5], q[440, 1, 1], q[445, 3, 2] = (math.nan, math.inf, -math.inf, math.nan, math.inf, math.nan, math.inf)
+    for b, pos, h in ((0, 450, 0), (1, 149, 1), (2, 2950, 0), (2, 2999, 1)):
+        c[0].view(torch.uint8)[table[b][pos // 64], h, pos % 64, 7] = 0x7f
+    out, tol = attend_ref(clean, c, table, lens, starts, dim ** -0.5)
+    for i in range(440):
+        for h in range(4):
+            if not torch.isfinite(q[i, h]).all():
+                out[i, h] = math.nan
+    got = run_attention((q, c, table, lens, starts))
+    check(got, (out, tol))
+    assert (got[440:470] == 0).all() and torch.isnan(got[399, 0]).all()         # rows ahead of position 0, whatever they hold
